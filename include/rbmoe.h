@@ -4,7 +4,9 @@
  * Drop-in boundary for RustingBrain's `MoeLayer`: the forward pass with the two
  * auxiliary losses (reference src/moe.rs:203-341), the backward pass
  * (src/moe.rs:348-489) and the block's RMSNorm and residual add either side of
- * the layer (src/transformer_block.rs:216-222, 257-263).  The reference
+ * the layer (src/transformer_block.rs:216-222, 257-263); and, on their own, two
+ * operators of a training step around it: a sub-layer joined to the residual
+ * stream, and orthogonalised weight updates.  The reference
  * has no FFI seam for this layer; each entry point below names the reference
  * interface it stands in for, so that a Rust `extern "C"` block can bind them
  * one to one.  Plain pointers and sizes only.  Every function returns an
@@ -312,6 +314,61 @@ int rbmoe_backward_block(rbmoe_layer* layer, const void* grad_output, int32_t to
 /* Same on HOST pointers; synchronises. */
 int rbmoe_backward_block_host(rbmoe_layer* layer, const void* grad_output, int32_t tokens, int32_t cols,
                               void* grad_input);
+
+/* ---- a sub-layer joined to the residual stream ----------------------------------------------------
+ * What stands between a sub-layer's output and the next sub-layer's input, in one call each way: a norm behind the sub-layer,
+ * a gate, a residual scale, the residual add and the next norm.  The reference's block has the add and the norm in front
+ * (src/transformer_block.rs:216-222); with a norm behind, a gate or a scale it has no counterpart.
+ *   b      = RmsNorm(y) * post_weight      (y itself where post_weight is NULL)
+ *   out    = x + scale * gate * b
+ *   normed = RmsNorm(out) * next_weight    (of the rows as they are stored; only with next_weight)
+ * Rows [rows, cols] are of the join's dtype, weights [cols] f32; a gate by channel is [cols] f32, one by row [rows, cols] of the join's
+ * dtype.  All of them DEVICE pointers.  `valid` [rows] bytes or NULL: a padding row (0) takes y as zero, so its `out` is its x; what
+ * lies in its y and gate is not used, and it adds nothing to the gradients of weights and gate.  Statistics and sums are f32, each
+ * output is rounded once.  `out` may be x, `normed` may be y; apart from that outputs must not overlap inputs or one another. */
+typedef enum rbmoe_gate {
+    RBMOE_GATE_NONE = 0,
+    RBMOE_GATE_CHANNEL = 1, /* [cols] f32, a parameter */
+    RBMOE_GATE_ROW = 2      /* [rows, cols] of the rows' dtype */
+} rbmoe_gate;
+typedef struct rbmoe_join rbmoe_join;
+/* Holds the workspace of the backward pass (counted against the context's budget).  1 to 65536 columns. */
+int rbmoe_join_create(rbmoe_ctx* ctx, int32_t cols, int32_t dtype, int32_t gate, rbmoe_join** out);
+void rbmoe_join_destroy(rbmoe_join* join);
+/* Enqueued on the context's stream; allocates nothing. */
+int rbmoe_join_forward(rbmoe_join* join, int32_t rows, const void* x, const void* y, const uint8_t* valid,
+                       const float* post_weight, const void* gate, float scale, const float* next_weight, float eps,
+                       void* out, void* normed);
+/* Gradients of both inputs (grad_x, grad_y, required), and of post_weight, gate and next_weight (each may be NULL).  y, valid, weights,
+ * gate, scale and eps are the forward's, `out` the rows that it wrote (read with next_weight only).  grad_out is what reaches `out`
+ * from elsewhere (NULL: nothing), grad_normed what reaches `normed` (with next_weight).  Gradients of [cols] parameters are
+ * written, or with accumulate != 0 added to what is there; a gate's by row is always written.  A gradient of an input may lie where
+ * grad_out or grad_normed lies.  The same call gives the same bits.  Calls on one join must not overlap in time. */
+int rbmoe_join_backward(rbmoe_join* join, int32_t rows, const void* y, const void* out, const uint8_t* valid,
+                        const float* post_weight, const void* gate, float scale, const float* next_weight, float eps,
+                        const void* grad_out, const void* grad_normed, int32_t accumulate, void* grad_x, void* grad_y,
+                        float* grad_post, void* grad_gate, float* grad_next);
+
+/* ---- orthogonalised weight updates -----------------------------------------------------------------
+ * The reference's optimisers run on the host over Param.grad; this is a step on the device for weight matrices.  A handle
+ * takes a stack of `count` matrices [rows, cols] (row-major, contiguous, at most 16384 a side) and holds the workspace: about 16 bytes an element
+ * and 8 bytes a squared shorter side, counted against the context's budget.
+ * rbmoe_orthogonalize brings the singular values of every matrix near one: X = U / (|U|_F + 1e-7), then `steps` times
+ *   A = X X^T, B = b A + c A A, X = a X + B X,  (a, b, c) = (3.4445, -4.7750, 2.0315)
+ * (five steps: values from 0.003 |U|_F up end in [0.68, 1.21]).  Accuracy is f32's whatever the types of `in` and `out`, each RBMOE_F32 or
+ * RBMOE_BF16; `out` may be `in`.  A matrix of zeros stays one.
+ * rbmoe_muon_step is an optimiser step with it (decoupled weight decay):
+ *   M = momentum_factor M + G,  U = G + momentum_factor M (nesterov != 0) or M,
+ *   W = (1 - lr weight_decay) W - lr update_scale O,  O the orthogonalised U;  update_scale 0 stands for sqrt(max(1, rows / cols)).
+ * M and W are f32 and updated in place.  DEVICE pointers, enqueued on the context's stream, nothing is allocated; the same call
+ * gives the same bits.  Calls on one handle must not overlap in time.  A matrix with infinities or NaN among its gradients ends as NaN,
+ * the others of the stack do not. */
+typedef struct rbmoe_muon rbmoe_muon;
+int rbmoe_muon_create(rbmoe_ctx* ctx, int32_t count, int32_t rows, int32_t cols, rbmoe_muon** out);
+void rbmoe_muon_destroy(rbmoe_muon* muon);
+int rbmoe_orthogonalize(rbmoe_muon* muon, const void* in, int32_t in_dtype, int32_t steps, void* out, int32_t out_dtype);
+int rbmoe_muon_step(rbmoe_muon* muon, const void* grad, int32_t grad_dtype, float* momentum, float* weight, float lr,
+                    float momentum_factor, float weight_decay, float update_scale, int32_t nesterov, int32_t steps);
 
 /* Per-stage timing of one forward with HIP events on the context's stream.
  * `ms` receives RBMOE_NUM_STAGES durations in milliseconds.  Synchronises.

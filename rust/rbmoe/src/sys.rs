@@ -26,6 +26,10 @@ pub const RBMOE_W_SHARED_UP: i32 = 5;
 pub const RBMOE_W_SHARED_DOWN: i32 = 6;
 pub const RBMOE_W_NORM: i32 = 7;
 
+pub const RBMOE_GATE_NONE: i32 = 0;
+pub const RBMOE_GATE_CHANNEL: i32 = 1;
+pub const RBMOE_GATE_ROW: i32 = 2;
+
 pub const RBMOE_OPT_FORCE_GENERIC: i32 = 0;
 pub const RBMOE_OPT_EXPLICIT_GATHER: i32 = 1;
 pub const RBMOE_OPT_GROUP_M: i32 = 2;
@@ -78,6 +82,14 @@ pub struct rbmoe_ctx {
 pub struct rbmoe_layer {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct rbmoe_join {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct rbmoe_muon {
+    _private: [u8; 0],
+}
 
 extern "C" {
     pub fn rbmoe_config_init(cfg: *mut rbmoe_config, d_model: i32, num_experts: i32, experts_per_token: i32,
@@ -102,6 +114,22 @@ extern "C" {
                                 router_bias: *const f32, residual: *const c_void, out: *mut c_void) -> c_int;
     pub fn rbmoe_forward_host(layer: *mut rbmoe_layer, x: *const c_void, tokens: i32, cols: i32, valid: *const u8,
                               router_bias: *const f32, residual: *const c_void, out: *mut c_void) -> c_int;
+    pub fn rbmoe_join_create(ctx: *mut rbmoe_ctx, cols: i32, dtype: i32, gate: i32, out: *mut *mut rbmoe_join) -> c_int;
+    pub fn rbmoe_join_destroy(join: *mut rbmoe_join);
+    pub fn rbmoe_join_forward(join: *mut rbmoe_join, rows: i32, x: *const c_void, y: *const c_void, valid: *const u8,
+                              post_weight: *const f32, gate: *const c_void, scale: f32, next_weight: *const f32, eps: f32,
+                              out: *mut c_void, normed: *mut c_void) -> c_int;
+    pub fn rbmoe_join_backward(join: *mut rbmoe_join, rows: i32, y: *const c_void, out: *const c_void, valid: *const u8,
+                               post_weight: *const f32, gate: *const c_void, scale: f32, next_weight: *const f32, eps: f32,
+                               grad_out: *const c_void, grad_normed: *const c_void, accumulate: i32, grad_x: *mut c_void,
+                               grad_y: *mut c_void, grad_post: *mut f32, grad_gate: *mut c_void, grad_next: *mut f32) -> c_int;
+    pub fn rbmoe_muon_create(ctx: *mut rbmoe_ctx, count: i32, rows: i32, cols: i32, out: *mut *mut rbmoe_muon) -> c_int;
+    pub fn rbmoe_muon_destroy(muon: *mut rbmoe_muon);
+    pub fn rbmoe_orthogonalize(muon: *mut rbmoe_muon, input: *const c_void, in_dtype: i32, steps: i32, out: *mut c_void,
+                               out_dtype: i32) -> c_int;
+    pub fn rbmoe_muon_step(muon: *mut rbmoe_muon, grad: *const c_void, grad_dtype: i32, momentum: *mut f32, weight: *mut f32,
+                           lr: f32, momentum_factor: f32, weight_decay: f32, update_scale: f32, nesterov: i32,
+                           steps: i32) -> c_int;
     pub fn rbmoe_forward_timed(layer: *mut rbmoe_layer, x: *const c_void, tokens: i32, cols: i32, valid: *const u8,
                                router_bias: *const f32, residual: *const c_void, out: *mut c_void,
                                ms: *mut f32) -> c_int;

@@ -1,0 +1,620 @@
+// A sub-layer joined to the residual stream, and its backward pass.
+//
+//   b      = N(y) * post          N(v)_j = v_j / sqrt(mean(v^2) + eps);  y itself without a norm behind the sub-layer
+//   out    = x + scale * g * b
+//   normed = N(out) * next        of the rows as they are stored in `out`, so that it equals a norm of its own behind this call
+//
+// Both directions are bound by memory: a row is read once, kept in registers in 32 bits, and everything that leaves it is
+// written once.  A row belongs to one wave while it is short (no barrier, the sums go through lane permutations) and to a
+// workgroup where it is long; rows beyond what registers hold are read again instead (the *_any kernels).
+// The statistics and every sum are f32.  An output is rounded once, from f32.
+//
+// Backward, D = everything that reaches `out`:  with s = 1 / rms(out), t = 1 / rms(y), u = grad_normed * next
+//   D         = grad_out + s u - out s^3 (out . u) / d
+//   grad_x    = D
+//   grad_gate = scale * D * b             db = scale * g * D              v = db * post
+//   grad_y    = t v - y t^3 (y . v) / d
+//   grad_post = sum_rows db * y * t       grad_next = sum_rows grad_normed * out * s
+// Each of the three parameter gradients is a sum over rows: a wave (or workgroup) takes every n-th row and keeps the sums of
+// its columns in registers; workgroups then leave them in memory and a second, small launch adds them in a fixed order, so
+// the same call gives the same bits.
+#include "join_kernels.h"
+
+#include <algorithm>
+
+namespace rbmoe {
+
+namespace {
+
+// V neighbouring elements of a row.
+template <typename XT, int V>
+struct Piece;
+template <>
+struct Piece<float, 4> {
+    float4 raw;
+    __device__ __forceinline__ void load(const float* p) { raw = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void zero() { raw = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void widen(float (&v)[4]) const { v[0] = raw.x; v[1] = raw.y; v[2] = raw.z; v[3] = raw.w; }
+    static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+};
+template <>
+struct Piece<float, 1> {
+    float raw;
+    __device__ __forceinline__ void load(const float* p) { raw = *p; }
+    __device__ __forceinline__ void zero() { raw = 0.0f; }
+    __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = raw; }
+    static __device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
+};
+template <>
+struct Piece<bf16_t, 8> {
+    uint4 raw;
+    __device__ __forceinline__ void load(const bf16_t* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void widen(float (&v)[8]) const { Vec16<bf16_t>::widen(raw, v); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+    }
+};
+template <>
+struct Piece<bf16_t, 2> {
+    uint32_t raw;
+    __device__ __forceinline__ void load(const bf16_t* p) { raw = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ __forceinline__ void zero() { raw = 0; }
+    __device__ __forceinline__ void widen(float (&v)[2]) const {
+        v[0] = __uint_as_float(raw << 16);
+        v[1] = __uint_as_float(raw & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[2]) { *reinterpret_cast<uint32_t*>(p) = pack2(v[0], v[1]); }
+};
+template <>
+struct Piece<bf16_t, 1> {
+    uint16_t raw;
+    __device__ __forceinline__ void load(const bf16_t* p) { raw = p->bits; }
+    __device__ __forceinline__ void zero() { raw = 0; }
+    __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = bf16_bits_to_f32(raw); }
+    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[1]) { p->bits = f32_to_bf16_bits(v[0]); }
+};
+
+// V values of a parameter [d] (f32)
+template <int V>
+__device__ __forceinline__ void load_parameter(const float* p, float (&v)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            const float4 a = *reinterpret_cast<const float4*>(p + 4 * q);
+            v[4 * q] = a.x; v[4 * q + 1] = a.y; v[4 * q + 2] = a.z; v[4 * q + 3] = a.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = p[i];
+    }
+}
+
+// What the stored row holds for an f32 value.
+template <typename XT>
+__device__ __forceinline__ float as_stored(float v) {
+    if constexpr (sizeof(XT) == 2) return bf16_bits_to_f32(f32_to_bf16_bits(v));
+    return v;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+    return __uint_as_float(group_reduce(__float_as_uint(v), 64, [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+
+// N sums over the G threads of a row, the same in all of them: G is a wave, or the whole workgroup (every thread of which
+// then calls; `room`: 4 N floats that the next call of this function may overwrite at once - two are used in turn).
+template <int G, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float* room) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = wave_sum(s[i]);
+    if constexpr (G > 64) {
+        constexpr int W = G / 64;
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) room[i * W + wave] = s[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float t = room[i * W];
+#pragma unroll
+            for (int w = 1; w < W; ++w) t += room[i * W + w];
+            s[i] = t;
+        }
+    }
+}
+
+__device__ __forceinline__ float inverse_rms(float sum_of_squares, int d, float eps) {
+    return 1.0f / sqrtf(sum_of_squares / (float)d + eps);
+}
+
+// ---- forward -----------------------------------------------------------------------------------
+template <typename XT, int V, int P, int G>
+__global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
+    constexpr int RPB = 256 / G;  // rows of a workgroup
+    __shared__ float room[2][4];
+    const int lane = threadIdx.x % G, d = a.cols;
+    const int row = blockIdx.x * RPB + threadIdx.x / G;
+    if (row >= a.rows) return;  // (a whole wave's rows, or the whole workgroup's)
+    const size_t at = (size_t)row * d;
+    const XT* const x = static_cast<const XT*>(a.x) + at;
+    const XT* const y = static_cast<const XT*>(a.y) + at;
+    const bool live = a.valid == nullptr || a.valid[row] != 0;
+    Piece<XT, V> yr[P], xr[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int c = (p * G + lane) * V;
+        const bool in = c < d;
+        if (in && live) yr[p].load(y + c); else yr[p].zero();
+        if (in) xr[p].load(x + c); else xr[p].zero();
+    }
+    float factor = 1.0f;
+    if (a.post) {
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            float v[V];
+            yr[p].widen(v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] = fmaf(v[i], v[i], s[0]);
+        }
+        row_sums<G>(s, room[0]);
+        factor = inverse_rms(s[0], d, a.eps);
+    }
+    float out[P][V], s2[1] = {0.0f};
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int c = (p * G + lane) * V;
+        float xv[V], b[V];
+        xr[p].widen(xv);
+        yr[p].widen(b);
+        if (c < d) {
+            if (live) {
+                if (a.post) {
+                    float w[V];
+                    load_parameter<V>(a.post + c, w);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) b[i] = b[i] * factor * w[i];
+                }
+                if (a.gate_mode == RBMOE_GATE_CHANNEL) {
+                    float g[V];
+                    load_parameter<V>(static_cast<const float*>(a.gate) + c, g);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) b[i] *= g[i];
+                } else if (a.gate_mode == RBMOE_GATE_ROW) {
+                    Piece<XT, V> gr;
+                    gr.load(static_cast<const XT*>(a.gate) + at + c);
+                    float g[V];
+                    gr.widen(g);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) b[i] *= g[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[p][i] = live ? as_stored<XT>(fmaf(a.scale, b[i], xv[i])) : xv[i];
+            Piece<XT, V>::store(static_cast<XT*>(a.out) + at + c, out[p]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) out[p][i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s2[0] = fmaf(out[p][i], out[p][i], s2[0]);
+    }
+    if (!a.next) return;
+    row_sums<G>(s2, room[1]);
+    const float f2 = inverse_rms(s2[0], d, a.eps);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int c = (p * G + lane) * V;
+        if (c < d) {
+            float w[V];
+            load_parameter<V>(a.next + c, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = out[p][i] * f2 * w[i];
+            Piece<XT, V>::store(static_cast<XT*>(a.normed) + at + c, w);
+        }
+    }
+}
+
+// Rows of any width: a workgroup a row, read again for each step.  A thread reads back only what it wrote itself.
+template <typename XT>
+__global__ __launch_bounds__(256) void join_forward_any_kernel(JoinForward a) {
+    __shared__ float room[2][4];
+    const int d = a.cols, row = blockIdx.x;
+    const size_t at = (size_t)row * d;
+    const XT* const x = static_cast<const XT*>(a.x) + at;
+    const XT* const y = static_cast<const XT*>(a.y) + at;
+    XT* const out = static_cast<XT*>(a.out) + at;
+    const bool live = a.valid == nullptr || a.valid[row] != 0;
+    float factor = 1.0f;
+    if (a.post) {
+        float s[1] = {0.0f};
+        for (int c = threadIdx.x; live && c < d; c += 256) {
+            const float v = to_f32(y[c]);
+            s[0] = fmaf(v, v, s[0]);
+        }
+        row_sums<256>(s, room[0]);
+        factor = inverse_rms(s[0], d, a.eps);
+    }
+    float s2[1] = {0.0f};
+    for (int c = threadIdx.x; c < d; c += 256) {
+        float o = to_f32(x[c]);
+        if (live) {
+            float b = to_f32(y[c]);
+            if (a.post) b = b * factor * a.post[c];
+            if (a.gate_mode == RBMOE_GATE_CHANNEL) b *= static_cast<const float*>(a.gate)[c];
+            else if (a.gate_mode == RBMOE_GATE_ROW) b *= to_f32(static_cast<const XT*>(a.gate)[at + c]);
+            o = as_stored<XT>(fmaf(a.scale, b, o));
+        }
+        out[c] = from_f32<XT>(o);
+        s2[0] = fmaf(o, o, s2[0]);
+    }
+    if (!a.next) return;
+    row_sums<256>(s2, room[1]);
+    const float f2 = inverse_rms(s2[0], d, a.eps);
+    for (int c = threadIdx.x; c < d; c += 256)
+        static_cast<XT*>(a.normed)[at + c] = from_f32<XT>(to_f32(out[c]) * f2 * a.next[c]);
+}
+
+// ---- backward ----------------------------------------------------------------------------------
+// Where the sums over rows go: workgroup b of n leaves its own in partial[b][which][d]; with one workgroup they are final.
+__device__ __forceinline__ float* sum_target(const JoinBackward& a, int which) {
+    return which == 0 ? a.grad_post : which == 1 ? (a.gate_mode == RBMOE_GATE_CHANNEL ? static_cast<float*>(a.grad_gate) : nullptr)
+                                                 : a.grad_next;
+}
+
+template <typename XT, int V, int P, int G>
+__global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
+    constexpr int RPB = 256 / G;
+    __shared__ float room[2][12];
+    const int lane = threadIdx.x % G, d = a.cols;
+    const float inv_d = 1.0f / (float)d;
+    const bool has_post = a.post != nullptr, has_next = a.next != nullptr;
+    float sums[3][P][V];
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int i = 0; i < V; ++i) sums[k][p][i] = 0.0f;
+    for (int row = blockIdx.x * RPB + threadIdx.x / G; row < a.rows; row += gridDim.x * RPB) {
+        const size_t at = (size_t)row * d;
+        const bool live = a.valid == nullptr || a.valid[row] != 0;
+        Piece<XT, V> yr[P], rr[P], gr[P], nr[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = (p * G + lane) * V;
+            const bool in = c < d;
+            if (in && live) yr[p].load(static_cast<const XT*>(a.y) + at + c); else yr[p].zero();
+            if (in && a.grad_out) gr[p].load(static_cast<const XT*>(a.grad_out) + at + c); else gr[p].zero();
+            if (in && has_next) {
+                rr[p].load(static_cast<const XT*>(a.out) + at + c);
+                nr[p].load(static_cast<const XT*>(a.grad_normed) + at + c);
+            } else {
+                rr[p].zero();
+                nr[p].zero();
+            }
+        }
+        float s[3] = {0.0f, 0.0f, 0.0f};  // out^2, out . u, y^2
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = (p * G + lane) * V;
+            float yv[V];
+            yr[p].widen(yv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[2] = fmaf(yv[i], yv[i], s[2]);
+            if (has_next && c < d) {
+                float rv[V], nv[V], w[V];
+                rr[p].widen(rv);
+                nr[p].widen(nv);
+                load_parameter<V>(a.next + c, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s[0] = fmaf(rv[i], rv[i], s[0]);
+                    s[1] = fmaf(rv[i], nv[i] * w[i], s[1]);
+                }
+            }
+        }
+        row_sums<G>(s, room[0]);
+        const float k2 = has_next ? inverse_rms(s[0], d, a.eps) : 0.0f;
+        const float back2 = k2 * k2 * k2 * (s[1] * inv_d);
+        const float k1 = has_post ? inverse_rms(s[2], d, a.eps) : 1.0f;
+        float D[P][V], yv_dot[1] = {0.0f};
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = (p * G + lane) * V;
+            gr[p].widen(D[p]);
+            if (c >= d) continue;
+            if (has_next) {
+                float rv[V], nv[V], w[V];
+                rr[p].widen(rv);
+                nr[p].widen(nv);
+                load_parameter<V>(a.next + c, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    D[p][i] += k2 * (nv[i] * w[i]) - rv[i] * back2;
+                    if (live) sums[2][p][i] = fmaf(nv[i], rv[i] * k2, sums[2][p][i]);
+                }
+            }
+            Piece<XT, V>::store(static_cast<XT*>(a.grad_x) + at + c, D[p]);
+            // from here on D is the gradient of what the gate let through, then of the norm's output
+            float yv[V], w[V], g[V];
+            yr[p].widen(yv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = g[i] = 1.0f;
+            if (has_post) load_parameter<V>(a.post + c, w);
+            if (a.gate_mode == RBMOE_GATE_CHANNEL) {
+                load_parameter<V>(static_cast<const float*>(a.gate) + c, g);
+            } else if (a.gate_mode == RBMOE_GATE_ROW && live) {
+                Piece<XT, V> q;
+                q.load(static_cast<const XT*>(a.gate) + at + c);
+                q.widen(g);
+            }
+            float dg[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float n = yv[i] * k1, e = live ? a.scale * D[p][i] : 0.0f;
+                dg[i] = live ? e * (n * w[i]) : 0.0f;
+                const float db = e * g[i];
+                sums[0][p][i] = live ? fmaf(db, n, sums[0][p][i]) : sums[0][p][i];
+                sums[1][p][i] += dg[i];
+                D[p][i] = has_post ? db * w[i] : db;
+                yv_dot[0] = fmaf(yv[i], D[p][i], yv_dot[0]);
+            }
+            if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) Piece<XT, V>::store(static_cast<XT*>(a.grad_gate) + at + c, dg);
+        }
+        float back1 = 0.0f;
+        if (has_post) {
+            row_sums<G>(yv_dot, room[1]);
+            back1 = k1 * k1 * k1 * (yv_dot[0] * inv_d);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = (p * G + lane) * V;
+            if (c >= d) continue;
+            float yv[V];
+            yr[p].widen(yv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) yv[i] = live ? k1 * D[p][i] - yv[i] * back1 : 0.0f;
+            Piece<XT, V>::store(static_cast<XT*>(a.grad_y) + at + c, yv);
+        }
+        if constexpr (G > 64) __syncthreads();  // `room` is written again
+    }
+    // the sums of the workgroup's waves, in wave order
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        float* const target = sum_target(a, k);
+        if (!target) continue;  // uniform
+        float* const dst = gridDim.x == 1 ? target : a.partial + ((size_t)blockIdx.x * 3 + k) * d;
+        const bool add = gridDim.x == 1 && a.accumulate;
+        if constexpr (RPB > 1) {
+            __shared__ float stage[RPB - 1][P * G * V];
+            const int wave = threadIdx.x / G;
+            __syncthreads();  // the previous array has been read out
+            if (wave > 0)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) stage[wave - 1][(p * V + i) * G + lane] = sums[k][p][i];
+            __syncthreads();
+            if (wave == 0)
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+#pragma unroll
+                        for (int w = 0; w < RPB - 1; ++w) sums[k][p][i] += stage[w][(p * V + i) * G + lane];
+            if (wave != 0) continue;
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = (p * G + lane) * V;
+            if (c >= d) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) dst[c + i] = sums[k][p][i] + (add ? dst[c + i] : 0.0f);
+        }
+    }
+}
+
+// Rows of any width: a workgroup takes every n-th row and reads it again for each step; its sums over rows lie in memory of
+// its own (partial[b]), where a thread adds only to columns of its own.
+template <typename XT>
+__global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) {
+    __shared__ float room[2][12];
+    const int d = a.cols;
+    const float inv_d = 1.0f / (float)d;
+    const bool has_post = a.post != nullptr, has_next = a.next != nullptr;
+    float* const mine = a.partial + (size_t)blockIdx.x * 3 * d;
+    for (int c = threadIdx.x; c < d; c += 256) mine[c] = mine[d + c] = mine[2 * (size_t)d + c] = 0.0f;
+    for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const size_t at = (size_t)row * d;
+        const bool live = a.valid == nullptr || a.valid[row] != 0;
+        const XT* const y = static_cast<const XT*>(a.y) + at;
+        const XT* const r = has_next ? static_cast<const XT*>(a.out) + at : nullptr;
+        const XT* const go = a.grad_out ? static_cast<const XT*>(a.grad_out) + at : nullptr;
+        const XT* const gn = has_next ? static_cast<const XT*>(a.grad_normed) + at : nullptr;
+        float s[3] = {0.0f, 0.0f, 0.0f};
+        for (int c = threadIdx.x; c < d; c += 256) {
+            const float yv = live ? to_f32(y[c]) : 0.0f;
+            s[2] = fmaf(yv, yv, s[2]);
+            if (has_next) {
+                const float rv = to_f32(r[c]);
+                s[0] = fmaf(rv, rv, s[0]);
+                s[1] = fmaf(rv, to_f32(gn[c]) * a.next[c], s[1]);
+            }
+        }
+        row_sums<256>(s, room[0]);
+        const float k2 = has_next ? inverse_rms(s[0], d, a.eps) : 0.0f;
+        const float back2 = k2 * k2 * k2 * (s[1] * inv_d);
+        const float k1 = has_post ? inverse_rms(s[2], d, a.eps) : 1.0f;
+        auto total = [&](int c) {  // D
+            float v = go ? to_f32(go[c]) : 0.0f;
+            if (has_next) v += k2 * (to_f32(gn[c]) * a.next[c]) - to_f32(r[c]) * back2;
+            return v;
+        };
+        auto gate = [&](int c) {
+            return a.gate_mode == RBMOE_GATE_CHANNEL ? static_cast<const float*>(a.gate)[c]
+                   : a.gate_mode == RBMOE_GATE_ROW   ? to_f32(static_cast<const XT*>(a.gate)[at + c])
+                                                     : 1.0f;
+        };
+        float dot[1] = {0.0f};
+        if (has_post) {
+            for (int c = threadIdx.x; live && c < d; c += 256)
+                dot[0] = fmaf(to_f32(y[c]), a.scale * total(c) * gate(c) * a.post[c], dot[0]);
+            row_sums<256>(dot, room[1]);
+        }
+        const float back1 = has_post ? k1 * k1 * k1 * (dot[0] * inv_d) : 0.0f;
+        for (int c = threadIdx.x; c < d; c += 256) {
+            const float D = total(c);
+            float dy = 0.0f, dg = 0.0f;
+            if (live) {
+                const float yv = to_f32(y[c]), n = yv * k1, w = has_post ? a.post[c] : 1.0f, e = a.scale * D, db = e * gate(c);
+                dg = e * (n * w);
+                mine[c] += db * n;
+                mine[d + c] += dg;
+                dy = k1 * (has_post ? db * w : db) - yv * back1;
+                if (has_next) mine[2 * (size_t)d + c] = fmaf(to_f32(gn[c]), to_f32(r[c]) * k2, mine[2 * (size_t)d + c]);
+            }
+            if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) static_cast<XT*>(a.grad_gate)[at + c] = from_f32<XT>(dg);
+            static_cast<XT*>(a.grad_x)[at + c] = from_f32<XT>(D);
+            static_cast<XT*>(a.grad_y)[at + c] = from_f32<XT>(dy);
+        }
+        __syncthreads();  // `room` is written again
+    }
+}
+
+// The workgroups' sums, added in the order of the workgroups: 32 columns a workgroup, 8 threads a column, each over every
+// eighth workgroup.
+__global__ __launch_bounds__(256) void join_sums_kernel(JoinBackward a, int parts) {
+    float* const dst = sum_target(a, blockIdx.y);
+    if (!dst) return;
+    __shared__ float room[8][32];
+    const int d = a.cols, c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+    float s = 0.0f;
+    if (c < d) {
+        const float* src = a.partial + (size_t)blockIdx.y * d + c;
+#pragma unroll 8
+        for (int b = slice; b < parts; b += 8) s += src[(size_t)b * 3 * d];
+    }
+    room[slice][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (slice == 0 && c < d) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += room[w][threadIdx.x & 31];
+        dst[c] = s + (a.accumulate ? dst[c] : 0.0f);
+    }
+}
+
+// Elements of a vector access that rows of `cols` elements and these addresses allow: 16 bytes, 4, or one element.
+int elements_of(int cols, bool bf16, uintptr_t rows_at, uintptr_t parameters_at) {
+    const int es = bf16 ? 2 : 4, whole = 16 / es;
+    if (cols % whole == 0 && rows_at % 16 == 0 && parameters_at % 16 == 0) return whole;
+    if (bf16 && cols % 2 == 0 && rows_at % 4 == 0) return 2;
+    return 1;
+}
+
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// f(V, P, G) as integral constants for rows of `cols` elements by vectors of v, or `any()` where registers do not hold them.
+// A wave takes rows of up to `wave_pieces` vectors a lane, a workgroup those of up to `group_pieces`.
+template <typename XT, int WAVE_ELEMENTS, int GROUP_ELEMENTS, typename F, typename A>
+hipError_t with_shape(int cols, int v, F&& f, A&& any) {
+    auto pick = [&](auto vector) -> hipError_t {
+        constexpr int V = decltype(vector)::value;
+        const int wave = (cols + 64 * V - 1) / (64 * V), group = (cols + 256 * V - 1) / (256 * V);
+        if (wave <= 1) return f(vector, std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
+        if constexpr (2 * V <= WAVE_ELEMENTS)
+            if (wave <= 2) return f(vector, std::integral_constant<int, 2>{}, std::integral_constant<int, 64>{});
+        if constexpr (4 * V <= WAVE_ELEMENTS)
+            if (wave <= 4) return f(vector, std::integral_constant<int, 4>{}, std::integral_constant<int, 64>{});
+        if constexpr (8 * V <= WAVE_ELEMENTS)
+            if (wave <= 8) return f(vector, std::integral_constant<int, 8>{}, std::integral_constant<int, 64>{});
+        if (group <= 1) return f(vector, std::integral_constant<int, 1>{}, std::integral_constant<int, 256>{});
+        if constexpr (2 * V <= GROUP_ELEMENTS)
+            if (group <= 2) return f(vector, std::integral_constant<int, 2>{}, std::integral_constant<int, 256>{});
+        if constexpr (4 * V <= GROUP_ELEMENTS)
+            if (group <= 4) return f(vector, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
+        if constexpr (8 * V <= GROUP_ELEMENTS)
+            if (group <= 8) return f(vector, std::integral_constant<int, 8>{}, std::integral_constant<int, 256>{});
+        return any();
+    };
+    if constexpr (sizeof(XT) == 2) {
+        if (v == 8) return pick(std::integral_constant<int, 8>{});
+        if (v == 2) return pick(std::integral_constant<int, 2>{});
+    } else {
+        if (v == 4) return pick(std::integral_constant<int, 4>{});
+    }
+    return pick(std::integral_constant<int, 1>{});
+}
+
+// Rows of a workgroup's share: enough workgroups to fill the chip (256 units, two each), no more partial sums than that.
+constexpr int kMostParts = 512;
+
+hipError_t add_parts(const JoinBackward& a, int parts, hipStream_t s) {
+    if (!a.grad_post && !a.grad_next && !(a.gate_mode == RBMOE_GATE_CHANNEL && a.grad_gate)) return hipSuccess;
+    hipLaunchKernelGGL(join_sums_kernel, dim3((a.cols + 31) / 32, 3), dim3(256), 0, s, a, parts);
+    return hipGetLastError();
+}
+
+template <typename XT>
+hipError_t forward(const JoinForward& a, hipStream_t s) {
+    const uintptr_t rows = address(a.x) | address(a.y) | address(a.out) | address(a.normed) |
+                           (a.gate_mode == RBMOE_GATE_ROW ? address(a.gate) : 0);
+    const uintptr_t parameters = address(a.post) | address(a.next) | (a.gate_mode == RBMOE_GATE_CHANNEL ? address(a.gate) : 0);
+    return with_shape<XT, 32, 32>(
+        a.cols, elements_of(a.cols, sizeof(XT) == 2, rows, parameters),
+        [&](auto v, auto p, auto g) {
+            constexpr int V = decltype(v)::value, P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
+            hipLaunchKernelGGL((join_forward_kernel<XT, V, P, G>), dim3((a.rows + RPB - 1) / RPB), dim3(256), 0, s, a);
+            return hipGetLastError();
+        },
+        [&] {
+            hipLaunchKernelGGL((join_forward_any_kernel<XT>), dim3(a.rows), dim3(256), 0, s, a);
+            return hipGetLastError();
+        });
+}
+
+template <typename XT>
+hipError_t backward(const JoinBackward& a, hipStream_t s) {
+    const uintptr_t rows = address(a.y) | address(a.out) | address(a.grad_out) | address(a.grad_normed) | address(a.grad_x) |
+                           address(a.grad_y) | (a.gate_mode == RBMOE_GATE_ROW ? address(a.gate) | address(a.grad_gate) : 0);
+    const uintptr_t parameters = address(a.post) | address(a.next) | (a.gate_mode == RBMOE_GATE_CHANNEL ? address(a.gate) : 0);
+    const int most = join_parts(a.cols);
+    int parts = 0;
+    bool final = false;
+    hipError_t e = with_shape<XT, 16, 16>(
+        a.cols, elements_of(a.cols, sizeof(XT) == 2, rows, parameters),
+        [&](auto v, auto p, auto g) {
+            constexpr int V = decltype(v)::value, P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
+            parts = std::min((a.rows + RPB - 1) / RPB, most);
+            final = parts == 1;
+            hipLaunchKernelGGL((join_backward_kernel<XT, V, P, G>), dim3(parts), dim3(256), 0, s, a);
+            return hipGetLastError();
+        },
+        [&] {
+            parts = std::min(a.rows, most);
+            hipLaunchKernelGGL((join_backward_any_kernel<XT>), dim3(parts), dim3(256), 0, s, a);
+            return hipGetLastError();
+        });
+    return e != hipSuccess || final ? e : add_parts(a, parts, s);
+}
+
+}  // namespace
+
+int join_parts(int cols) { return std::max(32, std::min(kMostParts, (1 << 22) / std::max(cols, 1))); }
+
+hipError_t launch_join_forward(const JoinForward& a, bool bf16, hipStream_t s) {
+    if (a.rows == 0) return hipSuccess;
+    return bf16 ? forward<bf16_t>(a, s) : forward<float>(a, s);
+}
+
+hipError_t launch_join_backward(const JoinBackward& a, bool bf16, hipStream_t s) {
+    if (a.rows == 0) return a.accumulate ? hipSuccess : add_parts(a, 0, s);  // (sums over no rows: zero)
+    return bf16 ? backward<bf16_t>(a, s) : backward<float>(a, s);
+}
+
+}  // namespace rbmoe

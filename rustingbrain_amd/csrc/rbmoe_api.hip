@@ -20,11 +20,52 @@
 #include <vector>
 
 #include "host_io.h"
+#include "rbmoe_context.h"
 #include "rbmoe_kernels.h"
 
 using namespace rbmoe;
 
 thread_local rbmoe::KernelTimer* rbmoe::g_kernel_timer = nullptr;
+
+static thread_local std::string g_global_error;
+
+int rbmoe::fail(rbmoe_ctx* ctx, int code, const std::string& msg) {
+    if (ctx) ctx->last_error = msg;
+    g_global_error = msg;
+    return code;
+}
+
+int rbmoe::hip_fail(rbmoe_ctx* ctx, hipError_t e, const char* what) {
+    std::string msg = std::string(what) + ": " + hipGetErrorString(e);
+    if (e == hipErrorOutOfMemory) return fail(ctx, RBMOE_OUT_OF_MEMORY, msg);
+    return fail(ctx, RBMOE_DEVICE_ERROR, msg);
+}
+
+int rbmoe::ctx_alloc(rbmoe_ctx* ctx, size_t bytes, const char* what, void** out) {
+    *out = nullptr;
+    if (ctx->budget_bytes && ctx->allocated + bytes > ctx->budget_bytes) {
+        char buf[200];
+        std::snprintf(buf, sizeof buf, "memory budget exceeded: estimated %zu MiB exceeds budget %zu MiB",
+                      (ctx->allocated + bytes + (1 << 20) - 1) >> 20, ctx->budget_bytes >> 20);
+        return fail(ctx, RBMOE_MEMORY_BUDGET, buf);
+    }
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    const hipError_t e = hipMalloc(out, bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        *out = nullptr;
+        if (e == hipErrorOutOfMemory) return fail(ctx, RBMOE_OUT_OF_MEMORY, std::string("out of memory while allocating ") + what);
+        return hip_fail(ctx, e, what);
+    }
+    ctx->allocated += bytes;
+    return RBMOE_OK;
+}
+
+void rbmoe::ctx_free(rbmoe_ctx* ctx, void* p, size_t bytes) {
+    if (!p) return;
+    (void)hipFree(p);
+    if (ctx->allocated >= bytes) ctx->allocated -= bytes;
+}
 
 // Scratch of rbmoe_forward_static: device memory that exists without any allocation call.  Every GPU the library
 // runs on holds its own copy of the array, at its own address, until the process ends.  In host code the
@@ -55,8 +96,6 @@ hipError_t static_scratch_of(int device, void** out) {
     *out = g_scratch_ptr[device];
     return hipSuccess;
 }
-
-thread_local std::string g_global_error;
 
 size_t dtype_size(int dt) { return dt == RBMOE_F32 ? 4 : dt == RBMOE_BF16 ? 2 : 1; }
 
@@ -119,48 +158,12 @@ std::string limit_problem(const rbmoe_config* c) {
 
 }  // namespace
 
-struct rbmoe_ctx {
-    int device = 0;
-    hipStream_t own_stream = nullptr;
-    hipStream_t stream = nullptr;
-    // The backward pass runs the router's branch beside the weight gradients: a second stream (default
-    // priority, like the first) forked from and joined to `stream` with two events.  Created on first use.
-    hipStream_t side_stream = nullptr;
-    hipEvent_t ev_fork = nullptr, ev_fork2 = nullptr, ev_join = nullptr, ev_tables = nullptr;
-    // host calls: the routing of a forward is complete (recorded on `stream`), its tables are in host memory (recorded
-    // on the side stream).  Created with the side stream.
-    hipEvent_t ev_routed = nullptr, ev_fetched = nullptr;
-    size_t budget_bytes = 0;
-    size_t allocated = 0;
-    void* static_scratch = nullptr;  // this device's copy of rbmoe_static_scratch (RBMOE_STATIC_SCRATCH_BYTES)
-    std::string last_error;
-    int refs = 1;  // the caller's handle + one per live layer; torn down when the last one goes
-};
-
 namespace {
 
 struct Buf {
     void* p = nullptr;
     size_t bytes = 0;
 };
-
-int fail(rbmoe_ctx* ctx, int code, const std::string& msg) {
-    if (ctx) ctx->last_error = msg;
-    g_global_error = msg;
-    return code;
-}
-
-int hip_fail(rbmoe_ctx* ctx, hipError_t e, const char* what) {
-    std::string msg = std::string(what) + ": " + hipGetErrorString(e);
-    if (e == hipErrorOutOfMemory) return fail(ctx, RBMOE_OUT_OF_MEMORY, msg);
-    return fail(ctx, RBMOE_DEVICE_ERROR, msg);
-}
-
-#define HIP_TRY(ctx, expr)                                         \
-    do {                                                           \
-        hipError_t _e = (expr);                                    \
-        if (_e != hipSuccess) return hip_fail((ctx), _e, #expr);   \
-    } while (0)
 
 }  // namespace
 
@@ -586,6 +589,26 @@ void make_tight(rbmoe_layer* L) {
 
 }  // namespace
 
+void rbmoe::ctx_release(rbmoe_ctx* ctx) {
+    if (!ctx || --ctx->refs > 0) return;
+    if (ctx->side_stream) {
+        (void)hipStreamSynchronize(ctx->side_stream);
+        (void)hipStreamDestroy(ctx->side_stream);
+    }
+    if (ctx->ev_fork) (void)hipEventDestroy(ctx->ev_fork);
+    if (ctx->ev_fork2) (void)hipEventDestroy(ctx->ev_fork2);
+    if (ctx->ev_join) (void)hipEventDestroy(ctx->ev_join);
+    if (ctx->ev_tables) (void)hipEventDestroy(ctx->ev_tables);
+    if (ctx->ev_routed) (void)hipEventDestroy(ctx->ev_routed);
+    if (ctx->ev_fetched) (void)hipEventDestroy(ctx->ev_fetched);
+    if (ctx->own_stream) {
+        (void)hipStreamSynchronize(ctx->own_stream);
+        (void)hipStreamDestroy(ctx->own_stream);
+    }
+    delete ctx;
+    host_pool_release();
+}
+
 extern "C" {
 
 const char* rbmoe_version(void) { return "rbmoe 0.1 (gfx950)"; }
@@ -668,26 +691,6 @@ int rbmoe_ctx_create(int32_t device, size_t budget_mib, rbmoe_ctx** out) {
     host_pool_hold();
     *out = ctx;
     return RBMOE_OK;
-}
-
-static void ctx_release(rbmoe_ctx* ctx) {
-    if (!ctx || --ctx->refs > 0) return;
-    if (ctx->side_stream) {
-        (void)hipStreamSynchronize(ctx->side_stream);
-        (void)hipStreamDestroy(ctx->side_stream);
-    }
-    if (ctx->ev_fork) (void)hipEventDestroy(ctx->ev_fork);
-    if (ctx->ev_fork2) (void)hipEventDestroy(ctx->ev_fork2);
-    if (ctx->ev_join) (void)hipEventDestroy(ctx->ev_join);
-    if (ctx->ev_tables) (void)hipEventDestroy(ctx->ev_tables);
-    if (ctx->ev_routed) (void)hipEventDestroy(ctx->ev_routed);
-    if (ctx->ev_fetched) (void)hipEventDestroy(ctx->ev_fetched);
-    if (ctx->own_stream) {
-        (void)hipStreamSynchronize(ctx->own_stream);
-        (void)hipStreamDestroy(ctx->own_stream);
-    }
-    delete ctx;
-    host_pool_release();
 }
 
 // Layers keep their context alive: destroying the context while layers exist
