@@ -351,7 +351,7 @@ int rbmoe_join_backward(rbmoe_join* join, int32_t rows, const void* y, const voi
 
 /* ---- orthogonalised weight updates -----------------------------------------------------------------
  * The reference's optimisers run on the host over Param.grad; this is a step on the device for weight matrices.  A handle
- * takes a stack of `count` matrices [rows, cols] (row-major, contiguous, at most 16384 a side) and holds the workspace: about 16 bytes an element
+ * takes a stack of `count` matrices [rows, cols] (row-major, contiguous, at most 16384 a side) and holds the workspace: about 12 bytes an element
  * and 8 bytes a squared shorter side, counted against the context's budget.
  * rbmoe_orthogonalize brings the singular values of every matrix near one: X = U / (|U|_F + 1e-7), then `steps` times
  *   A = X X^T, B = b A + c A A, X = a X + B X,  (a, b, c) = (3.4445, -4.7750, 2.0315)
