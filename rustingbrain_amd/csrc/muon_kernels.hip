@@ -362,7 +362,7 @@ __device__ __forceinline__ void write_turned(const ProductArgs& a, int matrix, i
 template <Product kind>
 constexpr bool kSymmetric = kind == kGram || kind == kPoly;
 
-// ---- few tiles: 32 x 32 of C a workgroup, a quarter of the reduction a wave ----------------------------
+// ---- few tiles: the reduction split over a workgroup's waves ----------------------------------------------
 // Tile t of the upper triangle (with the diagonal), counted by columns: (row, column) with row <= column.
 __device__ __forceinline__ void triangle(int t, int& row, int& col) {
     int c = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
@@ -372,51 +372,137 @@ __device__ __forceinline__ void triangle(int t, int& row, int& col) {
     row = t - c * (c + 1) / 2;
 }
 
-template <Product kind>
-__global__ __launch_bounds__(256) void muon_product_small_kernel(ProductArgs a) {
-    __shared__ float4 room[4][4][64];
+// A workgroup takes B x B blocks of 32 x 32 of C, and each of its W waves every W-th piece of the reduction, straight from the caches to
+// its registers: nothing to wait for but the loads themselves, most of which are under way at once.  The waves' sums meet in LDS.
+template <Product kind, int B, int W>
+__global__ __launch_bounds__(64 * W) void muon_product_split_kernel(ProductArgs a) {
+    constexpr int S = B == 1 ? 4 : 2;        // steps of a piece
+    constexpr int kQuads = B * B * 4;        // (block, j): four elements a lane
+    __shared__ __align__(16) float4 room[W * kQuads * 64];
+    static_assert(sizeof(room) >= B * B * 32 * kTurnedPitch * 4, "the turned blocks take the sums' place");
     const int matrix = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tp, tq;
     if constexpr (kSymmetric<kind>) {
         triangle(blockIdx.x, tp, tq);
     } else {
-        tp = blockIdx.x % a.pg;
-        tq = blockIdx.x / a.pg;
+        const int rows = (a.pg + B - 1) / B;
+        tp = blockIdx.x % rows;
+        tq = blockIdx.x / rows;
     }
-    const char* const p = a.p + (size_t)matrix * a.p_bytes + (size_t)tp * a.steps * kFragment + lane * 16;
-    const char* const q = a.q + (size_t)matrix * a.q_bytes + (size_t)tq * a.steps * kFragment + lane * 16;
-    floatx16 acc = {};
-    const int per = (a.steps + 3) / 4, k1 = min(a.steps, (wave + 1) * per);
-    for (int k = wave * per; k < k1; ++k) {
-        const halfx8 ph = *reinterpret_cast<const halfx8*>(p + (size_t)k * kFragment);
-        const halfx8 pl = *reinterpret_cast<const halfx8*>(p + (size_t)k * kFragment + 1024);
-        const halfx8 qh = *reinterpret_cast<const halfx8*>(q + (size_t)k * kFragment);
-        const halfx8 ql = *reinterpret_cast<const halfx8*>(q + (size_t)k * kFragment + 1024);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    const char* const pm = a.p + (size_t)matrix * a.p_bytes;
+    const char* const qm = a.q + (size_t)matrix * a.q_bytes;
+    const __amdgpu_buffer_rsrc_t p_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pm), 0, (int)a.p_bytes, kRawBuffer);
+    const __amdgpu_buffer_rsrc_t q_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qm), 0, (int)a.q_bytes, kRawBuffer);
+    int ps[B], qs[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        ps[i] = min(tp * B + i, a.pg - 1) * a.steps * kFragment;
+        qs[i] = min(tq * B + i, a.qg - 1) * a.steps * kFragment;
+    }
+    struct Piece {
+        halfx8 ph[S][B], pl[S][B], qh[S][B], ql[S][B];
+    };
+    const int at = lane * 16;
+    auto load = [&](Piece& d, int piece) {
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            const int step = min(piece * S + k, a.steps - 1) * kFragment;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                d.ph[k][i] = __builtin_bit_cast(halfx8, __builtin_amdgcn_raw_buffer_load_b128(p_buffer, at, ps[i] + step, kVolatile));
+                d.pl[k][i] = __builtin_bit_cast(halfx8, __builtin_amdgcn_raw_buffer_load_b128(p_buffer, at + 1024, ps[i] + step, kVolatile));
+                d.qh[k][i] = __builtin_bit_cast(halfx8, __builtin_amdgcn_raw_buffer_load_b128(q_buffer, at, qs[i] + step, kVolatile));
+                d.ql[k][i] = __builtin_bit_cast(halfx8, __builtin_amdgcn_raw_buffer_load_b128(q_buffer, at + 1024, qs[i] + step, kVolatile));
+            }
+        }
+    };
+    floatx16 acc[B][B];
+#pragma unroll
+    for (int r = 0; r < B; ++r)
+#pragma unroll
+        for (int c = 0; c < B; ++c) acc[r][c] = floatx16{};
+    auto multiply = [&](const Piece& d, int piece) {
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            if (piece * S + k >= a.steps) break;
+#pragma unroll
+            for (int part = 0; part < 3; ++part)
+#pragma unroll
+                for (int r = 0; r < B; ++r)
+#pragma unroll
+                    for (int c = 0; c < B; ++c)
+                        acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(part == 0 ? d.pl[k][r] : d.ph[k][r],
+                                                                           part == 1 ? d.ql[k][c] : d.qh[k][c], acc[r][c], 0, 0, 0);
+        }
+    };
+    const int pieces = (a.steps + S - 1) / S;
+    Piece one, two;
+    if (wave < pieces) load(one, wave);
+    for (int piece = wave; piece < pieces; piece += 2 * W) {
+        if (piece + W < pieces) load(two, piece + W);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(one, piece);
+        if (piece + W >= pieces) break;
+        if (piece + 2 * W < pieces) load(one, piece + 2 * W);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(two, piece + W);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) room[wave][j][lane] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+    for (int r = 0; r < B; ++r)
+#pragma unroll
+        for (int c = 0; c < B; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                room[(wave * kQuads + (r * B + c) * 4 + j) * 64 + lane] =
+                    make_float4(acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]);
+    // a wave adds and writes every W-th quad
+    constexpr int T = (kQuads + W - 1) / W;
+    auto block_of = [&](int t, int& gp, int& gq, int& j) {  // false: nothing to write there
+        const int quad = wave + t * W;
+        j = quad % 4;
+        gp = tp * B + quad / 4 / B;
+        gq = tq * B + quad / 4 % B;
+        return quad < kQuads && gp < a.pg && gq < a.qg && !(kSymmetric<kind> && gp > gq);
+    };
+    Before<kind> before[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        int gp, gq, j;
+        if (block_of(t, gp, gq, j)) read_before<kind>(a, matrix, gp, gq, j, 0, lane, before[t]);
+    }
     __syncthreads();
-    Before<kind> before;
-    read_before<kind>(a, matrix, tp, tq, wave, 0, lane, before);
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sum[T][4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float4 v = room[w][wave][lane];
-        sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+    for (int t = 0; t < T; ++t) {
+        const int quad = min(wave + t * W, kQuads - 1);
+        float4 v = room[quad * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            const float4 x = room[(w * kQuads + quad) * 64 + lane];
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        sum[t][0] = v.x; sum[t][1] = v.y; sum[t][2] = v.z; sum[t][3] = v.w;
     }
-    // the block transposed, for the mirrored operand: [column][row], hi | lo
+    __syncthreads();  // the sums have been read: the turned blocks, for the mirrored operand, take their place
     uint32_t* const turned = reinterpret_cast<uint32_t*>(room);
-    uint32_t parts[4];
-    write4<kind>(a, matrix, tp, tq, wave, 0, lane, sum, before, parts);
-    if (kind == kLast || (kSymmetric<kind> && tp == tq)) return;
-    __syncthreads();
-    *reinterpret_cast<uint4*>(turned + (lane & 31) * kTurnedPitch + 8 * wave + 4 * (lane >> 5)) =
-        make_uint4(parts[0], parts[1], parts[2], parts[3]);
-    __syncthreads();
-    if (wave < 2) write_turned(a, matrix, tp, tq, wave, lane, turned);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        int gp, gq, j;
+        if (!block_of(t, gp, gq, j)) continue;
+        uint32_t parts[4];
+        write4<kind>(a, matrix, gp, gq, j, 0, lane, sum[t], before[t], parts);
+        if constexpr (kind != kLast)
+            *reinterpret_cast<uint4*>(turned + (((wave + t * W) / 4) * 32 + (lane & 31)) * kTurnedPitch + 8 * j + 4 * (lane >> 5)) =
+                make_uint4(parts[0], parts[1], parts[2], parts[3]);
+    }
+    if constexpr (kind != kLast) {
+        __syncthreads();
+        for (int i = wave; i < B * B * 2; i += W) {
+            const int block = i / 2, gp = tp * B + block / B, gq = tq * B + block % B;
+            if (gp < a.pg && gq < a.qg && !(kSymmetric<kind> && gp >= gq))
+                write_turned(a, matrix, gp, gq, i % 2, lane, turned + block * 32 * kTurnedPitch);
+        }
+    }
 }
 
 // f(integral_constant<int, I>) ... f(integral_constant<int, N - 1>), in order
@@ -638,25 +724,34 @@ hipError_t launch_tiles(const ProductArgs& a, int count, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <Product kind, int B>
+int split_tiles_of(const ProductArgs& a) {
+    const int rows = (a.pg + B - 1) / B, cols = (a.qg + B - 1) / B;
+    return kSymmetric<kind> ? rows * (rows + 1) / 2 : rows * cols;
+}
+
+template <Product kind, int B, int W>
+hipError_t launch_split(const ProductArgs& a, int count, hipStream_t s) {
+    hipLaunchKernelGGL((muon_product_split_kernel<kind, B, W>), dim3(split_tiles_of<kind, B>(a), count), dim3(64 * W), 0, s, a);
+    return hipGetLastError();
+}
+
+// Which kernel takes a product.  us a call of five steps (17 launches), count x [rows, cols], by 32 x 32 split eightfold / 64 x 64 split
+// fourfold / 64 x 128 / 128 x 256:
+//   1 x [512, 512] 84 / 125 / 158 / 383, 1 x [768, 768] 141 / 141 / 208 / 515, 1 x [1024, 1024] 228 / 180 / 239 / 635, 1 x [1408, 1408] 487 / 294 / 334 /
+//   813, 4 x [352, 512] 125 / 122 / 142 / 331, 8 x [352, 512] 195 / 156 / 145 / 337, 16 x [352, 512] 319 / 254 / 186 / 349, 24 x [227, 341] 240 / 172 /
+//   148 / 292, 4 x [768, 1408] 526 / 427 / 351 / 624, 128 x [64, 64] 91 / 72 / 82 / 104.
+// What tells them apart is how many workgroups a launch has: under two 64 x 64 tiles for every five compute units the reduction
+// has to be split to use them, and from four for every five on the larger tiles' smaller traffic counts.  128 x 256 (twice the
+// multiplies for every byte) needs two workgroups a unit: 16 x [768, 1408], 192 of them for A 62 us / 72, 576 for X 117 / 106; 128 x [704, 1024], 1536
+// for A 305 / 272, 3072 for X 553 / 430.
 template <Product kind>
 hipError_t launch_product(const ProductArgs& a, int count, hipStream_t s) {
-    // What a launch takes, in units of a 128 x 128 tile's multiplies: tiles of the busiest compute unit times a tile's share, over the rate that
-    // tiles of the size reach.
-    auto cost = [&](int tiles, double tile) { return (double)(((long long)tiles * count + kUnits - 1) / kUnits) * tile; };
-    const double c42 = cost(tiles_of<kind, 4, 2>(a), 2.0), c41 = cost(tiles_of<kind, 4, 1>(a), 1.05), c21 = cost(tiles_of<kind, 2, 1>(a), 0.59);
-#ifdef MUON_FORCE
-    if (MUON_FORCE == 42) return launch_tiles<kind, 4, 2>(a, count, s);
-    if (MUON_FORCE == 41) return launch_tiles<kind, 4, 1>(a, count, s);
-    if (MUON_FORCE == 21) return launch_tiles<kind, 2, 1>(a, count, s);
-#endif
-    if (tiles_of<kind, 2, 1>(a) * count >= 128) {
-        if (c42 <= c41 && c42 <= c21) return launch_tiles<kind, 4, 2>(a, count, s);
-        if (c41 <= c21) return launch_tiles<kind, 4, 1>(a, count, s);
-        return launch_tiles<kind, 2, 1>(a, count, s);
-    }
-    const int tiles = kSymmetric<kind> ? a.pg * (a.pg + 1) / 2 : a.pg * a.qg;
-    hipLaunchKernelGGL((muon_product_small_kernel<kind>), dim3(tiles, count), dim3(256), 0, s, a);
-    return hipGetLastError();
+    const long long tiles = (long long)split_tiles_of<kind, 2>(a) * count;  // of 64 x 64
+    if (tiles * 5 <= kUnits * 2) return launch_split<kind, 1, 8>(a, count, s);
+    if (tiles * 5 <= kUnits * 4) return launch_split<kind, 2, 4>(a, count, s);
+    if ((long long)tiles_of<kind, 4, 2>(a) * count < 2 * kUnits) return launch_tiles<kind, 2, 1>(a, count, s);
+    return launch_tiles<kind, 4, 2>(a, count, s);
 }
 
 size_t rounded(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
