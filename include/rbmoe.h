@@ -56,7 +56,9 @@ typedef enum rbmoe_weight {
     RBMOE_W_SHARED_GATE = 4,  /* [Fs, d]             MoeLayer.shared    (src/moe.rs:210)    */
     RBMOE_W_SHARED_UP = 5,    /* [Fs, d]                                                    */
     RBMOE_W_SHARED_DOWN = 6,  /* [d, Fs]                                                    */
-    RBMOE_W_NORM = 7          /* [1, d]  feed_forward_norm.weight: rbmoe_get_weight_grad only  */
+    RBMOE_W_NORM = 7,         /* [1, d]  feed_forward_norm.weight: rbmoe_get_weight_grad only  */
+    RBMOE_W_POST_NORM = 8,    /* [1, d]  rbmoe_set_block_join's weight: likewise                 */
+    RBMOE_W_BLOCK_GATE = 9    /* [1, d]  rbmoe_set_block_join's gate: likewise                   */
 } rbmoe_weight;
 
 /* `MoeConfig` (reference src/moe.rs:25-39) plus what a device layer must know
@@ -268,6 +270,13 @@ int rbmoe_forward_block(rbmoe_layer* layer, const void* x, int32_t tokens, int32
 int rbmoe_forward_block_host(rbmoe_layer* layer, const void* x, int32_t tokens, int32_t cols,
                              const uint8_t* valid, const float* router_bias, void* out);
 
+/* The block step's join, where it is more than the residual add: out = x + scale * gate * RmsNorm(layer(rmsnorm(x))) * post_weight, as
+ * rbmoe_join_forward has it (below).  post_weight and gate are HOST [d_model] f32 or NULL; both NULL with scale 1 is the residual add
+ * again.  From then on rbmoe_forward_block and rbmoe_backward_block (and their host forms) include it; padding rows pass x through, the
+ * shared expert's rows included.  In training mode the gradients of post_weight and gate accumulate like the norm's
+ * (RBMOE_W_POST_NORM, RBMOE_W_BLOCK_GATE).  Needs the feed-forward norm; a backward pass for a forward from before this call is refused. */
+int rbmoe_set_block_join(rbmoe_layer* layer, const float* post_weight, const float* gate, int32_t cols, float eps, float scale);
+
 /* ---- backward pass (MoeLayer::backward, src/moe.rs:348-489) ------------------------------
  * Training mode makes the forward keep what MoeCache keeps for the backward pass (the input,
  * src/moe.rs:133-135; gate and up pre-activations, src/ffn.rs:27-33) and allocates f32 gradient
@@ -369,6 +378,19 @@ void rbmoe_muon_destroy(rbmoe_muon* muon);
 int rbmoe_orthogonalize(rbmoe_muon* muon, const void* in, int32_t in_dtype, int32_t steps, void* out, int32_t out_dtype);
 int rbmoe_muon_step(rbmoe_muon* muon, const void* grad, int32_t grad_dtype, float* momentum, float* weight, float lr,
                     float momentum_factor, float weight_decay, float update_scale, int32_t nesterov, int32_t steps);
+
+/* The same step for a layer's expert matrices, from its own accumulated gradients: every gate, up and down matrix of the routed
+ * and the shared expert gets one, and the stored weights (operand order and the backward pass's transposed copies included) follow on the
+ * device.  rbmoe_layer_enable_muon, after rbmoe_layer_enable_training and before the weights are set, allocates momentum (zeros), for a bf16
+ * layer f32 weights that the stored ones are rounded from, and the workspace.  The router, the norm and the join keep their
+ * weights: they are vectors or nearly so, and the host updates them.  rbmoe_layer_muon_step enqueues kernels only (it can be captured);
+ * RBMOE_INVALID_INPUT where no backward pass has run since rbmoe_zero_grads.  The gradients stay as they are. */
+int rbmoe_layer_enable_muon(rbmoe_layer* layer);
+int rbmoe_layer_muon_step(rbmoe_layer* layer, float lr, float momentum_factor, float weight_decay, float update_scale,
+                          int32_t nesterov, int32_t steps);
+/* One expert matrix as f32 [rows, cols] (ids and shapes as rbmoe_set_weight; f32 layers, or with updates enabled) into HOST memory: what
+ * a checkpoint holds.  Synchronises. */
+int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* host, int32_t rows, int32_t cols);
 
 /* Per-stage timing of one forward with HIP events on the context's stream.
  * `ms` receives RBMOE_NUM_STAGES durations in milliseconds.  Synchronises.

@@ -25,6 +25,8 @@ pub const RBMOE_W_SHARED_GATE: i32 = 4;
 pub const RBMOE_W_SHARED_UP: i32 = 5;
 pub const RBMOE_W_SHARED_DOWN: i32 = 6;
 pub const RBMOE_W_NORM: i32 = 7;
+pub const RBMOE_W_POST_NORM: i32 = 8;
+pub const RBMOE_W_BLOCK_GATE: i32 = 9;
 
 pub const RBMOE_GATE_NONE: i32 = 0;
 pub const RBMOE_GATE_CHANNEL: i32 = 1;
@@ -114,6 +116,12 @@ extern "C" {
                                 router_bias: *const f32, residual: *const c_void, out: *mut c_void) -> c_int;
     pub fn rbmoe_forward_host(layer: *mut rbmoe_layer, x: *const c_void, tokens: i32, cols: i32, valid: *const u8,
                               router_bias: *const f32, residual: *const c_void, out: *mut c_void) -> c_int;
+    pub fn rbmoe_set_block_join(layer: *mut rbmoe_layer, post_weight: *const f32, gate: *const f32, cols: i32, eps: f32,
+                                scale: f32) -> c_int;
+    pub fn rbmoe_layer_enable_muon(layer: *mut rbmoe_layer) -> c_int;
+    pub fn rbmoe_layer_muon_step(layer: *mut rbmoe_layer, lr: f32, momentum_factor: f32, weight_decay: f32, update_scale: f32,
+                                 nesterov: i32, steps: i32) -> c_int;
+    pub fn rbmoe_get_weight(layer: *mut rbmoe_layer, which: i32, expert: i32, host: *mut f32, rows: i32, cols: i32) -> c_int;
     pub fn rbmoe_join_create(ctx: *mut rbmoe_ctx, cols: i32, dtype: i32, gate: i32, out: *mut *mut rbmoe_join) -> c_int;
     pub fn rbmoe_join_destroy(join: *mut rbmoe_join);
     pub fn rbmoe_join_forward(join: *mut rbmoe_join, rows: i32, x: *const c_void, y: *const c_void, valid: *const u8,

@@ -35,7 +35,7 @@ struct JoinBackward {
     const float* next;
     const void* grad_out;     // or null: zero
     const void* grad_normed;  // read with `next` only
-    void* grad_x;
+    void* grad_x;             // or null
     void* grad_y;
     float* grad_post;         // these three: or null
     void* grad_gate;

@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
                     if (live) sums[2][p][i] = fmaf(nv[i], rv[i] * k2, sums[2][p][i]);
                 }
             }
-            Piece<XT, V>::store(static_cast<XT*>(a.grad_x) + at + c, D[p]);
+            if (a.grad_x) Piece<XT, V>::store(static_cast<XT*>(a.grad_x) + at + c, D[p]);
             // from here on D is the gradient of what the gate let through, then of the norm's output
             float yv[V], w[V], g[V];
             yr[p].widen(yv);
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) 
                 if (has_next) mine[2 * (size_t)d + c] = fmaf(to_f32(gn[c]), to_f32(r[c]) * k2, mine[2 * (size_t)d + c]);
             }
             if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) static_cast<XT*>(a.grad_gate)[at + c] = from_f32<XT>(dg);
-            static_cast<XT*>(a.grad_x)[at + c] = from_f32<XT>(D);
+            if (a.grad_x) static_cast<XT*>(a.grad_x)[at + c] = from_f32<XT>(D);
             static_cast<XT*>(a.grad_y)[at + c] = from_f32<XT>(dy);
         }
         __syncthreads();  // `room` is written again

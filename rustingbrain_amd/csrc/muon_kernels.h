@@ -19,6 +19,8 @@ struct MuonStack {
     int pitch = 0;
 };
 
+constexpr int kMostMuonSide = 1 << 14;  // rows or columns: an operand's offsets are 32-bit
+
 struct MuonCall {
     int count = 0, rows = 0, cols = 0;
     int steps = 5;

@@ -28,7 +28,7 @@ struct rbmoe_muon {
 
 namespace {
 
-constexpr int kMostJoinCols = 1 << 16, kMostMuonSide = 1 << 14, kMostMuonCount = 65535;
+constexpr int kMostJoinCols = 1 << 16, kMostMuonCount = 65535;
 
 bool off_element(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == RBMOE_BF16 ? 2 : 4) != 0; }
 

@@ -20,6 +20,8 @@
 #include <vector>
 
 #include "host_io.h"
+#include "join_kernels.h"
+#include "muon_kernels.h"
 #include "rbmoe_context.h"
 #include "rbmoe_kernels.h"
 
@@ -294,6 +296,15 @@ struct rbmoe_layer {
     // training through the block step (allocated once both the norm and training mode are there)
     Buf xraw, dxn, inv_rms, norm_partial, g_norm;  // [T, d] x2 activation dtype, [T], [T/32][d], [d] f32
     bool last_was_block = false;
+    // the block step's join where it is more than the residual add (rbmoe_set_block_join)
+    Buf yj, join_post, join_gate;         // [max_T, d] the layer's rows, [d] f32 x2
+    bool join_set = false, join_has_post = false, join_has_gate = false;
+    float join_eps = 0.0f, join_scale = 1.0f;
+    Buf dyj, join_partial, join_valid, g_post, g_join_gate;  // training: [max_T, d], partial sums, [max_T], [d] f32 x2
+    bool last_joined = false, last_join_valid = false;       // the last forward: joined so, with padding rows
+    // updates on the device (rbmoe_layer_enable_muon): f32 weights of bf16 layers, momentum, both [matrix][rows, cols] of true widths
+    bool muon = false;
+    Buf mw_gu, mw_d, mw_sgu, mw_sd, mo_gu, mo_d, mo_sgu, mo_sd, muon_work;
     // training (allocated by rbmoe_layer_enable_training)
     bool training = false;
     bool weights_set = false;
@@ -507,6 +518,43 @@ void free_layer_buffers(rbmoe_layer* L) {
     L->all.clear();
 }
 
+// The matrices that an update on the device takes together: the gradients as the backward pass leaves them, f32 weights (of an f32 layer
+// the stored ones), momentum, and where the layer keeps what its products read.
+struct UpdateGroup {
+    int count, rows, cols;      // true widths
+    const float* grad;
+    size_t stride;              // of the gradients, and of stored f32 weights
+    int pitch;
+    Buf* weight;                // f32 weights of a bf16 layer
+    Buf* momentum;
+    Buf* stored;
+    int stored_rows, stored_cols;
+    Buf* turned;
+    int side, turned_cols;
+};
+std::vector<UpdateGroup> update_groups(rbmoe_layer* L) {
+    const rbmoe_config& c = L->cfg;
+    const int E = c.num_experts, d = c.d_model, F = c.d_ff, Fw = L->Fw, Fs = L->Fs, Fsw = L->Fsw;
+    std::vector<UpdateGroup> g = {
+        {2 * E, F, d, (const float*)L->g_gu.p, (size_t)Fw * d, d, &L->mw_gu, &L->mo_gu, &L->wgu, Fw, d, &L->wguT, 2, 2 * Fw},
+        {E, d, F, (const float*)L->g_down.p, (size_t)d * Fw, Fw, &L->mw_d, &L->mo_d, &L->wd, d, Fw, &L->wdT, 1, d},
+    };
+    if (c.shared_expert) {
+        g.push_back({2, Fs, d, (const float*)L->g_sgu.p, (size_t)Fsw * d, d, &L->mw_sgu, &L->mo_sgu, &L->swgu, Fsw, d, &L->swguT, 2, 2 * Fsw});
+        g.push_back({1, d, Fs, (const float*)L->g_sdown.p, (size_t)d * Fsw, Fsw, &L->mw_sd, &L->mo_sd, &L->swd, d, Fsw, &L->swdT, 1, d});
+    }
+    return g;
+}
+// The group and the matrix in it that a weight id stands for; null for the others.
+const UpdateGroup* update_group_of(const std::vector<UpdateGroup>& groups, int which, int expert, int* matrix) {
+    const bool shared = which >= RBMOE_W_SHARED_GATE && which <= RBMOE_W_SHARED_DOWN;
+    if (!shared && (which < RBMOE_W_GATE || which > RBMOE_W_DOWN)) return nullptr;
+    const int kind = which - (shared ? RBMOE_W_SHARED_GATE : RBMOE_W_GATE);  // gate, up, down
+    const size_t at = (shared ? 2 : 0) + (kind == 2 ? 1 : 0);
+    if (at >= groups.size()) return nullptr;
+    *matrix = kind == 2 ? (shared ? 0 : expert) : 2 * (shared ? 0 : expert) + kind;
+    return &groups[at];
+}
 // The buffers of a new layer, cleared.  A failure leaves none of them behind.
 int allocate_layer(rbmoe_layer* L) {
     rbmoe_ctx* ctx = L->ctx;
@@ -930,6 +978,19 @@ int rbmoe_set_weight(rbmoe_layer* L, int32_t which, int32_t expert, const void* 
         src = packed.data();
     }
     HIP_TRY(ctx, hipMemcpy(dst + elem_off * es, src, n * es, hipMemcpyHostToDevice));
+    if (L->muon && target == RBMOE_BF16) {  // the f32 weight that updates on the device start from
+        const std::vector<UpdateGroup> groups = update_groups(L);
+        int matrix = 0;
+        const UpdateGroup* const g = update_group_of(groups, which, expert, &matrix);
+        std::vector<float> wide;
+        const void* given = data;
+        if (dtype == RBMOE_BF16) {
+            wide.resize(n_given);
+            for (size_t i = 0; i < n_given; ++i) wide[i] = host_bf16_to_f32(static_cast<const uint16_t*>(data)[i]);
+            given = wide.data();
+        }
+        HIP_TRY(ctx, hipMemcpy((float*)g->weight->p + (size_t)matrix * n_given, given, n_given * 4, hipMemcpyHostToDevice));
+    }
     if (target == RBMOE_I8)
         HIP_TRY(ctx, hipMemcpy(sdst + scale_off, scales, (size_t)scale_rows * 4, hipMemcpyHostToDevice));
     L->weights_set = true;
@@ -1738,6 +1799,23 @@ void add_block_training(rbmoe_layer* L, Plan& p) {
     p.add(&L->norm_partial, (size_t)rmsnorm_grad_tiles((int)T) * d * 4);
     p.add(&L->g_norm, d * 4);
 }
+// ... and through the join, by whichever of rbmoe_set_block_join and rbmoe_layer_enable_training comes second.
+void add_join_training(rbmoe_layer* L, Plan& p) {
+    if (!L->yj.p || L->dyj.p) return;
+    const size_t T = L->max_T, d = L->cfg.d_model;
+    p.add(&L->dyj, T * d * dtype_size(L->cfg.act_dtype));
+    p.add(&L->join_partial, (size_t)join_parts((int)d) * 3 * d * 4);
+    p.add(&L->join_valid, T);
+    p.add(&L->g_post, d * 4);
+    p.add(&L->g_join_gate, d * 4);
+}
+int ensure_join_training_buffers(rbmoe_layer* L) {
+    if (!L->training || !L->yj.p || L->dyj.p) return RBMOE_OK;
+    Plan p;
+    add_join_training(L, p);
+    return allocate_plan(L, p, "the join's backward buffers");
+}
+
 int ensure_block_training_buffers(rbmoe_layer* L) {
     if (!L->training || !L->norm_w.p || L->xraw.p) return RBMOE_OK;
     Plan p;
@@ -1796,6 +1874,7 @@ Plan training_plan(rbmoe_layer* L) {
         p.add(&L->swguT, d * 2 * Fs * ws);
     }
     add_block_training(L, p);
+    add_join_training(L, p);
     return p;
 }
 
@@ -2197,6 +2276,42 @@ int rbmoe_set_feed_forward_norm(rbmoe_layer* L, const float* weight, int32_t col
     return ensure_block_training_buffers(L);
 }
 
+int rbmoe_set_block_join(rbmoe_layer* L, const float* post_weight, const float* gate, int32_t cols, float eps, float scale) {
+    if (!L) return fail(nullptr, RBMOE_NULL_POINTER, "layer is NULL");
+    rbmoe_ctx* ctx = L->ctx;
+    const rbmoe_config& c = L->cfg;
+    if (cols != c.d_model) {
+        char buf[120];
+        std::snprintf(buf, sizeof buf, "join weight length %d does not match expected length %d", cols, c.d_model);
+        return fail(ctx, RBMOE_INVALID_INPUT, buf);
+    }
+    if (!std::isfinite(scale)) return fail(ctx, RBMOE_INVALID_INPUT, "scale must be finite");
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(ctx, RBMOE_INVALID_INPUT, "eps must be finite and not negative");
+    if (!L->norm_set) return fail(ctx, RBMOE_INVALID_CONFIG, "the feed-forward norm has not been set");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    const bool plain = !post_weight && !gate && scale == 1.0f;  // the residual add alone, which the combine does
+    if (!plain && !L->yj.p) {
+        Plan p;
+        p.add(&L->yj, (size_t)L->max_T * c.d_model * dtype_size(c.act_dtype));
+        p.add(&L->join_post, (size_t)c.d_model * 4);
+        p.add(&L->join_gate, (size_t)c.d_model * 4);
+        if (const int rc = allocate_plan(L, p, "the join's rows")) return rc;
+    }
+    if (!plain)
+        if (const int rc = ensure_join_training_buffers(L)) return rc;
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));  // no forward may still read the old weights
+    // (a backward pass for a forward under other settings would mix the two)
+    L->last_was_block = L->last_joined = false;
+    if (post_weight) HIP_TRY(ctx, hipMemcpy(L->join_post.p, post_weight, (size_t)c.d_model * 4, hipMemcpyHostToDevice));
+    if (gate) HIP_TRY(ctx, hipMemcpy(L->join_gate.p, gate, (size_t)c.d_model * 4, hipMemcpyHostToDevice));
+    L->join_set = !plain;
+    L->join_has_post = post_weight != nullptr;
+    L->join_has_gate = gate != nullptr;
+    L->join_eps = eps;
+    L->join_scale = scale;
+    return RBMOE_OK;
+}
+
 int rbmoe_forward_block(rbmoe_layer* L, const void* x, int32_t T, int32_t cols, const uint8_t* valid,
                         const float* router_bias, void* out) {
     if (!L) return fail(nullptr, RBMOE_NULL_POINTER, "layer is NULL");
@@ -2213,9 +2328,21 @@ int rbmoe_forward_block(rbmoe_layer* L, const void* x, int32_t T, int32_t cols, 
     if (L->training && T > 0)  // TransformerBlockCache keeps the residual (src/transformer_block.rs:224-232)
         HIP_TRY(ctx, hipMemcpyAsync(L->xraw.p, x, (size_t)T * cols * dtype_size(L->cfg.act_dtype),
                                     hipMemcpyDeviceToDevice, ctx->stream));
-    const int rc = forward_impl(L, L->xn.p, T, cols, valid, router_bias, x, out, 0, x);
-    if (rc == RBMOE_OK) L->last_was_block = true;
-    return rc;
+    const bool joined = L->join_set;
+    const int rc = forward_impl(L, L->xn.p, T, cols, valid, router_bias, joined ? nullptr : x, joined ? L->yj.p : out, 0, x);
+    if (rc != RBMOE_OK) return rc;
+    if (joined && T > 0) {
+        const JoinForward j{x, L->yj.p, valid, L->join_has_post ? (const float*)L->join_post.p : nullptr,
+                            L->join_has_gate ? L->join_gate.p : nullptr, nullptr, out, nullptr, T, cols,
+                            L->join_has_gate ? RBMOE_GATE_CHANNEL : RBMOE_GATE_NONE, L->join_scale, L->join_eps};
+        HIP_TRY(ctx, launch_join_forward(j, L->cfg.act_dtype == RBMOE_BF16, ctx->stream));
+        if (L->training && valid)  // the backward pass leaves padding rows out as well, and the caller's bytes may be gone by then
+            HIP_TRY(ctx, hipMemcpyAsync(L->join_valid.p, valid, (size_t)T, hipMemcpyDeviceToDevice, ctx->stream));
+    }
+    L->last_joined = joined;
+    L->last_join_valid = valid != nullptr;
+    L->last_was_block = true;
+    return RBMOE_OK;
 }
 
 int rbmoe_forward_block_host(rbmoe_layer* L, const void* x, int32_t T, int32_t cols, const uint8_t* valid,
@@ -2317,7 +2444,8 @@ int rbmoe_zero_grads(rbmoe_layer* L) {
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     // (a fill kernel, not a memset: a caller may capture a training step in a graph)
     HIP_TRY(ctx, launch_fill_f32((float*)L->g_router.p, 0.0f, (long long)(L->g_router.bytes / 4), ctx->stream));
-    if (L->g_norm.p) HIP_TRY(ctx, launch_fill_f32((float*)L->g_norm.p, 0.0f, (long long)(L->g_norm.bytes / 4), ctx->stream));
+    for (const Buf* g : {&L->g_norm, &L->g_post, &L->g_join_gate})
+        if (g->p) HIP_TRY(ctx, launch_fill_f32((float*)g->p, 0.0f, (long long)(g->bytes / 4), ctx->stream));
     L->grads_clear = true;
     return RBMOE_OK;
 }
@@ -2510,8 +2638,31 @@ int rbmoe_backward_block(rbmoe_layer* L, const void* grad_output, int32_t tokens
     const int T = L->last_T, d = L->cfg.d_model;
     if (T == 0) return RBMOE_OK;
     if (!grad_output || !grad_input) return fail(ctx, RBMOE_NULL_POINTER, "grad_output or grad_input is NULL");
+    const void* upstream = grad_output;
+    if (L->last_joined) {  // ... through the join first (a training layer that has one holds its buffers)
+        if (!L->dyj.p) return fail(ctx, RBMOE_INVALID_INPUT, "no forward pass has run in training mode yet");
+        HIP_TRY(ctx, hipSetDevice(ctx->device));
+        JoinBackward j{};
+        j.y = L->yj.p;
+        j.valid = L->last_join_valid ? (const uint8_t*)L->join_valid.p : nullptr;
+        j.post = L->join_has_post ? (const float*)L->join_post.p : nullptr;
+        j.gate = L->join_has_gate ? L->join_gate.p : nullptr;
+        j.gate_mode = L->join_has_gate ? RBMOE_GATE_CHANNEL : RBMOE_GATE_NONE;
+        j.grad_out = grad_output;
+        j.grad_y = L->dyj.p;
+        j.grad_post = L->join_has_post ? (float*)L->g_post.p : nullptr;
+        j.grad_gate = L->join_has_gate ? L->g_join_gate.p : nullptr;
+        j.partial = (float*)L->join_partial.p;
+        j.rows = T;
+        j.cols = d;
+        j.accumulate = 1;
+        j.scale = L->join_scale;
+        j.eps = L->join_eps;
+        HIP_TRY(ctx, launch_join_backward(j, L->cfg.act_dtype == RBMOE_BF16, ctx->stream));
+        upstream = L->dyj.p;
+    }
     // grad_projected = feed_forward.backward(cache, grad_output)  (src/transformer_block.rs:257)
-    const int rc = rbmoe_backward(L, grad_output, tokens, cols, L->dxn.p);
+    const int rc = rbmoe_backward(L, upstream, tokens, cols, L->dxn.p);
     if (rc != RBMOE_OK) return rc;
     // grad_residual = feed_forward_norm.backward(residual, grad_projected) + grad_output  (:258-263)
     HIP_TRY(ctx, launch_rmsnorm_backward(L->xraw.p, L->dxn.p, (const float*)L->norm_w.p, L->norm_eps, grad_output, T, d,
@@ -2565,12 +2716,21 @@ int rbmoe_get_weight_grad(rbmoe_layer* L, int32_t which, int32_t expert, float* 
             src = (const float*)L->g_norm.p;
             want_rows = 1; want_cols = d;
             break;
+        case RBMOE_W_POST_NORM:
+        case RBMOE_W_BLOCK_GATE: {
+            const bool gate = which == RBMOE_W_BLOCK_GATE;
+            if (!L->join_set || !(gate ? L->join_has_gate : L->join_has_post))
+                return fail(ctx, RBMOE_INVALID_CONFIG, gate ? "the block's join has no gate" : "the block's join has no norm");
+            src = (const float*)(gate ? L->g_join_gate.p : L->g_post.p);
+            want_rows = 1; want_cols = d;
+            break;
+        }
         default:
             return fail(ctx, RBMOE_INVALID_CONFIG, "unknown weight id");
     }
     if ((size_t)rows != want_rows || (size_t)cols != want_cols)
         return fail(ctx, RBMOE_INVALID_INPUT, "gradient shape does not match the weight");
-    if (L->grads_clear && which != RBMOE_W_ROUTER && which != RBMOE_W_NORM) {  // cleared and not written since
+    if (L->grads_clear && which != RBMOE_W_ROUTER && which < RBMOE_W_NORM) {  // cleared and not written since
         std::memset(host, 0, want_rows * want_cols * 4);
         return RBMOE_OK;
     }
@@ -2606,6 +2766,95 @@ int rbmoe_get_weight_grad(rbmoe_layer* L, int32_t which, int32_t expert, float* 
     }
     HIP_TRY(ctx, hipStreamSynchronize(s));
     for (size_t r = 0; r < want_rows; ++r) std::memcpy(host + r * want_cols, stage.p + r * apart, want_cols * 4);
+    return RBMOE_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Updates on the device.
+// ---------------------------------------------------------------------------
+int rbmoe_layer_enable_muon(rbmoe_layer* L) {
+    if (!L) return fail(nullptr, RBMOE_NULL_POINTER, "layer is NULL");
+    rbmoe_ctx* ctx = L->ctx;
+    if (L->muon) return RBMOE_OK;
+    if (!L->training) return fail(ctx, RBMOE_INVALID_CONFIG, "training is not enabled on this layer");
+    if (L->weights_set) return fail(ctx, RBMOE_INVALID_CONFIG, "enable updates before the weights are set");
+    Plan p;
+    size_t work = 0;
+    for (const UpdateGroup& g : update_groups(L)) {
+        if (g.rows > kMostMuonSide || g.cols > kMostMuonSide)
+            return fail(ctx, RBMOE_UNSUPPORTED, "updates on the device take matrices of at most 16384 rows and columns");
+        const size_t bytes = (size_t)g.count * g.rows * g.cols * 4;
+        if (L->cfg.weight_dtype == RBMOE_BF16) p.add(g.weight, bytes);
+        p.add(g.momentum, bytes);
+        work = std::max(work, muon_workspace_bytes(g.count, g.rows, g.cols));
+    }
+    p.add(&L->muon_work, work);
+    if (const int rc = allocate_plan(L, p, "the update's buffers")) return rc;
+    L->muon = true;
+    return RBMOE_OK;
+}
+
+int rbmoe_layer_muon_step(rbmoe_layer* L, float lr, float momentum_factor, float weight_decay, float update_scale, int32_t nesterov,
+                          int32_t steps) {
+    if (!L) return fail(nullptr, RBMOE_NULL_POINTER, "layer is NULL");
+    rbmoe_ctx* ctx = L->ctx;
+    if (!L->muon) return fail(ctx, RBMOE_INVALID_CONFIG, "updates are not enabled on this layer");
+    if (const char* problem = muon_settings_problem(lr, momentum_factor, weight_decay, update_scale, steps))
+        return fail(ctx, RBMOE_INVALID_CONFIG, problem);
+    if (L->grads_clear) return fail(ctx, RBMOE_INVALID_INPUT, "no backward pass has run since the gradients were cleared");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    const bool bf16 = L->cfg.weight_dtype == RBMOE_BF16;
+    for (const UpdateGroup& g : update_groups(L)) {
+        const size_t elements = (size_t)g.rows * g.cols;
+        MuonCall c;
+        c.count = g.count;
+        c.rows = g.rows;
+        c.cols = g.cols;
+        c.steps = steps;
+        c.grad = {g.grad, g.stride, g.pitch};
+        c.momentum = {g.momentum->p, elements, g.cols};
+        if (bf16) c.weight = {g.weight->p, elements, g.cols};
+        else c.weight = {g.stored->p, g.stride, g.pitch};
+        c.mu = momentum_factor;
+        c.keep = 1.0f - lr * weight_decay;
+        c.rate = lr * muon_scale(update_scale, g.rows, g.cols);
+        c.nesterov = nesterov != 0;
+        c.workspace = L->muon_work.p;
+        HIP_TRY(ctx, launch_muon(c, ctx->stream));
+        const WeightRefresh w{static_cast<const float*>(c.weight.p), c.weight.stride, c.weight.pitch, g.rows, g.cols, g.count,
+                              g.stored->p, bf16, g.stored_rows, g.stored_cols, g.turned->p, g.side, g.turned_cols};
+        HIP_TRY(ctx, launch_weight_refresh(w, bf16, L->use_stream, ctx->stream));
+    }
+    return RBMOE_OK;
+}
+
+int rbmoe_get_weight(rbmoe_layer* L, int32_t which, int32_t expert, float* host, int32_t rows, int32_t cols) {
+    if (!L) return fail(nullptr, RBMOE_NULL_POINTER, "layer is NULL");
+    rbmoe_ctx* ctx = L->ctx;
+    if (!host) return fail(ctx, RBMOE_NULL_POINTER, "host buffer is NULL");
+    const std::vector<UpdateGroup> groups = update_groups(L);
+    int matrix = 0;
+    const UpdateGroup* const g = update_group_of(groups, which, expert, &matrix);
+    if (!g) return fail(ctx, RBMOE_INVALID_CONFIG, "not an expert matrix of this layer");
+    if ((which == RBMOE_W_GATE || which == RBMOE_W_UP || which == RBMOE_W_DOWN) && (expert < 0 || expert >= L->cfg.num_experts))
+        return fail(ctx, RBMOE_INVALID_CONFIG, "expert index out of range");
+    if (rows != g->rows || cols != g->cols) return fail(ctx, RBMOE_INVALID_INPUT, "shape does not match the weight");
+    const bool stored = L->cfg.weight_dtype == RBMOE_F32;
+    if (!stored && !L->muon) return fail(ctx, RBMOE_UNSUPPORTED, "f32 weights are kept where updates on the device are enabled");
+    HIP_TRY(ctx, hipSetDevice(ctx->device));
+    HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+    const float* const src = stored ? (const float*)g->stored->p + (size_t)matrix * g->stride
+                                    : (const float*)g->weight->p + (size_t)matrix * g->rows * g->cols;
+    const size_t pitch = stored ? g->pitch : g->cols;
+    if (pitch == (size_t)cols) {
+        HIP_TRY(ctx, hipMemcpy(host, src, (size_t)rows * cols * 4, hipMemcpyDeviceToHost));
+        return RBMOE_OK;
+    }
+    // (whole rows of the rounded width, as rbmoe_get_weight_grad)
+    Staging stage;
+    if (!stage.take((size_t)rows * pitch * 4)) return fail(ctx, RBMOE_OUT_OF_MEMORY, "no host memory for the weight's rows");
+    HIP_TRY(ctx, hipMemcpy(stage.p, src, (size_t)rows * pitch * 4, hipMemcpyDeviceToHost));
+    for (int r = 0; r < rows; ++r) std::memcpy(host + (size_t)r * cols, stage.p + (size_t)r * pitch * 4, (size_t)cols * 4);
     return RBMOE_OK;
 }
 

@@ -451,4 +451,18 @@ hipError_t launch_decode_down_by_expert(const DecodeGemmArgs& g, const DecodeLay
 bool decode_down_few_ok(const DecodeGemmArgs& g, WeightKind wk, int T, int k);
 hipError_t launch_decode_down_few(const DecodeGemmArgs& g, const DecodeLayoutArgs& t, WeightKind wk, hipStream_t s);
 
+// A stack of f32 matrices [count][rows, cols] (row pitch and stride in elements) as the layer stores them: [dst_rows, dst_cols], rounded up,
+// and transposed: `side` matrices side by side in one of [dst_cols, turned_cols] (gate and up: 2, turned_cols = 2 dst_rows).
+struct WeightRefresh {
+    const float* src;
+    size_t src_stride;
+    int src_pitch, rows, cols, count;
+    void* dst;
+    bool write_dst;  // false: `src` is the stored matrix itself
+    int dst_rows, dst_cols;
+    void* turned;
+    int side, turned_cols;
+};
+hipError_t launch_weight_refresh(const WeightRefresh& a, bool bf16, bool packed, hipStream_t s);
+
 }  // namespace rbmoe

@@ -537,6 +537,24 @@ class MoeLayer:
         _check(self._lib.rbmoe_set_feed_forward_norm(self.handle, w.ctypes.data_as(C.POINTER(C.c_float)), w.size,
                                                      C.c_float(eps)), self.device.handle)
 
+    def set_block_join(self, post_weight: Optional[np.ndarray] = None, gate: Optional[np.ndarray] = None, scale: float = 1.0,
+                       eps: float = 1e-6) -> None:
+        """The block step's join from here on: ``x + scale * gate * rmsnorm(layer(rmsnorm(x))) * post_weight`` (``[d_model]`` f32 each, or
+        None).  Without arguments: the residual add alone again."""
+        fp = C.POINTER(C.c_float)
+        arrays = []
+        for v in (post_weight, gate):
+            if v is None:
+                arrays.append(None)
+                continue
+            a = np.ascontiguousarray(np.asarray(v, dtype=np.float32).reshape(-1))
+            if a.size != self._d_model:
+                raise InvalidInput(f"join weight length {a.size} does not match expected length {self._d_model}",
+                                   expected=self._d_model, actual=a.size)
+            arrays.append(a)
+        _check(self._lib.rbmoe_set_block_join(self.handle, *[None if a is None else a.ctypes.data_as(fp) for a in arrays],
+                                              self._d_model, eps, scale), self.device.handle)
+
     def forward_block(self, residual: np.ndarray, layout: Layout = Layout(),
                       router_bias: Optional[np.ndarray] = None) -> Tuple[np.ndarray, MoeCache]:
         """``residual + forward_train(feed_forward_norm(residual))``; the cache describes the normed rows."""
@@ -594,11 +612,35 @@ class MoeLayer:
     def zero_grads(self) -> None:
         _check(self._lib.rbmoe_zero_grads(self.handle), self.device.handle)
 
+    def _shape_of(self, which: int) -> Tuple[int, int]:
+        F, d, Fs = self.config.d_ff, self._d_model, self.shared_d_ff
+        return {L.W_ROUTER: (self.config.num_experts, d), L.W_GATE: (F, d), L.W_UP: (F, d), L.W_DOWN: (d, F),
+                L.W_SHARED_GATE: (Fs, d), L.W_SHARED_UP: (Fs, d), L.W_SHARED_DOWN: (d, Fs), L.W_NORM: (1, d),
+                L.W_POST_NORM: (1, d), L.W_BLOCK_GATE: (1, d)}[which]
+
+    # ---- updates on the device
+    def enable_muon(self) -> None:
+        """Momentum, f32 weights and workspace for ``muon_step``.  Call after ``enable_training`` and before the weights are set."""
+        _check(self._lib.rbmoe_layer_enable_muon(self.handle), self.device.handle)
+
+    def muon_step(self, lr: float, momentum: float = 0.95, weight_decay: float = 0.0, update_scale: float = 0.0,
+                  nesterov: bool = True, steps: int = 5) -> None:
+        """One optimiser step for every expert matrix from the accumulated gradients (see ``Muon.step_device``), enqueued without
+        synchronisation; the stored weights follow on the device."""
+        _check(self._lib.rbmoe_layer_muon_step(self.handle, lr, momentum, weight_decay, update_scale, int(nesterov), steps),
+               self.device.handle)
+
+    def weight(self, which: int, expert: int = 0) -> np.ndarray:
+        """One expert matrix as f32 (f32 layers, or with ``enable_muon``): ``which`` is one of ``_lib.W_*``."""
+        shape = self._shape_of(which)
+        w = np.empty(shape, np.float32)
+        _check(self._lib.rbmoe_get_weight(self.handle, which, expert, w.ctypes.data_as(C.POINTER(C.c_float)), *shape),
+               self.device.handle)
+        return w
+
     def weight_grad(self, which: int, expert: int = 0) -> np.ndarray:
         """Accumulated gradient (f32) of one weight matrix: ``which`` is one of ``_lib.W_*``."""
-        F, d, Fs = self.config.d_ff, self._d_model, self.shared_d_ff
-        shape = {L.W_ROUTER: (self.config.num_experts, d), L.W_GATE: (F, d), L.W_UP: (F, d), L.W_DOWN: (d, F),
-                 L.W_SHARED_GATE: (Fs, d), L.W_SHARED_UP: (Fs, d), L.W_SHARED_DOWN: (d, Fs), L.W_NORM: (1, d)}[which]
+        shape = self._shape_of(which)
         g = self.device.empty(shape, np.float32)
         _check(self._lib.rbmoe_get_weight_grad(self.handle, which, expert, g.ctypes.data_as(C.POINTER(C.c_float)),
                                                shape[0], shape[1]), self.device.handle)

@@ -12,8 +12,8 @@ from . import _lib as L
 from .moe import Device, InvalidConfig, _check
 
 
-def _p(address: int) -> C.c_void_p:
-    return C.c_void_p(address or None)
+def _p(address: int):
+    return address or None
 
 
 def _dtype(name: str) -> int:
