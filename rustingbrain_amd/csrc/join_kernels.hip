@@ -281,6 +281,18 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
         for (int p = 0; p < P; ++p)
 #pragma unroll
             for (int i = 0; i < V; ++i) sums[k][p][i] = 0.0f;
+    // the parameters of the thread's columns stay in registers from row to row
+    float next[P][V], post[P][V], gate[P][V];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int c = (p * G + lane) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) next[p][i] = 0.0f, post[p][i] = gate[p][i] = 1.0f;
+        if (c >= d) continue;
+        if (has_next) load_parameter<V>(a.next + c, next[p]);
+        if (has_post) load_parameter<V>(a.post + c, post[p]);
+        if (a.gate_mode == RBMOE_GATE_CHANNEL) load_parameter<V>(static_cast<const float*>(a.gate) + c, gate[p]);
+    }
     for (int row = blockIdx.x * RPB + threadIdx.x / G; row < a.rows; row += gridDim.x * RPB) {
         const size_t at = (size_t)row * d;
         const bool live = a.valid == nullptr || a.valid[row] != 0;
@@ -302,20 +314,18 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
         float s[3] = {0.0f, 0.0f, 0.0f};  // out^2, out . u, y^2
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = (p * G + lane) * V;
             float yv[V];
             yr[p].widen(yv);
 #pragma unroll
             for (int i = 0; i < V; ++i) s[2] = fmaf(yv[i], yv[i], s[2]);
-            if (has_next && c < d) {
-                float rv[V], nv[V], w[V];
+            if (has_next) {
+                float rv[V], nv[V];
                 rr[p].widen(rv);
                 nr[p].widen(nv);
-                load_parameter<V>(a.next + c, w);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     s[0] = fmaf(rv[i], rv[i], s[0]);
-                    s[1] = fmaf(rv[i], nv[i] * w[i], s[1]);
+                    s[1] = fmaf(rv[i], nv[i] * next[p][i], s[1]);
                 }
             }
         }
@@ -330,26 +340,22 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
             gr[p].widen(D[p]);
             if (c >= d) continue;
             if (has_next) {
-                float rv[V], nv[V], w[V];
+                float rv[V], nv[V];
                 rr[p].widen(rv);
                 nr[p].widen(nv);
-                load_parameter<V>(a.next + c, w);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    D[p][i] += k2 * (nv[i] * w[i]) - rv[i] * back2;
+                    D[p][i] += k2 * (nv[i] * next[p][i]) - rv[i] * back2;
                     if (live) sums[2][p][i] = fmaf(nv[i], rv[i] * k2, sums[2][p][i]);
                 }
             }
             if (a.grad_x) Piece<XT, V>::store(static_cast<XT*>(a.grad_x) + at + c, D[p]);
             // from here on D is the gradient of what the gate let through, then of the norm's output
-            float yv[V], w[V], g[V];
+            float yv[V], g[V];
             yr[p].widen(yv);
 #pragma unroll
-            for (int i = 0; i < V; ++i) w[i] = g[i] = 1.0f;
-            if (has_post) load_parameter<V>(a.post + c, w);
-            if (a.gate_mode == RBMOE_GATE_CHANNEL) {
-                load_parameter<V>(static_cast<const float*>(a.gate) + c, g);
-            } else if (a.gate_mode == RBMOE_GATE_ROW && live) {
+            for (int i = 0; i < V; ++i) g[i] = gate[p][i];
+            if (a.gate_mode == RBMOE_GATE_ROW && live) {
                 Piece<XT, V> q;
                 q.load(static_cast<const XT*>(a.gate) + at + c);
                 q.widen(g);
@@ -358,11 +364,11 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float n = yv[i] * k1, e = live ? a.scale * D[p][i] : 0.0f;
-                dg[i] = live ? e * (n * w[i]) : 0.0f;
+                dg[i] = live ? e * (n * post[p][i]) : 0.0f;
                 const float db = e * g[i];
                 sums[0][p][i] = live ? fmaf(db, n, sums[0][p][i]) : sums[0][p][i];
                 sums[1][p][i] += dg[i];
-                D[p][i] = has_post ? db * w[i] : db;
+                D[p][i] = has_post ? db * post[p][i] : db;
                 yv_dot[0] = fmaf(yv[i], D[p][i], yv_dot[0]);
             }
             if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) Piece<XT, V>::store(static_cast<XT*>(a.grad_gate) + at + c, dg);
