@@ -280,6 +280,38 @@ impl MoeLayer {
         Ok(g)
     }
 
+    /// The block step's join from here on (`rbmoe_set_block_join`): a norm behind the layer, a gate, a scale; `None, None, 1.0` is the
+    /// residual add alone.
+    pub fn set_block_join(&mut self, post_weight: Option<&[f32]>, gate: Option<&[f32]>, eps: f32, scale: f32) -> Result<(), NetworkError> {
+        for v in [post_weight, gate].into_iter().flatten() {
+            if v.len() != self.d_model {
+                return Err(NetworkError::InvalidInput { expected: self.d_model, actual: v.len() });
+            }
+        }
+        let p = |v: Option<&[f32]>| v.map_or(ptr::null(), |s| s.as_ptr());
+        check(unsafe { sys::rbmoe_set_block_join(self.layer, p(post_weight), p(gate), self.d_model as i32, eps, scale) },
+              self.device.raw(), 0, 0)
+    }
+
+    /// Momentum, f32 weights and workspace for `muon_step`; after `enable_training` and before the weights are set.
+    pub fn enable_muon(&mut self) -> Result<(), NetworkError> {
+        check(unsafe { sys::rbmoe_layer_enable_muon(self.layer) }, self.device.raw(), 0, 0)
+    }
+
+    /// One orthogonalised update of every expert matrix from the accumulated gradients, on the device.
+    pub fn muon_step(&mut self, lr: f32, momentum: f32, weight_decay: f32) -> Result<(), NetworkError> {
+        check(unsafe { sys::rbmoe_layer_muon_step(self.layer, lr, momentum, weight_decay, 0.0, 1, 5) }, self.device.raw(), 0, 0)
+    }
+
+    /// One expert matrix as f32 (`which`: `sys::RBMOE_W_*`), `[rows, cols]` as the weight.
+    pub fn weight(&self, which: i32, expert: usize, rows: usize, cols: usize) -> Result<Vec<f32>, NetworkError> {
+        let mut w = vec![0f32; rows * cols];
+        check(unsafe {
+            sys::rbmoe_get_weight(self.layer, which, expert as i32, w.as_mut_ptr(), rows as i32, cols as i32)
+        }, self.device.raw(), 0, 0)?;
+        Ok(w)
+    }
+
     /// `MoeLayer::forward` (src/moe.rs:237-241).
     pub fn forward(&self, input: &[f32], rows: usize, cols: usize) -> Result<Vec<f32>, NetworkError> {
         self.forward_train(input, rows, cols, Layout::default()).map(|(out, _)| out)

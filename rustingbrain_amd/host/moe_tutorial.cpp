@@ -218,6 +218,34 @@ static void gpu_checks() {
         bool cleared = true;
         for (float v : train.weight_grad(RBMOE_W_DOWN, 1).data) cleared = cleared && v == 0.0f;
         EXPECT(cleared);
+        // a norm behind the layer and a gate: the branch's gradients reach both, and without them the block is the plain one again
+        train.set_block_join(norm_w, std::vector<float>(TD, 0.5f), 0.7f);
+        train.forward_block(x);
+        train.backward_block(ones);
+        bool post_grad = false;
+        for (float v : train.weight_grad(RBMOE_W_POST_NORM).data) post_grad = post_grad || v != 0.0f;
+        EXPECT(post_grad && train.weight_grad(RBMOE_W_BLOCK_GATE).cols == TD);
+        EXPECT(throws<InvalidInput>([&] { train.set_block_join(std::vector<float>(TD + 1, 1.0f)); }));
+        train.set_block_join();
+        EXPECT(train.forward_block(x).data == out.data);
+        // updates on the device are enabled before the weights are set
+        EXPECT(throws<InvalidConfig>([&] { train.enable_muon(); }));
+        MoeLayer update(TD, MoeConfig(TE, 2, TF), device, TR);
+        update.enable_training();
+        update.enable_muon();
+        update.set_router(random_matrix(TE, TD, 0.5f, 21));
+        for (size_t e = 0; e < TE; ++e)
+            update.set_expert(e, random_matrix(TF, TD, tb, 200 + 3 * e), random_matrix(TF, TD, tb, 201 + 3 * e),
+                              random_matrix(TD, TF, tb, 202 + 3 * e));
+        EXPECT(update.weight(RBMOE_W_UP, 2).data == random_matrix(TF, TD, tb, 207).data);
+        EXPECT(throws<InvalidInput>([&] { update.muon_step(0.02f); }));  // no gradients yet
+        update.forward(x);
+        update.backward(ones);
+        update.muon_step(0.02f);
+        const Matrix moved = update.weight(RBMOE_W_UP, 2), was = random_matrix(TF, TD, tb, 207);
+        double change = 0.0;  // |lr O| = 0.02 sqrt(sum of the squared singular values of O), each about one
+        for (size_t i = 0; i < moved.data.size(); ++i) change += (double)(moved.data[i] - was.data[i]) * (moved.data[i] - was.data[i]);
+        EXPECT(std::sqrt(change) > 0.02 * 0.5 * std::sqrt((double)TF) && std::sqrt(change) < 0.02 * 1.25 * std::sqrt((double)TF));
         // no backward pass for a layer that is not in training mode
         EXPECT(throws<InvalidConfig>([&] { layer.backward(Matrix(ROWS, D)); }));
     }

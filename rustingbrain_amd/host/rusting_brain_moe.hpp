@@ -340,24 +340,40 @@ class MoeLayer {
         return grad_input;
     }
 
+    // The block step's join from here on: input + scale * gate * rmsnorm(layer) * post_weight (an empty vector leaves a factor out);
+    // without arguments the residual add alone again.
+    void set_block_join(const std::vector<float>& post_weight = {}, const std::vector<float>& gate = {}, float scale = 1.0f,
+                        float eps = 1e-6f) {
+        for (const auto* v : {&post_weight, &gate})
+            if (!v->empty() && v->size() != d_model_)
+                throw InvalidInput("join weight length " + std::to_string(v->size()) + " does not match expected length " +
+                                       std::to_string(d_model_),
+                                   d_model_, v->size());
+        check(rbmoe_set_block_join(layer_, post_weight.empty() ? nullptr : post_weight.data(), gate.empty() ? nullptr : gate.data(),
+                                   (int32_t)d_model_, eps, scale),
+              device_->raw());
+    }
+
+    // Updates of the expert matrices on the device: momentum, f32 weights and workspace (after enable_training, before the weights), one
+    // step from the accumulated gradients, and a matrix as it stands.
+    void enable_muon() { check(rbmoe_layer_enable_muon(layer_), device_->raw()); }
+    void muon_step(float lr, float momentum = 0.95f, float weight_decay = 0.0f, float update_scale = 0.0f, bool nesterov = true,
+                   int steps = 5) {
+        check(rbmoe_layer_muon_step(layer_, lr, momentum, weight_decay, update_scale, nesterov ? 1 : 0, steps), device_->raw());
+    }
+    Matrix weight(int which, size_t expert = 0) {
+        Matrix w = shaped_like(which);
+        check(rbmoe_get_weight(layer_, which, (int32_t)expert, w.data.data(), (int32_t)w.rows, (int32_t)w.cols), device_->raw());
+        return w;
+    }
+
     // Param::zero_grad over the layer's parameters (src/param.rs)
     void zero_grads() { check(rbmoe_zero_grads(layer_), device_->raw()); }
 
     // accumulated gradient of one weight matrix (`which`: RBMOE_W_*), shaped like the weight
     Matrix weight_grad(int which, size_t expert = 0) {
-        const size_t E = config.num_experts, F = config.d_ff, Fs = shared_d_ff_ ? shared_d_ff_ : config.d_ff;
-        size_t rows = 0, cols = 0;
-        switch (which) {
-            case RBMOE_W_ROUTER: rows = E; cols = d_model_; break;
-            case RBMOE_W_GATE: case RBMOE_W_UP: rows = F; cols = d_model_; break;
-            case RBMOE_W_DOWN: rows = d_model_; cols = F; break;
-            case RBMOE_W_SHARED_GATE: case RBMOE_W_SHARED_UP: rows = Fs; cols = d_model_; break;
-            case RBMOE_W_SHARED_DOWN: rows = d_model_; cols = Fs; break;
-            case RBMOE_W_NORM: rows = 1; cols = d_model_; break;
-            default: throw InvalidConfig("unknown weight id");
-        }
-        Matrix g(rows, cols);
-        check(rbmoe_get_weight_grad(layer_, which, (int32_t)expert, g.data.data(), (int32_t)rows, (int32_t)cols),
+        Matrix g = shaped_like(which);
+        check(rbmoe_get_weight_grad(layer_, which, (int32_t)expert, g.data.data(), (int32_t)g.rows, (int32_t)g.cols),
               device_->raw());
         return g;
     }
@@ -367,6 +383,18 @@ class MoeLayer {
     std::string kernel_name() const { return rbmoe_expert_kernel_name(layer_); }
 
   private:
+    Matrix shaped_like(int which) const {
+        const size_t E = config.num_experts, F = config.d_ff, Fs = shared_d_ff_ ? shared_d_ff_ : config.d_ff;
+        switch (which) {
+            case RBMOE_W_ROUTER: return Matrix(E, d_model_);
+            case RBMOE_W_GATE: case RBMOE_W_UP: return Matrix(F, d_model_);
+            case RBMOE_W_DOWN: return Matrix(d_model_, F);
+            case RBMOE_W_SHARED_GATE: case RBMOE_W_SHARED_UP: return Matrix(Fs, d_model_);
+            case RBMOE_W_SHARED_DOWN: return Matrix(d_model_, Fs);
+            case RBMOE_W_NORM: case RBMOE_W_POST_NORM: case RBMOE_W_BLOCK_GATE: return Matrix(1, d_model_);
+            default: throw InvalidConfig("unknown weight id");
+        }
+    }
     static uint16_t to_bf16(float f) {
         uint32_t b;
         std::memcpy(&b, &f, 4);
