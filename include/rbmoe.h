@@ -274,7 +274,8 @@ int rbmoe_forward_block_host(rbmoe_layer* layer, const void* x, int32_t tokens, 
  * rbmoe_join_forward has it (below).  post_weight and gate are HOST [d_model] f32 or NULL; both NULL with scale 1 is the residual add
  * again.  From then on rbmoe_forward_block and rbmoe_backward_block (and their host forms) include it; padding rows pass x through, the
  * shared expert's rows included.  In training mode the gradients of post_weight and gate accumulate like the norm's
- * (RBMOE_W_POST_NORM, RBMOE_W_BLOCK_GATE).  Needs the feed-forward norm; a backward pass for a forward from before this call is refused. */
+ * (RBMOE_W_POST_NORM, RBMOE_W_BLOCK_GATE).  Needs the feed-forward norm; a backward pass for a forward from before this call is refused.
+ * (rbmoe_backward behind a joined block step is the layer's alone: its grad_output is that of the layer's rows.) */
 int rbmoe_set_block_join(rbmoe_layer* layer, const float* post_weight, const float* gate, int32_t cols, float eps, float scale);
 
 /* ---- backward pass (MoeLayer::backward, src/moe.rs:348-489) ------------------------------
@@ -341,7 +342,7 @@ typedef enum rbmoe_gate {
     RBMOE_GATE_ROW = 2      /* [rows, cols] of the rows' dtype */
 } rbmoe_gate;
 typedef struct rbmoe_join rbmoe_join;
-/* Holds the workspace of the backward pass (counted against the context's budget).  1 to 65536 columns. */
+/* Holds the workspace of the backward pass (counted against the context's budget).  1 to 65536 columns; calls take up to 2^30 rows. */
 int rbmoe_join_create(rbmoe_ctx* ctx, int32_t cols, int32_t dtype, int32_t gate, rbmoe_join** out);
 void rbmoe_join_destroy(rbmoe_join* join);
 /* Enqueued on the context's stream; allocates nothing. */
@@ -364,7 +365,7 @@ int rbmoe_join_backward(rbmoe_join* join, int32_t rows, const void* y, const voi
  * and 8 bytes a squared shorter side, counted against the context's budget.
  * rbmoe_orthogonalize brings the singular values of every matrix near one: X = U / (|U|_F + 1e-7), then `steps` times
  *   A = X X^T, B = b A + c A A, X = a X + B X,  (a, b, c) = (3.4445, -4.7750, 2.0315)
- * (five steps: values from 0.003 |U|_F up end in [0.68, 1.21]).  Accuracy is f32's whatever the types of `in` and `out`, each RBMOE_F32 or
+ * (five steps: values from 0.003 |U|_F up end in [0.68, 1.21]; elements below 2^-38 |U|_F count as zero).  Accuracy is f32's whatever the types of `in` and `out`, each RBMOE_F32 or
  * RBMOE_BF16; `out` may be `in`.  A matrix of zeros stays one.
  * rbmoe_muon_step is an optimiser step with it (decoupled weight decay):
  *   M = momentum_factor M + G,  U = G + momentum_factor M (nesterov != 0) or M,

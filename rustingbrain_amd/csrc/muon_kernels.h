@@ -49,6 +49,10 @@ inline float muon_scale(float given, int rows, int cols) {
     return given > 0.0f ? given : std::sqrt(std::max(1.0f, (float)rows / (float)cols));
 }
 
+// The kernel that takes a product (0: A, 1: B, 2: X) of a call.
+enum class MuonTile { Split32, Split64, Rows64, Rows128 };
+MuonTile muon_tile(int count, int rows, int cols, int product);
+
 size_t muon_workspace_bytes(int count, int rows, int cols);
 hipError_t launch_muon(const MuonCall& c, hipStream_t s);
 

@@ -746,17 +746,36 @@ hipError_t launch_split(const ProductArgs& a, int count, hipStream_t s) {
 // multiplies for every byte) needs two workgroups a unit: 16 x [768, 1408], 192 of them for A 62 us / 72, 576 for X 117 / 106; 128 x [704, 1024], 1536
 // for A 305 / 272, 3072 for X 553 / 430.
 template <Product kind>
-hipError_t launch_product(const ProductArgs& a, int count, hipStream_t s) {
+MuonTile tile_of(const ProductArgs& a, int count) {
     const long long tiles = (long long)split_tiles_of<kind, 2>(a) * count;  // of 64 x 64
-    if (tiles * 5 <= kUnits * 2) return launch_split<kind, 1, 8>(a, count, s);
-    if (tiles * 5 <= kUnits * 4) return launch_split<kind, 2, 4>(a, count, s);
-    if ((long long)tiles_of<kind, 4, 2>(a) * count < 2 * kUnits) return launch_tiles<kind, 2, 1>(a, count, s);
+    if (tiles * 5 <= kUnits * 2) return MuonTile::Split32;
+    if (tiles * 5 <= kUnits * 4) return MuonTile::Split64;
+    return (long long)tiles_of<kind, 4, 2>(a) * count < 2 * kUnits ? MuonTile::Rows64 : MuonTile::Rows128;
+}
+
+template <Product kind>
+hipError_t launch_product(const ProductArgs& a, int count, hipStream_t s) {
+    switch (tile_of<kind>(a, count)) {
+        case MuonTile::Split32: return launch_split<kind, 1, 8>(a, count, s);
+        case MuonTile::Split64: return launch_split<kind, 2, 4>(a, count, s);
+        case MuonTile::Rows64: return launch_tiles<kind, 2, 1>(a, count, s);
+        case MuonTile::Rows128: break;
+    }
     return launch_tiles<kind, 4, 2>(a, count, s);
 }
 
 size_t rounded(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 }  // namespace
+
+MuonTile muon_tile(int count, int rows, int cols, int product) {
+    const Shape s = shape_of(rows, cols);
+    ProductArgs a{};
+    a.s = s;
+    a.pg = s.mg;
+    a.qg = product == 2 ? s.ng : s.mg;
+    return product == 2 ? tile_of<kApply>(a, count) : tile_of<kGram>(a, count);
+}
 
 size_t muon_workspace_bytes(int count, int rows, int cols) {
     const Shape s = shape_of(rows, cols);

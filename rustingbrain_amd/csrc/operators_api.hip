@@ -28,13 +28,14 @@ struct rbmoe_muon {
 
 namespace {
 
-constexpr int kMostJoinCols = 1 << 16, kMostMuonCount = 65535;
+constexpr int kMostJoinCols = 1 << 16, kMostJoinRows = 1 << 30, kMostMuonCount = 65535;
 
 bool off_element(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == RBMOE_BF16 ? 2 : 4) != 0; }
 
 // What both directions of a join ask of their common arguments.
 int join_problem(rbmoe_join* j, int32_t rows, const void* gate, float scale, float eps) {
     if (rows < 0) return fail(j->ctx, RBMOE_INVALID_INPUT, "the row count must not be negative");
+    if (rows > kMostJoinRows) return fail(j->ctx, RBMOE_UNSUPPORTED, "more than 2^30 rows");
     if (rows > 0 && (j->gate != RBMOE_GATE_NONE) != (gate != nullptr))
         return fail(j->ctx, gate ? RBMOE_INVALID_INPUT : RBMOE_NULL_POINTER,
                     gate ? "this join was created without a gate" : "gate is NULL");
@@ -233,6 +234,11 @@ int rbmoe_muon_step(rbmoe_muon* m, const void* grad, int32_t grad_dtype, float* 
     c.workspace = m->workspace;
     HIP_TRY(ctx, launch_muon(c, ctx->stream));
     return RBMOE_OK;
+}
+
+// Which kernel takes a product (0: A, 1: B, 2: X) of a call: for tests (no GPU needed).
+int rbmoe_internal_muon_tile(int32_t count, int32_t rows, int32_t cols, int32_t product) {
+    return static_cast<int>(muon_tile(count, rows, cols, product));
 }
 
 }  // extern "C"

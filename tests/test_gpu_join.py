@@ -195,6 +195,37 @@ def test_in_place_and_accumulated(device, dtype, cols):
     check_forward(p, in_place=True)
 
 
+@pytest.mark.parametrize("dtype,cols", [("bf16", 1024), ("f32", 300), ("f32", 9001)])
+def test_input_gradients_may_take_the_place_of_what_they_are_made_from(device, dtype, cols):
+    p = Problem(device, 21, cols, dtype, "row", padding=True)
+    stream = stored(np.random.default_rng(8).standard_normal((21, cols)), dtype)
+    apart = check_backward(p, stream)
+    out, gate = Array(device, stream.shape, dtype, stream), p.empty(p.x, dtype)
+    p.join.backward_device(21, p.d["y"].ptr, out.ptr, p.d["go"].ptr, p.d["gn"].ptr, p.d["go"].ptr, p.d["gn"].ptr, grad_gate_ptr=gate.ptr,
+                           **p.common())
+    device.synchronize()
+    assert np.array_equal(p.d["go"].get(), apart["grad_x"]) and np.array_equal(p.d["gn"].get(), apart["grad_y"])
+    assert np.array_equal(gate.get(), apart["grad_gate"])
+
+
+def test_parts_of_the_backward_pass_left_out(device):
+    """No gradient of a parameter wanted, and none behind the add: the others are what they are with them."""
+    p = Problem(device, 33, 512, "bf16", "channel")
+    stream = stored(np.random.default_rng(8).standard_normal((33, 512)), "bf16")
+    whole = check_backward(p, stream)
+    out = Array(device, stream.shape, "bf16", stream)
+    gx, gy, zeros = p.empty(p.x, "bf16"), p.empty(p.x, "bf16"), Array(device, p.x.shape, "bf16", np.zeros_like(p.x))
+    p.join.backward_device(33, p.d["y"].ptr, out.ptr, p.d["go"].ptr, p.d["gn"].ptr, gx.ptr, gy.ptr, **p.common())
+    device.synchronize()
+    assert np.array_equal(gx.get(), whole["grad_x"]) and np.array_equal(gy.get(), whole["grad_y"])
+    got = []
+    for go in (0, zeros.ptr):
+        p.join.backward_device(33, p.d["y"].ptr, out.ptr, go, p.d["gn"].ptr, gx.ptr, gy.ptr, **p.common())
+        device.synchronize()
+        got.append((gx.get(), gy.get()))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
+
+
 def test_more_rows_than_one_round_of_workgroups(device):
     for dtype, rows, cols in (("bf16", 5003, 512), ("f32", 2500, 96), ("bf16", 700, 3000)):
         p = Problem(device, rows, cols, dtype, "channel", padding=True)
@@ -245,6 +276,8 @@ def test_refusals(device):
                 dict(normed=out.ptr, next_weight_ptr=d["next"].ptr)):
         with pytest.raises(rb.InvalidInput):
             fwd(**bad)
+    with pytest.raises(rb.Unsupported):
+        p.join.forward_device((1 << 30) + 1, d["x"].ptr, d["y"].ptr, out.ptr, **{**ok, "next_weight_ptr": 0})
     for rows, x, y, o in ((-1, 1, 1, 1), (4, 0, 1, 1), (4, 1, 0, 1), (4, 1, 1, 0)):
         with pytest.raises(rb.InvalidInput):
             p.join.forward_device(rows, x and d["x"].ptr, y and d["y"].ptr, o and out.ptr, **{**ok, "next_weight_ptr": 0})
