@@ -92,6 +92,17 @@ __device__ __forceinline__ void load_parameter(const float* p, float (&v)[V]) {
     }
 }
 
+template <int V>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) *reinterpret_cast<float4*>(p + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = v[i];
+    }
+}
+
 // What the stored row holds for an f32 value.
 template <typename XT>
 __device__ __forceinline__ float as_stored(float v) {
@@ -390,38 +401,40 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
         }
         if constexpr (G > 64) __syncthreads();  // `room` is written again
     }
-    // the sums of the workgroup's waves, in wave order
+    // the sums of the workgroup: where it has several waves, added in wave order, every thread some columns
+    const bool add = gridDim.x == 1 && a.accumulate;
+    auto place = [&](int k) { return gridDim.x == 1 ? sum_target(a, k) : a.partial + ((size_t)blockIdx.x * 3 + k) * d; };
+    if constexpr (RPB > 1) {
+        __shared__ __align__(16) float stage[3][RPB][P * G * V];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        float* const target = sum_target(a, k);
-        if (!target) continue;  // uniform
-        float* const dst = gridDim.x == 1 ? target : a.partial + ((size_t)blockIdx.x * 3 + k) * d;
-        const bool add = gridDim.x == 1 && a.accumulate;
-        if constexpr (RPB > 1) {
-            __shared__ float stage[RPB - 1][P * G * V];
-            const int wave = threadIdx.x / G;
-            __syncthreads();  // the previous array has been read out
-            if (wave > 0)
+        for (int k = 0; k < 3; ++k)
+            if (sum_target(a, k))  // uniform
 #pragma unroll
-                for (int p = 0; p < P; ++p)
+                for (int p = 0; p < P; ++p) store_floats<V>(stage[k][threadIdx.x / G] + (p * G + lane) * V, sums[k][p]);
+        __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < V; ++i) stage[wave - 1][(p * V + i) * G + lane] = sums[k][p][i];
-            __syncthreads();
-            if (wave == 0)
+        for (int k = 0; k < 3; ++k) {
+            if (!sum_target(a, k)) continue;
+            float* const dst = place(k);
+            for (int c = threadIdx.x; c < d; c += 256) {
+                float v = stage[k][0][c];
 #pragma unroll
-                for (int p = 0; p < P; ++p)
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-#pragma unroll
-                        for (int w = 0; w < RPB - 1; ++w) sums[k][p][i] += stage[w][(p * V + i) * G + lane];
-            if (wave != 0) continue;
+                for (int w = 1; w < RPB; ++w) v += stage[k][w][c];
+                dst[c] = v + (add ? dst[c] : 0.0f);
+            }
         }
+    } else {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const int c = (p * G + lane) * V;
-            if (c >= d) continue;
+        for (int k = 0; k < 3; ++k) {
+            if (!sum_target(a, k)) continue;
+            float* const dst = place(k);
 #pragma unroll
-            for (int i = 0; i < V; ++i) dst[c + i] = sums[k][p][i] + (add ? dst[c + i] : 0.0f);
+            for (int p = 0; p < P; ++p) {
+                const int c = (p * G + lane) * V;
+                if (c >= d) continue;
+#pragma unroll
+                for (int i = 0; i < V; ++i) dst[c + i] = sums[k][p][i] + (add ? dst[c + i] : 0.0f);
+            }
         }
     }
 }
@@ -596,7 +609,9 @@ hipError_t backward(const JoinBackward& a, hipStream_t s) {
         a.cols, elements_of(a.cols, sizeof(XT) == 2, rows, parameters),
         [&](auto v, auto p, auto g) {
             constexpr int V = decltype(v)::value, P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
-            parts = std::min((a.rows + RPB - 1) / RPB, most);
+            // as many rows for every wave (or workgroup) as the busiest has
+            const int turns = (a.rows + RPB - 1) / RPB, each = (turns + most - 1) / most;
+            parts = (turns + each - 1) / each;
             final = parts == 1;
             hipLaunchKernelGGL((join_backward_kernel<XT, V, P, G>), dim3(parts), dim3(256), 0, s, a);
             return hipGetLastError();
