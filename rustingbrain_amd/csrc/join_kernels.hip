@@ -16,7 +16,7 @@
 //   grad_y    = t v - y t^3 (y . v) / d
 //   grad_post = sum_rows db * y * t       grad_next = sum_rows grad_normed * out * s
 // us a call (bytes a second): forward 16384 x 1024 bf16 29.6 (4.5 TB/s; a copy of as much 5.2), 1 x 512 5.1, of which the launch is 2.8;
-// backward 16384 x 1024 bf16 47 (4.3 TB/s), 1024 x 512 f32 9.2 (two launches of 5.5 and 3).
+// backward 16384 x 1024 bf16 46.3 (4.3 TB/s), 1024 x 512 f32 9.2 (launches of 6 and 3).
 // Each of the three parameter gradients is a sum over rows: a wave (or workgroup) takes every n-th row and keeps the sums of
 // its columns in registers; workgroups then leave them in memory and a second, small launch adds them in a fixed order, so
 // the same call gives the same bits.
@@ -512,24 +512,26 @@ __global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) 
     }
 }
 
-// The workgroups' sums, added in the order of the workgroups: 32 columns a workgroup, 32 threads a column, each over every
-// 32nd workgroup with its loads all under way together.
-__global__ __launch_bounds__(1024) void join_sums_kernel(JoinBackward a, int parts) {
+// The workgroups' sums, added in the order of the workgroups: 32 columns a workgroup, 16 threads a column, each over every
+// 16th workgroup with its loads under way together.  us a backward call of 1024 x 512 f32 / 3001 x 760 bf16 / 16384 x 1024 bf16: 8 threads 9.7 / 15.5 /
+// 48.0, 16 9.2 / 14.5 / 46.3, 32 10.6 / 15.1 / 46.5.
+constexpr int kSumSlices = 16;
+__global__ __launch_bounds__(32 * kSumSlices) void join_sums_kernel(JoinBackward a, int parts) {
     float* const dst = sum_target(a, blockIdx.y);
     if (!dst) return;
-    __shared__ float room[32][33];
+    __shared__ float room[kSumSlices][33];
     const int d = a.cols, c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
     float s = 0.0f;
     if (c < d) {
         const float* src = a.partial + (size_t)blockIdx.y * d + c;
 #pragma unroll 16
-        for (int b = slice; b < parts; b += 32) s += src[(size_t)b * 3 * d];
+        for (int b = slice; b < parts; b += kSumSlices) s += src[(size_t)b * 3 * d];
     }
     room[slice][threadIdx.x & 31] = s;
     __syncthreads();
     if (slice == 0 && c < d) {
 #pragma unroll
-        for (int w = 1; w < 32; ++w) s += room[w][threadIdx.x & 31];
+        for (int w = 1; w < kSumSlices; ++w) s += room[w][threadIdx.x & 31];
         dst[c] = s + (a.accumulate ? dst[c] : 0.0f);
     }
 }
@@ -583,7 +585,7 @@ constexpr int kMostParts = 512;
 
 hipError_t add_parts(const JoinBackward& a, int parts, hipStream_t s) {
     if (!a.grad_post && !a.grad_next && !(a.gate_mode == RBMOE_GATE_CHANNEL && a.grad_gate)) return hipSuccess;
-    hipLaunchKernelGGL(join_sums_kernel, dim3((a.cols + 31) / 32, 3), dim3(1024), 0, s, a, parts);
+    hipLaunchKernelGGL(join_sums_kernel, dim3((a.cols + 31) / 32, 3), dim3(32 * kSumSlices), 0, s, a, parts);
     return hipGetLastError();
 }
 
