@@ -12,10 +12,10 @@
 // the f32 ones.  (Two bf16 parts hold 16 bits, and five steps of them end 1e-5 from the exact result where f32 ends 2e-6.)
 //
 // What bounds it.  Large stacks: 128 x [704, 1024] f32 takes 4.8 ms a step, 0.46 of them the passes over gradients, momentum and weights
-// at the rate of a copy.  The rest is 3.6 TFLOP of fp16 multiplies (both triangles of A and B counted once), 0.83 PFLOP/s where a large fp16 product of the
-// library reaches 1.08 on such numbers: without its output a launch's loop runs at 1.25, and writing X both ways (0.74 GB a step) and A and B takes the
-// difference; two products of different kinds in one launch, so that one's output falls into the other's multiplies, took as long.  Small
-// ones: every launch starts on cold second-level caches and writes its output through at the end, 3 to 5 us for 17 launches (1 x [512, 512] 79 us).
+// at the rate of a copy.  The rest is 3.6 TFLOP of fp16 multiplies (A and B counted by halves), 0.83 PFLOP/s where a large fp16 product of
+// the library reaches 1.08: a launch without its output runs at 1.25 over all the blocks that its tiles cover, and the blocks below
+// the diagonal and the output (0.74 GB for X, 0.25 for A and for B) take the difference.  Small ones: every launch starts on cold second-level caches and
+// writes its output through at the end, 3 to 6 us for 17 launches (1 x [512, 512] 79 us).
 //
 // Layout.  Operands lie in the order in which the matrix cores take them: a fragment is 32 rows x 16 columns of the reduction, lane l
 // holds row l % 32, columns 8 (l / 32) .. + 7, so 64 lanes x 16 bytes hold the hi parts of a fragment and the 1024 bytes behind them
