@@ -150,21 +150,27 @@ struct Pack {
     char* xt;
 };
 
-// A workgroup takes 64 x 64 of X (m by n).
+// A workgroup takes 32 x 64 of X (m by n).
 template <typename GT>
 __global__ __launch_bounds__(256) void muon_pack_kernel(Pack a) {
-    __shared__ float tile[64][65];
+    __shared__ float tile[32][65];
     __shared__ double norm2;
     const Front& f = a.f;
     const int i = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const GT* const g = static_cast<const GT*>(f.grad.p) + i * f.grad.stride;
     const float* const mo = f.update ? static_cast<const float*>(f.momentum.p) + i * f.momentum.stride : nullptr;
-    const int p0 = blockIdx.x * 64, q0 = blockIdx.y * 64;  // of X
-    const int r0 = a.tall ? q0 : p0, c0 = a.tall ? p0 : q0; // of the matrix as it lies
-    float gv[16], m[16];
+    const int p0 = blockIdx.x * 32, q0 = blockIdx.y * 64;  // of X
+    // element k of this thread: neighbouring threads along the rows as they lie
+    auto place = [&](int k, int& p, int& q) {
+        p = a.tall ? tid & 31 : k * 4 + wave;
+        q = a.tall ? k * 8 + (tid >> 5) : lane;
+    };
+    float gv[8], m[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        const int r = r0 + k * 4 + wave, c = c0 + lane;
+    for (int k = 0; k < 8; ++k) {
+        int p, q;
+        place(k, p, q);
+        const int r = a.tall ? q0 + q : p0 + p, c = a.tall ? p0 + p : q0 + q;
         const bool in = r < f.rows && c < f.cols;
         gv[k] = in ? to_f32(g[(size_t)r * f.grad.pitch + c]) : 0.0f;
         m[k] = in && f.update ? mo[(size_t)r * f.momentum.pitch + c] : 0.0f;
@@ -179,34 +185,31 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Pack a) {
     __syncthreads();
     const double factor = (double)kUp / (sqrt(norm2) + 1e-7);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        const float v = (float)((double)direction(gv[k], m[k], f.update, f.nesterov, f.mu) * factor);
-        if (a.tall) tile[lane][k * 4 + wave] = v; else tile[k * 4 + wave][lane] = v;
+    for (int k = 0; k < 8; ++k) {
+        int p, q;
+        place(k, p, q);
+        tile[p][q] = (float)((double)direction(gv[k], m[k], f.update, f.nesterov, f.mu) * factor);
     }
     __syncthreads();
-    // 2 groups of rows x 4 columns steps x 64 lanes, each way
+    // a fragment a wave each way: of X one group of rows and four steps, of X^T two groups and two steps
 #pragma unroll
     for (int way = 0; way < 2; ++way) {
         char* const base = (way ? a.xt : a.x) + (size_t)i * a.s.x_bytes();
         const int groups = way ? a.s.ng : a.s.mg, steps = 2 * (way ? a.s.mg : a.s.ng);
+        const int group = way ? q0 / 32 + wave / 2 : p0 / 32, step = way ? p0 / 16 + wave % 2 : q0 / 16 + wave;
+        if (group >= groups || step >= steps) continue;
+        const int row = (way ? 32 * (wave / 2) : 0) + (lane & 31), col = 16 * (way ? wave % 2 : wave) + 8 * (lane >> 5);
+        halfx8 hi, lo;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int block = k * 4 + wave;
-            const int group = (way ? q0 : p0) / 32 + block / 4, step = (way ? p0 : q0) / 16 + block % 4;
-            if (group >= groups || step >= steps) continue;
-            const int row = (block / 4) * 32 + (lane & 31), col = (block % 4) * 16 + 8 * (lane >> 5);
-            halfx8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                _Float16 h, l;
-                split(way ? tile[col + e][row] : tile[row][col + e], h, l);
-                hi[e] = h;
-                lo[e] = l;
-            }
-            char* const at = base + ((size_t)group * steps + step) * kFragment + lane * 16;
-            *reinterpret_cast<halfx8*>(at) = hi;
-            *reinterpret_cast<halfx8*>(at + 1024) = lo;
+        for (int e = 0; e < 8; ++e) {
+            _Float16 h, l;
+            split(way ? tile[col + e][row] : tile[row][col + e], h, l);
+            hi[e] = h;
+            lo[e] = l;
         }
+        char* const at = base + ((size_t)group * steps + step) * kFragment + lane * 16;
+        *reinterpret_cast<halfx8*>(at) = hi;
+        *reinterpret_cast<halfx8*>(at + 1024) = lo;
     }
 }
 
@@ -803,7 +806,7 @@ hipError_t launch_muon(const MuonCall& c, hipStream_t s) {
     }
     am = at;
     bm = at + c.count * sh.a_bytes();
-    const dim3 fg(f.parts, c.count), pgrid((sh.mg + 1) / 2, (sh.ng + 1) / 2, c.count);
+    const dim3 fg(f.parts, c.count), pgrid(sh.mg, (sh.ng + 1) / 2, c.count);
     const Pack pk{f, sh, tall, x, xt[0]};
     const size_t elements = (size_t)c.rows * c.cols;
     auto fours = [&](const MuonStack& st, int size) {  // four neighbouring elements at once, wherever they stand
