@@ -28,80 +28,90 @@ namespace rbmoe {
 
 namespace {
 
-// V neighbouring elements of a row.
-template <typename XT, int V>
-struct Piece;
-template <>
-struct Piece<float, 4> {
-    float4 raw;
-    __device__ __forceinline__ void load(const float* p) { raw = *reinterpret_cast<const float4*>(p); }
-    __device__ __forceinline__ void zero() { raw = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
-    __device__ __forceinline__ void widen(float (&v)[4]) const { v[0] = raw.x; v[1] = raw.y; v[2] = raw.z; v[3] = raw.w; }
-    static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    }
-};
-template <>
-struct Piece<float, 1> {
-    float raw;
-    __device__ __forceinline__ void load(const float* p) { raw = *p; }
-    __device__ __forceinline__ void zero() { raw = 0.0f; }
-    __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = raw; }
-    static __device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
-};
-template <>
-struct Piece<bf16_t, 8> {
+// 16 bytes of a row, or of a parameter [d] (f32).  `A`: they start on a 16-byte boundary, and rows are whole pieces.  Otherwise they may start
+// at any element (global memory takes 16-byte accesses at any address), and a row's last piece may have fewer elements: it is read as
+// the 16 bytes that end with the row, and settle() moves it down once the loads are under way.  So these rows have V elements at least.
+// What such a read holds of the lane before, which may be storing its piece in place, goes unused.
+typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef uint32_t Any8 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+typedef uint32_t Any4 __attribute__((aligned(2), may_alias));
+typedef uint16_t Any2 __attribute__((may_alias));
+
+template <typename XT, bool A>
+struct Piece {
+    static constexpr int V = 16 / sizeof(XT);
     uint4 raw;
-    __device__ __forceinline__ void load(const bf16_t* p) { raw = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void widen(float (&v)[8]) const { Vec16<bf16_t>::widen(raw, v); }
-    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[8]) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+    // p[0 .. n) of a row that ends at p + n, where n < V; nothing of it where n <= 0
+    __device__ __forceinline__ void load(const XT* p, int n) {
+        if (n <= 0) {
+            zero();
+        } else if constexpr (A) {
+            raw = *reinterpret_cast<const uint4*>(p);
+        } else {
+            const Any16 v = *reinterpret_cast<const Any16*>(p - (V - min(n, V)));
+            raw = make_uint4(v.x, v.y, v.z, v.w);
+        }
     }
-};
-template <>
-struct Piece<bf16_t, 2> {
-    uint32_t raw;
-    __device__ __forceinline__ void load(const bf16_t* p) { raw = *reinterpret_cast<const uint32_t*>(p); }
-    __device__ __forceinline__ void zero() { raw = 0; }
-    __device__ __forceinline__ void widen(float (&v)[2]) const {
-        v[0] = __uint_as_float(raw << 16);
-        v[1] = __uint_as_float(raw & 0xffff0000u);
+    // elements 0 .. n in their places, zeros behind them
+    __device__ __forceinline__ void settle(int n) {
+        if constexpr (!A) {
+            if (n <= 0 || n >= V) return;
+            const int away = V - n, words = sizeof(XT) == 2 ? away >> 1 : away;
+            if (words & 2) raw = make_uint4(raw.z, raw.w, 0, 0);
+            if (words & 1) raw = make_uint4(raw.y, raw.z, raw.w, 0);
+            if (sizeof(XT) == 2 && (away & 1))
+                raw = make_uint4(raw.x >> 16 | raw.y << 16, raw.y >> 16 | raw.z << 16, raw.z >> 16 | raw.w << 16, raw.w >> 16);
+        }
     }
-    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[2]) { *reinterpret_cast<uint32_t*>(p) = pack2(v[0], v[1]); }
-};
-template <>
-struct Piece<bf16_t, 1> {
-    uint16_t raw;
-    __device__ __forceinline__ void load(const bf16_t* p) { raw = p->bits; }
-    __device__ __forceinline__ void zero() { raw = 0; }
-    __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = bf16_bits_to_f32(raw); }
-    static __device__ __forceinline__ void store(bf16_t* p, const float (&v)[1]) { p->bits = f32_to_bf16_bits(v[0]); }
+    __device__ __forceinline__ void widen(float (&v)[V]) const { Vec16<XT>::widen(raw, v); }
+    // n > 0
+    static __device__ __forceinline__ void store(XT* p, const float (&v)[V], int n) {
+        uint4 o;
+        if constexpr (sizeof(XT) == 2) o = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+        else o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        if constexpr (A) {
+            *reinterpret_cast<uint4*>(p) = o;
+        } else if (n >= V) {
+            *reinterpret_cast<Any16*>(p) = Any16{o.x, o.y, o.z, o.w};
+        } else {
+            constexpr int W = 4 / sizeof(XT);  // elements of a word
+            if (n & 2 * W) {
+                *reinterpret_cast<Any8*>(p) = Any8{o.x, o.y};
+                o.x = o.z, o.y = o.w;
+                p += 2 * W;
+            }
+            if (n & W) {
+                *reinterpret_cast<Any4*>(p) = o.x;
+                o.x = o.y;
+                p += W;
+            }
+            if constexpr (W == 2)
+                if (n & 1) *reinterpret_cast<Any2*>(p) = (uint16_t)o.x;
+        }
+    }
 };
 
-// V values of a parameter [d] (f32)
-template <int V>
-__device__ __forceinline__ void load_parameter(const float* p, float (&v)[V]) {
-    if constexpr (V % 4 == 0) {
+// V values of a parameter at a column with n of the row's left (n > 0), and back
+template <int V, bool A>
+__device__ __forceinline__ void load_parameter(const float* p, float (&v)[V], int n) {
+    Piece<float, A> a[V / 4];
 #pragma unroll
-        for (int q = 0; q < V / 4; ++q) {
-            const float4 a = *reinterpret_cast<const float4*>(p + 4 * q);
-            v[4 * q] = a.x; v[4 * q + 1] = a.y; v[4 * q + 2] = a.z; v[4 * q + 3] = a.w;
-        }
-    } else {
+    for (int q = 0; q < V / 4; ++q) a[q].load(p + 4 * q, A ? V : n - 4 * q);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = p[i];
+    for (int q = 0; q < V / 4; ++q) {
+        a[q].settle(n - 4 * q);
+        float w[4];
+        a[q].widen(w);
+        v[4 * q] = w[0]; v[4 * q + 1] = w[1]; v[4 * q + 2] = w[2]; v[4 * q + 3] = w[3];
     }
 }
-
-template <int V>
-__device__ __forceinline__ void store_floats(float* p, const float (&v)[V]) {
-    if constexpr (V % 4 == 0) {
+template <int V, bool A>
+__device__ __forceinline__ void store_parameter(float* p, const float (&v)[V], int n) {
 #pragma unroll
-        for (int q = 0; q < V / 4; ++q) *reinterpret_cast<float4*>(p + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = v[i];
+    for (int q = 0; q < V / 4; ++q) {
+        const float w[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        if (A || n > 4 * q) Piece<float, A>::store(p + 4 * q, w, n - 4 * q);
     }
 }
 
@@ -146,9 +156,9 @@ __device__ __forceinline__ float inverse_rms(float sum_of_squares, int d, float 
 }
 
 // ---- forward -----------------------------------------------------------------------------------
-template <typename XT, int V, int P, int G>
+template <typename XT, bool A, int P, int G>
 __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
-    constexpr int RPB = 256 / G;  // rows of a workgroup
+    constexpr int V = Piece<XT, A>::V, RPB = 256 / G;  // elements of a piece, rows of a workgroup
     __shared__ float room[2][4];
     const int lane = threadIdx.x % G, d = a.cols;
     const int row = blockIdx.x * RPB + threadIdx.x / G;
@@ -157,13 +167,18 @@ __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
     const XT* const x = static_cast<const XT*>(a.x) + at;
     const XT* const y = static_cast<const XT*>(a.y) + at;
     const bool live = a.valid == nullptr || a.valid[row] != 0;
-    Piece<XT, V> yr[P], xr[P];
+    Piece<XT, A> yr[P], xr[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         const int c = (p * G + lane) * V;
-        const bool in = c < d;
-        if (in && live) yr[p].load(y + c); else yr[p].zero();
-        if (in) xr[p].load(x + c); else xr[p].zero();
+        yr[p].load(y + c, live ? d - c : 0);
+        xr[p].load(x + c, d - c);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int n = d - (p * G + lane) * V;
+        yr[p].settle(n);
+        xr[p].settle(n);
     }
     float factor = 1.0f;
     if (a.post) {
@@ -189,18 +204,19 @@ __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
             if (live) {
                 if (a.post) {
                     float w[V];
-                    load_parameter<V>(a.post + c, w);
+                    load_parameter<V, A>(a.post + c, w, d - c);
 #pragma unroll
                     for (int i = 0; i < V; ++i) b[i] = b[i] * factor * w[i];
                 }
                 if (a.gate_mode == RBMOE_GATE_CHANNEL) {
                     float g[V];
-                    load_parameter<V>(static_cast<const float*>(a.gate) + c, g);
+                    load_parameter<V, A>(static_cast<const float*>(a.gate) + c, g, d - c);
 #pragma unroll
                     for (int i = 0; i < V; ++i) b[i] *= g[i];
                 } else if (a.gate_mode == RBMOE_GATE_ROW) {
-                    Piece<XT, V> gr;
-                    gr.load(static_cast<const XT*>(a.gate) + at + c);
+                    Piece<XT, A> gr;
+                    gr.load(static_cast<const XT*>(a.gate) + at + c, d - c);
+                    gr.settle(d - c);
                     float g[V];
                     gr.widen(g);
 #pragma unroll
@@ -209,7 +225,7 @@ __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) out[p][i] = live ? as_stored<XT>(fmaf(a.scale, b[i], xv[i])) : xv[i];
-            Piece<XT, V>::store(static_cast<XT*>(a.out) + at + c, out[p]);
+            Piece<XT, A>::store(static_cast<XT*>(a.out) + at + c, out[p], d - c);
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) out[p][i] = 0.0f;
@@ -225,10 +241,10 @@ __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
         const int c = (p * G + lane) * V;
         if (c < d) {
             float w[V];
-            load_parameter<V>(a.next + c, w);
+            load_parameter<V, A>(a.next + c, w, d - c);
 #pragma unroll
             for (int i = 0; i < V; ++i) w[i] = out[p][i] * f2 * w[i];
-            Piece<XT, V>::store(static_cast<XT*>(a.normed) + at + c, w);
+            Piece<XT, A>::store(static_cast<XT*>(a.normed) + at + c, w, d - c);
         }
     }
 }
@@ -280,9 +296,9 @@ __device__ __forceinline__ float* sum_target(const JoinBackward& a, int which) {
                                                  : a.grad_next;
 }
 
-template <typename XT, int V, int P, int G>
+template <typename XT, bool A, int P, int G>
 __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
-    constexpr int RPB = 256 / G;
+    constexpr int V = Piece<XT, A>::V, RPB = 256 / G;
     __shared__ float room[2][12];
     const int lane = threadIdx.x % G, d = a.cols;
     const float inv_d = 1.0f / (float)d;
@@ -302,27 +318,29 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) next[p][i] = 0.0f, post[p][i] = gate[p][i] = 1.0f;
         if (c >= d) continue;
-        if (has_next) load_parameter<V>(a.next + c, next[p]);
-        if (has_post) load_parameter<V>(a.post + c, post[p]);
-        if (a.gate_mode == RBMOE_GATE_CHANNEL) load_parameter<V>(static_cast<const float*>(a.gate) + c, gate[p]);
+        if (has_next) load_parameter<V, A>(a.next + c, next[p], d - c);
+        if (has_post) load_parameter<V, A>(a.post + c, post[p], d - c);
+        if (a.gate_mode == RBMOE_GATE_CHANNEL) load_parameter<V, A>(static_cast<const float*>(a.gate) + c, gate[p], d - c);
     }
     for (int row = blockIdx.x * RPB + threadIdx.x / G; row < a.rows; row += gridDim.x * RPB) {
         const size_t at = (size_t)row * d;
         const bool live = a.valid == nullptr || a.valid[row] != 0;
-        Piece<XT, V> yr[P], rr[P], gr[P], nr[P];
+        Piece<XT, A> yr[P], rr[P], gr[P], nr[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int c = (p * G + lane) * V;
-            const bool in = c < d;
-            if (in && live) yr[p].load(static_cast<const XT*>(a.y) + at + c); else yr[p].zero();
-            if (in && a.grad_out) gr[p].load(static_cast<const XT*>(a.grad_out) + at + c); else gr[p].zero();
-            if (in && has_next) {
-                rr[p].load(static_cast<const XT*>(a.out) + at + c);
-                nr[p].load(static_cast<const XT*>(a.grad_normed) + at + c);
-            } else {
-                rr[p].zero();
-                nr[p].zero();
-            }
+            yr[p].load(static_cast<const XT*>(a.y) + at + c, live ? d - c : 0);
+            gr[p].load(static_cast<const XT*>(a.grad_out) + at + c, a.grad_out ? d - c : 0);
+            rr[p].load(static_cast<const XT*>(a.out) + at + c, has_next ? d - c : 0);
+            nr[p].load(static_cast<const XT*>(a.grad_normed) + at + c, has_next ? d - c : 0);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int n = d - (p * G + lane) * V;
+            yr[p].settle(n);
+            gr[p].settle(n);
+            rr[p].settle(n);
+            nr[p].settle(n);
         }
         float s[3] = {0.0f, 0.0f, 0.0f};  // out^2, out . u, y^2
 #pragma unroll
@@ -362,15 +380,16 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
                     if (live) sums[2][p][i] = fmaf(nv[i], rv[i] * k2, sums[2][p][i]);
                 }
             }
-            if (a.grad_x) Piece<XT, V>::store(static_cast<XT*>(a.grad_x) + at + c, D[p]);
+            if (a.grad_x) Piece<XT, A>::store(static_cast<XT*>(a.grad_x) + at + c, D[p], d - c);
             // from here on D is the gradient of what the gate let through, then of the norm's output
             float yv[V], g[V];
             yr[p].widen(yv);
 #pragma unroll
             for (int i = 0; i < V; ++i) g[i] = gate[p][i];
             if (a.gate_mode == RBMOE_GATE_ROW && live) {
-                Piece<XT, V> q;
-                q.load(static_cast<const XT*>(a.gate) + at + c);
+                Piece<XT, A> q;
+                q.load(static_cast<const XT*>(a.gate) + at + c, d - c);
+                q.settle(d - c);
                 q.widen(g);
             }
             float dg[V];
@@ -384,7 +403,7 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
                 D[p][i] = has_post ? db * post[p][i] : db;
                 yv_dot[0] = fmaf(yv[i], D[p][i], yv_dot[0]);
             }
-            if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) Piece<XT, V>::store(static_cast<XT*>(a.grad_gate) + at + c, dg);
+            if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) Piece<XT, A>::store(static_cast<XT*>(a.grad_gate) + at + c, dg, d - c);
         }
         float back1 = 0.0f;
         if (has_post) {
@@ -399,7 +418,7 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
             yr[p].widen(yv);
 #pragma unroll
             for (int i = 0; i < V; ++i) yv[i] = live ? k1 * D[p][i] - yv[i] * back1 : 0.0f;
-            Piece<XT, V>::store(static_cast<XT*>(a.grad_y) + at + c, yv);
+            Piece<XT, A>::store(static_cast<XT*>(a.grad_y) + at + c, yv, d - c);
         }
         if constexpr (G > 64) __syncthreads();  // `room` is written again
     }
@@ -412,7 +431,7 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
         for (int k = 0; k < 3; ++k)
             if (sum_target(a, k))  // uniform
 #pragma unroll
-                for (int p = 0; p < P; ++p) store_floats<V>(stage[k][threadIdx.x / G] + (p * G + lane) * V, sums[k][p]);
+                for (int p = 0; p < P; ++p) store_parameter<V, true>(stage[k][threadIdx.x / G] + (p * G + lane) * V, sums[k][p], V);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
@@ -434,12 +453,13 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
             for (int p = 0; p < P; ++p) {
                 const int c = (p * G + lane) * V;
                 if (c >= d) continue;
-                if (gridDim.x > 1) {  // (partial sums lie on the same boundaries as the rows)
-                    store_floats<V>(dst + c, sums[k][p]);
-                    continue;
-                }
+                if (add) {
+                    float before[V];
+                    load_parameter<V, false>(dst + c, before, d - c);
 #pragma unroll
-                for (int i = 0; i < V; ++i) dst[c + i] = sums[k][p][i] + (add ? dst[c + i] : 0.0f);
+                    for (int i = 0; i < V; ++i) sums[k][p][i] += before[i];
+                }
+                store_parameter<V, false>(dst + c, sums[k][p], d - c);
             }
         }
     }
@@ -536,47 +556,43 @@ __global__ __launch_bounds__(32 * kSumSlices) void join_sums_kernel(JoinBackward
     }
 }
 
-// Elements of a vector access that rows of `cols` elements and these addresses allow: 16 bytes, 4, or one element.
-int elements_of(int cols, bool bf16, uintptr_t rows_at, uintptr_t parameters_at) {
-    const int es = bf16 ? 2 : 4, whole = 16 / es;
-    if (cols % whole == 0 && rows_at % 16 == 0 && parameters_at % 16 == 0) return whole;
-    if (bf16 && cols % 2 == 0 && rows_at % 4 == 0) return 2;
-    return 1;
-}
-
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// f(V, P, G) as integral constants for rows of `cols` elements by vectors of v, or `any()` where registers do not hold them.  A wave takes a
-// row of up to WAVE_ELEMENTS a lane, a workgroup one of up to GROUP_ELEMENTS a thread.  us a call, rows of 2048 bf16 by a wave / by a
+// Whether rows of `cols` elements are whole pieces on 16-byte boundaries, and the parameters lie on them too.
+bool on_pieces(int cols, int size, uintptr_t rows_at, uintptr_t parameters_at) {
+    return (size_t)cols * size % 16 == 0 && rows_at % 16 == 0 && parameters_at % 16 == 0;
+}
+
+// f(A, P, G) as integral constants for rows of `cols` elements, or `any()` where registers do not hold them.  Rows off 16 bytes by whole
+// vectors too, against two (bf16) or one element an access, us forward / backward: 1533 x 1365 f32 8.7 / 25.3 -> 7.6 / 24.3, 2000 x 1365
+// bf16 10.2 / 41.6 -> 7.8 / 23.1, 2000 x 2047 bf16 13.5 / 48.7 -> 9.6 / 25.2; 1000 x 766 bf16 6.3 / 14.7 -> 6.0 / 15.6.  A wave takes a
+// row of up to 16 elements a lane, a workgroup one of up to GROUP_ELEMENTS a thread.  us a call, rows of 2048 bf16 by a wave / by a
 // workgroup: 200 rows 6.4 / 4.9, 2000 rows 9.2 / 8.0; rows of 768: 203 rows 4.9 / 4.9, 2000 rows 5.4 / 5.6, of 1024, 4096 rows 7.8 / 8.8.
-template <typename XT, int WAVE_ELEMENTS, int GROUP_ELEMENTS, typename F, typename A>
-hipError_t with_shape(int cols, int v, F&& f, A&& any) {
-    auto pick = [&](auto vector) -> hipError_t {
-        constexpr int V = decltype(vector)::value;
+template <typename XT, int GROUP_ELEMENTS, typename F, typename N>
+hipError_t with_shape(int cols, bool whole, F&& f, N&& any) {
+    constexpr int V = 16 / sizeof(XT);
+    auto pick = [&](auto pieces) -> hipError_t {
         const int wave = (cols + 64 * V - 1) / (64 * V), group = (cols + 256 * V - 1) / (256 * V);
-        if (wave <= 1) return f(vector, std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
-        if constexpr (2 * V <= WAVE_ELEMENTS)
-            if (wave <= 2) return f(vector, std::integral_constant<int, 2>{}, std::integral_constant<int, 64>{});
-        if constexpr (4 * V <= WAVE_ELEMENTS)
-            if (wave <= 4) return f(vector, std::integral_constant<int, 4>{}, std::integral_constant<int, 64>{});
-        if constexpr (8 * V <= WAVE_ELEMENTS)
-            if (wave <= 8) return f(vector, std::integral_constant<int, 8>{}, std::integral_constant<int, 64>{});
-        if (group <= 1) return f(vector, std::integral_constant<int, 1>{}, std::integral_constant<int, 256>{});
-        if constexpr (2 * V <= GROUP_ELEMENTS)
-            if (group <= 2) return f(vector, std::integral_constant<int, 2>{}, std::integral_constant<int, 256>{});
+        if (cols < V) return any();  // no whole piece in a row
+        typedef std::integral_constant<int, 1> One;
+        typedef std::integral_constant<int, 2> Two;
+        typedef std::integral_constant<int, 4> Four;
+        typedef std::integral_constant<int, 8> Eight;
+        typedef std::integral_constant<int, 64> Wave;
+        typedef std::integral_constant<int, 256> Group;
+        if (wave <= 1) return f(pieces, One{}, Wave{});
+        if (wave <= 2) return f(pieces, Two{}, Wave{});
+        if constexpr (4 * V <= 16)
+            if (wave <= 4) return f(pieces, Four{}, Wave{});
+        if (group <= 1) return f(pieces, One{}, Group{});
+        if (group <= 2) return f(pieces, Two{}, Group{});
         if constexpr (4 * V <= GROUP_ELEMENTS)
-            if (group <= 4) return f(vector, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
+            if (group <= 4) return f(pieces, Four{}, Group{});
         if constexpr (8 * V <= GROUP_ELEMENTS)
-            if (group <= 8) return f(vector, std::integral_constant<int, 8>{}, std::integral_constant<int, 256>{});
+            if (group <= 8) return f(pieces, Eight{}, Group{});
         return any();
     };
-    if constexpr (sizeof(XT) == 2) {
-        if (v == 8) return pick(std::integral_constant<int, 8>{});
-        if (v == 2) return pick(std::integral_constant<int, 2>{});
-    } else {
-        if (v == 4) return pick(std::integral_constant<int, 4>{});
-    }
-    return pick(std::integral_constant<int, 1>{});
+    return whole ? pick(std::true_type{}) : pick(std::false_type{});
 }
 
 // Workgroups of a backward launch at most: two a compute unit, which is what their registers allow and whose sums (12 bytes a column) are
@@ -594,11 +610,11 @@ hipError_t forward(const JoinForward& a, hipStream_t s) {
     const uintptr_t rows = address(a.x) | address(a.y) | address(a.out) | address(a.normed) |
                            (a.gate_mode == RBMOE_GATE_ROW ? address(a.gate) : 0);
     const uintptr_t parameters = address(a.post) | address(a.next) | (a.gate_mode == RBMOE_GATE_CHANNEL ? address(a.gate) : 0);
-    return with_shape<XT, 16, 32>(
-        a.cols, elements_of(a.cols, sizeof(XT) == 2, rows, parameters),
-        [&](auto v, auto p, auto g) {
-            constexpr int V = decltype(v)::value, P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
-            hipLaunchKernelGGL((join_forward_kernel<XT, V, P, G>), dim3((a.rows + RPB - 1) / RPB), dim3(256), 0, s, a);
+    return with_shape<XT, 32>(
+        a.cols, on_pieces(a.cols, sizeof(XT), rows, parameters),
+        [&](auto whole, auto p, auto g) {
+            constexpr int P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
+            hipLaunchKernelGGL((join_forward_kernel<XT, decltype(whole)::value, P, G>), dim3((a.rows + RPB - 1) / RPB), dim3(256), 0, s, a);
             return hipGetLastError();
         },
         [&] {
@@ -615,15 +631,15 @@ hipError_t backward(const JoinBackward& a, hipStream_t s) {
     const int most = join_parts(a.cols);
     int parts = 0;
     bool final = false;
-    hipError_t e = with_shape<XT, 16, 16>(
-        a.cols, elements_of(a.cols, sizeof(XT) == 2, rows, parameters),
-        [&](auto v, auto p, auto g) {
-            constexpr int V = decltype(v)::value, P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
+    hipError_t e = with_shape<XT, 16>(
+        a.cols, on_pieces(a.cols, sizeof(XT), rows, parameters),
+        [&](auto whole, auto p, auto g) {
+            constexpr int P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
             // as many rows for every wave (or workgroup) as the busiest has
             const int turns = (a.rows + RPB - 1) / RPB, each = (turns + most - 1) / most;
             parts = (turns + each - 1) / each;
             final = parts == 1;
-            hipLaunchKernelGGL((join_backward_kernel<XT, V, P, G>), dim3(parts), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((join_backward_kernel<XT, decltype(whole)::value, P, G>), dim3(parts), dim3(256), 0, s, a);
             return hipGetLastError();
         },
         [&] {

@@ -187,6 +187,24 @@ def test_rows_from_any_element_on(device, dtype, cols, shift):
     check_backward(p, got.astype(np.float32))
 
 
+# (rows end 1 to 7 elements into their last 16 bytes, whatever they start on)
+@pytest.mark.parametrize("dtype,cols", [("bf16", c) for c in [*range(7, 17), *range(1017, 1032), 2049, 2055]] +
+                                       [("f32", c) for c in [*range(3, 9), *range(1021, 1029), 2050]])
+def test_rows_that_end_inside_a_vector(device, dtype, cols):
+    p = Problem(device, 9, cols, dtype, "row", padding=True, shift=cols % 3)
+    got = check_forward(p)
+    check_backward(p, got.astype(np.float32))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("dtype,cols", [("bf16", 515), ("bf16", 1029), ("bf16", 4095), ("f32", 1023), ("f32", 2050), ("f32", 4093)])
+def test_in_place_and_accumulated_at_odd_widths(device, dtype, cols, rows):
+    p = Problem(device, rows, cols, dtype, "channel", padding=rows > 1, shift=1)
+    stream = stored(np.random.default_rng(8).standard_normal((rows, cols)), dtype)
+    check_backward(p, stream, accumulate=True)
+    check_forward(p, in_place=True)
+
+
 @pytest.mark.parametrize("dtype,cols", [("bf16", 1024), ("f32", 300), ("f32", 9001)])
 def test_in_place_and_accumulated(device, dtype, cols):
     p = Problem(device, 40, cols, dtype, "channel", padding=True)
