@@ -566,9 +566,11 @@ bool on_pieces(int cols, int size, uintptr_t rows_at, uintptr_t parameters_at) {
 // f(A, P, G) as integral constants for rows of `cols` elements, or `any()` where registers do not hold them.  Rows off 16 bytes by whole
 // vectors too, against two (bf16) or one element an access, us forward / backward: 1533 x 1365 f32 8.7 / 25.3 -> 7.6 / 24.3, 2000 x 1365
 // bf16 10.2 / 41.6 -> 7.8 / 23.1, 2000 x 2047 bf16 13.5 / 48.7 -> 9.6 / 25.2; 1000 x 766 bf16 6.3 / 14.7 -> 6.0 / 15.6.  A wave takes a
-// row of up to 16 elements a lane, a workgroup one of up to GROUP_ELEMENTS a thread.  us a call, rows of 2048 bf16 by a wave / by a
+// row of up to 16 elements a lane, a workgroup one of up to 32 a thread.  us a call, rows of 2048 bf16 by a wave / by a
 // workgroup: 200 rows 6.4 / 4.9, 2000 rows 9.2 / 8.0; rows of 768: 203 rows 4.9 / 4.9, 2000 rows 5.4 / 5.6, of 1024, 4096 rows 7.8 / 8.8.
-template <typename XT, int GROUP_ELEMENTS, typename F, typename N>
+// Backward, 32 elements a thread (up to 423 registers, one wave a SIMD, nothing in memory) against rows read again: 1 x 5000 bf16
+// 34 -> 7.2, 2000 x 5001 250 -> 60, 4096 x 8192 964 -> 113, 4096 x 8192 f32 842 -> 184.
+template <typename XT, typename F, typename N>
 hipError_t with_shape(int cols, bool whole, F&& f, N&& any) {
     constexpr int V = 16 / sizeof(XT);
     auto pick = [&](auto pieces) -> hipError_t {
@@ -586,16 +588,15 @@ hipError_t with_shape(int cols, bool whole, F&& f, N&& any) {
             if (wave <= 4) return f(pieces, Four{}, Wave{});
         if (group <= 1) return f(pieces, One{}, Group{});
         if (group <= 2) return f(pieces, Two{}, Group{});
-        if constexpr (4 * V <= GROUP_ELEMENTS)
-            if (group <= 4) return f(pieces, Four{}, Group{});
-        if constexpr (8 * V <= GROUP_ELEMENTS)
+        if (group <= 4) return f(pieces, Four{}, Group{});
+        if constexpr (8 * V <= 32)
             if (group <= 8) return f(pieces, Eight{}, Group{});
         return any();
     };
     return whole ? pick(std::true_type{}) : pick(std::false_type{});
 }
 
-// Workgroups of a backward launch at most: two a compute unit, which is what their registers allow and whose sums (12 bytes a column) are
+// Workgroups of a backward launch at most: two a compute unit, which is what their registers allow up to 16 elements a thread, and whose sums (12 bytes a column) are
 // written and read again.  16384 x 1024 bf16: 512 48 us, 768 65.
 constexpr int kMostParts = 512;
 
@@ -610,7 +611,7 @@ hipError_t forward(const JoinForward& a, hipStream_t s) {
     const uintptr_t rows = address(a.x) | address(a.y) | address(a.out) | address(a.normed) |
                            (a.gate_mode == RBMOE_GATE_ROW ? address(a.gate) : 0);
     const uintptr_t parameters = address(a.post) | address(a.next) | (a.gate_mode == RBMOE_GATE_CHANNEL ? address(a.gate) : 0);
-    return with_shape<XT, 32>(
+    return with_shape<XT>(
         a.cols, on_pieces(a.cols, sizeof(XT), rows, parameters),
         [&](auto whole, auto p, auto g) {
             constexpr int P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
@@ -631,12 +632,15 @@ hipError_t backward(const JoinBackward& a, hipStream_t s) {
     const int most = join_parts(a.cols);
     int parts = 0;
     bool final = false;
-    hipError_t e = with_shape<XT, 16>(
+    hipError_t e = with_shape<XT>(
         a.cols, on_pieces(a.cols, sizeof(XT), rows, parameters),
         [&](auto whole, auto p, auto g) {
             constexpr int P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
+            // one workgroup a compute unit where a thread's 32 elements leave room for no second: 2000 x 5001 bf16 68.6 -> 59.7 us,
+            // 4096 x 8192 122 -> 113, 300 x 8190 f32 41 -> 33
+            const int limit = P * 16 / (int)sizeof(XT) >= 32 ? std::min(most, 256) : most;
             // as many rows for every wave (or workgroup) as the busiest has
-            const int turns = (a.rows + RPB - 1) / RPB, each = (turns + most - 1) / most;
+            const int turns = (a.rows + RPB - 1) / RPB, each = (turns + limit - 1) / limit;
             parts = (turns + each - 1) / each;
             final = parts == 1;
             hipLaunchKernelGGL((join_backward_kernel<XT, decltype(whole)::value, P, G>), dim3(parts), dim3(256), 0, s, a);

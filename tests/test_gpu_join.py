@@ -197,7 +197,8 @@ def test_rows_that_end_inside_a_vector(device, dtype, cols):
 
 
 @pytest.mark.parametrize("rows", [1, 40])
-@pytest.mark.parametrize("dtype,cols", [("bf16", 515), ("bf16", 1029), ("bf16", 4095), ("f32", 1023), ("f32", 2050), ("f32", 4093)])
+@pytest.mark.parametrize("dtype,cols", [("bf16", 515), ("bf16", 1029), ("bf16", 4095), ("f32", 1023), ("f32", 2050), ("f32", 4093),
+                                        ("bf16", 6000), ("bf16", 8191), ("f32", 5000), ("f32", 8189)])
 def test_in_place_and_accumulated_at_odd_widths(device, dtype, cols, rows):
     p = Problem(device, rows, cols, dtype, "channel", padding=rows > 1, shift=1)
     stream = stored(np.random.default_rng(8).standard_normal((rows, cols)), dtype)
