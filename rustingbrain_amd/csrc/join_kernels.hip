@@ -565,7 +565,8 @@ bool on_pieces(int cols, int size, uintptr_t rows_at, uintptr_t parameters_at) {
 
 // f(A, P, G) as integral constants for rows of `cols` elements, or `any()` where registers do not hold them.  Rows off 16 bytes by whole
 // vectors too, against two (bf16) or one element an access, us forward / backward: 1533 x 1365 f32 8.7 / 25.3 -> 7.6 / 24.3, 2000 x 1365
-// bf16 10.2 / 41.6 -> 7.8 / 23.1, 2000 x 2047 bf16 13.5 / 48.7 -> 9.6 / 25.2; 1000 x 766 bf16 6.3 / 14.7 -> 6.0 / 15.6.  A wave takes a
+// bf16 10.2 / 41.6 -> 7.8 / 23.1, 2000 x 2047 bf16 13.5 / 48.7 -> 9.6 / 25.2; 1000 x 766 bf16 6.3 / 14.7 -> 6.0 / 15.6,
+// 4000 x 766 8.7 / 20.6 -> 8.7 / 22.9 (even widths gain in the forward pass only).  A wave takes a
 // row of up to 16 elements a lane, a workgroup one of up to 32 a thread.  us a call, rows of 2048 bf16 by a wave / by a
 // workgroup: 200 rows 6.4 / 4.9, 2000 rows 9.2 / 8.0; rows of 768: 203 rows 4.9 / 4.9, 2000 rows 5.4 / 5.6, of 1024, 4096 rows 7.8 / 8.8.
 // Backward, 32 elements a thread (up to 423 registers, one wave a SIMD, nothing in memory) against rows read again: 1 x 5000 bf16
