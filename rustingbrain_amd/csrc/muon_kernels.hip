@@ -753,7 +753,7 @@ hipError_t launch_split(const ProductArgs& a, int count, hipStream_t s) {
 // What tells them apart is how many workgroups a launch has: under two 64 x 64 tiles for every five compute units the reduction
 // has to be split to use them, and from four for every five on the larger tiles' smaller traffic counts.  128 x 256 (twice the
 // multiplies for every byte) needs two workgroups a unit: 16 x [768, 1408], 192 of them for A 62 us / 72, 576 for X 117 / 106; 128 x [704, 1024], 1536
-// for A 305 / 272, 3072 for X 553 / 430.
+// for A 305 / 272, for X twice as many 553 / 430.
 template <Product kind>
 MuonTile tile_of(const ProductArgs& a, int count) {
     const long long tiles = (long long)split_tiles_of<kind, 2>(a) * count;  // of 64 x 64
