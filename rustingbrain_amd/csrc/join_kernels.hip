@@ -156,12 +156,19 @@ __device__ __forceinline__ float inverse_rms(float sum_of_squares, int d, float 
 }
 
 // ---- forward -----------------------------------------------------------------------------------
+// A launch holds 2^32 threads a dimension at most, which is fewer than 2^30 rows take: the workgroups of a forward launch lie in two.
+__device__ __forceinline__ int row_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 row_grid(int blocks) {
+    const int wide = std::min(blocks, 1 << 20);
+    return dim3(wide, (blocks + wide - 1) / wide);
+}
+
 template <typename XT, bool A, int P, int G>
 __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
     constexpr int V = Piece<XT, A>::V, RPB = 256 / G;  // elements of a piece, rows of a workgroup
     __shared__ float room[2][4];
     const int lane = threadIdx.x % G, d = a.cols;
-    const int row = blockIdx.x * RPB + threadIdx.x / G;
+    const int row = row_block() * RPB + threadIdx.x / G;
     if (row >= a.rows) return;  // (a whole wave's rows, or the whole workgroup's)
     const size_t at = (size_t)row * d;
     const XT* const x = static_cast<const XT*>(a.x) + at;
@@ -253,7 +260,8 @@ __global__ __launch_bounds__(256) void join_forward_kernel(JoinForward a) {
 template <typename XT>
 __global__ __launch_bounds__(256) void join_forward_any_kernel(JoinForward a) {
     __shared__ float room[2][4];
-    const int d = a.cols, row = blockIdx.x;
+    const int d = a.cols, row = row_block();
+    if (row >= a.rows) return;
     const size_t at = (size_t)row * d;
     const XT* const x = static_cast<const XT*>(a.x) + at;
     const XT* const y = static_cast<const XT*>(a.y) + at;
@@ -616,11 +624,11 @@ hipError_t forward(const JoinForward& a, hipStream_t s) {
         a.cols, on_pieces(a.cols, sizeof(XT), rows, parameters),
         [&](auto whole, auto p, auto g) {
             constexpr int P = decltype(p)::value, G = decltype(g)::value, RPB = 256 / G;
-            hipLaunchKernelGGL((join_forward_kernel<XT, decltype(whole)::value, P, G>), dim3((a.rows + RPB - 1) / RPB), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((join_forward_kernel<XT, decltype(whole)::value, P, G>), row_grid((a.rows + RPB - 1) / RPB), dim3(256), 0, s, a);
             return hipGetLastError();
         },
         [&] {
-            hipLaunchKernelGGL((join_forward_any_kernel<XT>), dim3(a.rows), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((join_forward_any_kernel<XT>), row_grid(a.rows), dim3(256), 0, s, a);
             return hipGetLastError();
         });
 }

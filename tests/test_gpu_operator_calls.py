@@ -77,9 +77,8 @@ def test_on_a_stream_of_the_callers_own(device, hip):  # noqa: F811
     assert same(got, want)
 
 
-def test_offsets_beyond_32_bits(device):
-    """Rows of 4.3 GB each way: the last rows are what a call on them alone gives."""
-    rows, cols, tail = (1 << 25) + 5, 64, 9
+def last_rows_are_those_of_a_call_on_them_alone(device, rows, cols):
+    tail = 9
     j = rb.ResidualJoin(device, cols, dtype="bf16")
     rng = np.random.default_rng(0)
     bits = lambda: (rng.integers(0, 1 << 15, (tail, cols)) % 0x3f80 + 0x3f00).astype(np.uint16)  # noqa: E731
@@ -106,6 +105,17 @@ def test_offsets_beyond_32_bits(device):
     finally:
         for b in big + small:
             b.free()
+
+
+def test_offsets_beyond_32_bits(device):
+    """Rows of 4.3 GB each way."""
+    last_rows_are_those_of_a_call_on_them_alone(device, (1 << 25) + 5, 64)
+
+
+@pytest.mark.parametrize("rows,cols", [((1 << 26) + 5, 8), ((1 << 24) + 5, 3)])
+def test_more_rows_than_a_dimension_of_a_launch_has_threads_for(device, rows, cols):
+    """A row takes a wave, or where it is shorter than 16 bytes a workgroup."""
+    last_rows_are_those_of_a_call_on_them_alone(device, rows, cols)
 
 
 def test_an_operator_outlives_its_device_handle():
