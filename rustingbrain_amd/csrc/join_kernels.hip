@@ -10,10 +10,12 @@
 // The statistics and every sum are f32.  An output is rounded once, from f32.
 //
 // Backward, D = everything that reaches `out`:  with s = 1 / rms(out), t = 1 / rms(y), u = grad_normed * next
-//   D         = grad_out + s u - out s^3 (out . u) / d
+//   D         = grad_out + s (u - h (h . u) / d)     h = s out
 //   grad_x    = D
 //   grad_gate = scale * D * b             db = scale * g * D              v = db * post
-//   grad_y    = t v - y t^3 (y . v) / d
+//   grad_y    = t (v - n (n . v) / d)                n = t y
+// (never by the cube of s or t alone: it leaves f32's range, below for an RMS above 4e12 and above for one below 1e-13, where both h and n are
+// about one)
 //   grad_post = sum_rows db * y * t       grad_next = sum_rows grad_normed * out * s
 // us a call (bytes a second): forward 16384 x 1024 bf16 29.6 (4.5 TB/s; a copy of as much 5.2), 1 x 512 5.1, of which the launch is 2.8;
 // backward 16384 x 1024 bf16 46.3 (4.3 TB/s), 1024 x 512 f32 9.2 (launches of 6 and 3).
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
         }
         row_sums<G>(s, room[0]);
         const float k2 = has_next ? inverse_rms(s[0], d, a.eps) : 0.0f;
-        const float back2 = k2 * k2 * k2 * (s[1] * inv_d);
+        const float dot2 = s[1] * k2 * inv_d;
         const float k1 = has_post ? inverse_rms(s[2], d, a.eps) : 1.0f;
         float D[P][V], yv_dot[1] = {0.0f};
 #pragma unroll
@@ -384,8 +386,9 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
                 nr[p].widen(nv);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    D[p][i] += k2 * (nv[i] * next[p][i]) - rv[i] * back2;
-                    if (live) sums[2][p][i] = fmaf(nv[i], rv[i] * k2, sums[2][p][i]);
+                    const float h = rv[i] * k2;
+                    D[p][i] += k2 * (nv[i] * next[p][i] - h * dot2);
+                    if (live) sums[2][p][i] = fmaf(nv[i], h, sums[2][p][i]);
                 }
             }
             if (a.grad_x) Piece<XT, A>::store(static_cast<XT*>(a.grad_x) + at + c, D[p], d - c);
@@ -413,10 +416,10 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
             }
             if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) Piece<XT, A>::store(static_cast<XT*>(a.grad_gate) + at + c, dg, d - c);
         }
-        float back1 = 0.0f;
+        float dot1 = 0.0f;
         if (has_post) {
             row_sums<G>(yv_dot, room[1]);
-            back1 = k1 * k1 * k1 * (yv_dot[0] * inv_d);
+            dot1 = yv_dot[0] * k1 * inv_d;
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
@@ -425,7 +428,7 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
             float yv[V];
             yr[p].widen(yv);
 #pragma unroll
-            for (int i = 0; i < V; ++i) yv[i] = live ? k1 * D[p][i] - yv[i] * back1 : 0.0f;
+            for (int i = 0; i < V; ++i) yv[i] = live ? k1 * (D[p][i] - yv[i] * k1 * dot1) : 0.0f;
             Piece<XT, A>::store(static_cast<XT*>(a.grad_y) + at + c, yv, d - c);
         }
         if constexpr (G > 64) __syncthreads();  // `room` is written again
@@ -502,11 +505,11 @@ __global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) 
         }
         row_sums<256>(s, room[0]);
         const float k2 = has_next ? inverse_rms(s[0], d, a.eps) : 0.0f;
-        const float back2 = k2 * k2 * k2 * (s[1] * inv_d);
+        const float dot2 = s[1] * k2 * inv_d;
         const float k1 = has_post ? inverse_rms(s[2], d, a.eps) : 1.0f;
         auto total = [&](int c) {  // D
             float v = go ? to_f32(go[c]) : 0.0f;
-            if (has_next) v += k2 * (to_f32(gn[c]) * a.next[c]) - to_f32(r[c]) * back2;
+            if (has_next) v += k2 * (to_f32(gn[c]) * a.next[c] - to_f32(r[c]) * k2 * dot2);
             return v;
         };
         auto gate = [&](int c) {
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) 
                 dot[0] = fmaf(to_f32(y[c]), a.scale * total(c) * gate(c) * a.post[c], dot[0]);
             row_sums<256>(dot, room[1]);
         }
-        const float back1 = has_post ? k1 * k1 * k1 * (dot[0] * inv_d) : 0.0f;
+        const float dot1 = has_post ? dot[0] * k1 * inv_d : 0.0f;
         for (int c = threadIdx.x; c < d; c += 256) {
             const float D = total(c);
             float dy = 0.0f, dg = 0.0f;
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) 
                 dg = e * (n * w);
                 mine[c] += db * n;
                 mine[d + c] += dg;
-                dy = k1 * (has_post ? db * w : db) - yv * back1;
+                dy = k1 * ((has_post ? db * w : db) - n * dot1);
                 if (has_next) mine[2 * (size_t)d + c] = fmaf(to_f32(gn[c]), to_f32(r[c]) * k2, mine[2 * (size_t)d + c]);
             }
             if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) static_cast<XT*>(a.grad_gate)[at + c] = from_f32<XT>(dg);
