@@ -428,7 +428,8 @@ __global__ __launch_bounds__(256) void join_backward_kernel(JoinBackward a) {
             float yv[V];
             yr[p].widen(yv);
 #pragma unroll
-            for (int i = 0; i < V; ++i) yv[i] = live ? k1 * (D[p][i] - yv[i] * k1 * dot1) : 0.0f;
+            for (int i = 0; i < V; ++i)  // (without a norm it does not depend on y, which may be infinite)
+                yv[i] = !live ? 0.0f : has_post ? k1 * (D[p][i] - yv[i] * k1 * dot1) : D[p][i];
             Piece<XT, A>::store(static_cast<XT*>(a.grad_y) + at + c, yv, d - c);
         }
         if constexpr (G > 64) __syncthreads();  // `room` is written again
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(256) void join_backward_any_kernel(JoinBackward a) 
                 dg = e * (n * w);
                 mine[c] += db * n;
                 mine[d + c] += dg;
-                dy = k1 * ((has_post ? db * w : db) - n * dot1);
+                dy = has_post ? k1 * (db * w - n * dot1) : db;
                 if (has_next) mine[2 * (size_t)d + c] = fmaf(to_f32(gn[c]), to_f32(r[c]) * k2, mine[2 * (size_t)d + c]);
             }
             if (a.gate_mode == RBMOE_GATE_ROW && a.grad_gate) static_cast<XT*>(a.grad_gate)[at + c] = from_f32<XT>(dg);
