@@ -366,7 +366,8 @@ int rbmoe_join_backward(rbmoe_join* join, int32_t rows, const void* y, const voi
  * rbmoe_orthogonalize brings the singular values of every matrix near one: X = U / (|U|_F + 1e-7), then `steps` times
  *   A = X X^T, B = b A + c A A, X = a X + B X,  (a, b, c) = (3.4445, -4.7750, 2.0315)
  * (five steps: values from 0.003 |U|_F up end in [0.68, 1.21]; elements below 2^-38 |U|_F count as zero).  Accuracy is f32's whatever the types of `in` and `out`, each RBMOE_F32 or
- * RBMOE_BF16; `out` may be `in`.  A matrix of zeros stays one.
+ * RBMOE_BF16, and whatever |U|_F is, from 1e-35 up: one far below 1e-7 gives a small result, exact relative to itself.  `out` may be `in`.  A
+ * matrix of zeros stays one.
  * rbmoe_muon_step is an optimiser step with it (decoupled weight decay):
  *   M = momentum_factor M + G,  U = G + momentum_factor M (nesterov != 0) or M,
  *   W = (1 - lr weight_decay) W - lr update_scale O,  O the orthogonalised U;  update_scale 0 stands for sqrt(max(1, rows / cols)).

@@ -20,6 +20,7 @@ struct MuonStack {
 };
 
 constexpr int kMostMuonSide = 1 << 14;  // rows or columns: an operand's offsets are 32-bit
+constexpr int kMostMuonSteps = 64;
 
 struct MuonCall {
     int count = 0, rows = 0, cols = 0;
@@ -41,7 +42,7 @@ inline const char* muon_settings_problem(float lr, float momentum, float decay, 
     if (!(momentum >= 0.0f && momentum < 1.0f)) return "the momentum must be in [0, 1)";
     if (!std::isfinite(decay) || decay < 0.0f) return "the weight decay must be finite and not negative";
     if (!std::isfinite(scale) || scale < 0.0f) return "the update's scale must be finite and not negative";
-    if (steps < 1 || steps > 64) return "the number of steps must be between 1 and 64";
+    if (steps < 1 || steps > kMostMuonSteps) return "the number of steps must be between 1 and 64";
     return nullptr;
 }
 // 0 stands for sqrt(max(1, rows / cols)): an update moves every output of a layer by about the same, whatever its width.

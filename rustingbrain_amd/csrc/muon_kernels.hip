@@ -7,7 +7,10 @@
 // 0.003 up into [0.68, 1.21].  So throughout |X| <= 1.21, |A| <= 1.47 and |B| <= a (spectral norms, which bound the elements).
 //
 // Precision.  The result is f32-grade: every operand is kept as two fp16 numbers, hi = fp16(2^14 v) and lo = fp16(2^14 v - hi), together 22
-// bits; the bounds above keep 2^14 v below 65504, and an element as small as 2^-26 still has its bits.  A product is three on the matrix
+// bits.  The bounds above keep 2^14 v below 65504.  lo ends at fp16's 2^-24, so the 22 bits are whole from |v| = 2^-16 up and the error is 2^-39
+// below: next to an |X|_F of about one that is 2^-39 sqrt(m n) at most, 2^-28 for 1408 x 1408.  A matrix whose |U|_F is not far above
+// 1e-7 begins with a smaller |X|_F, |U|_F / (|U|_F + 1e-7), and grows by 3.4 a step at most: such an X is kept times a power of two (Lift) that
+// brings it near one at every step.  A and B need none: their errors count beside a.  A product is three on the matrix
 // cores, hi hi + hi lo + lo hi, with f32 sums; what is left out is 2^-22 of a term.  That is three fp16 products at 16 times the rate of
 // the f32 ones.  (Two bf16 parts hold 16 bits, and five steps of them end 1e-5 from the exact result where f32 ends 2e-6.)
 //
@@ -142,9 +145,23 @@ __global__ __launch_bounds__(256) void muon_front_kernel(Front f) {
 }
 
 // ---- U into operand order, both ways -------------------------------------------------------------------
+// X_k is stored times 2^14 / down, down = 2^-e: e is the largest whole number, 0 at least, for which 1.25 times 2^-e bounds the singular
+// values of X_k.  (For an |U|_F of 1.7e-7 and more that is 0 throughout.  At most 98, so that 2^-28 down is a normal number.)
+struct Lift {
+    float down, up;
+};
+__device__ __forceinline__ Lift lift_of(double norm, int k) {
+    float bound = fminf((float)(norm / (norm + 1e-7)), 1.0f);  // (of a norm that is not a number, too)
+    for (int i = 0; i < k; ++i) bound = fminf(bound * 3.4446f, 1.2025f);
+    const int e = min(max(ilogbf(1.25f / bound), 0), 98);
+    return {ldexpf(1.0f, -e), ldexpf(1.0f, e)};
+}
+
 struct Pack {
     Front f;
     Shape s;
+    Lift* lift;  // [count][steps]
+    int steps;
     bool tall;  // rows > cols: the matrix is taken transposed
     char* x;    // X, X^T of matrix i at i * x_bytes()
     char* xt;
@@ -183,7 +200,8 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(Pack a) {
         if (lane == 0) norm2 = sum;
     }
     __syncthreads();
-    const double factor = (double)kUp / (sqrt(norm2) + 1e-7);
+    const double norm = sqrt(norm2), factor = (double)kUp * lift_of(norm, 0).up / (norm + 1e-7);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid < a.steps) a.lift[(size_t)i * a.steps + tid] = lift_of(norm, tid);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         int p, q;
@@ -230,12 +248,24 @@ struct ProductArgs {
     char* direct;            // C^T in operand order: rows q, reduction p
     char* mirrored;          // C in operand order:   rows p, reduction q
     size_t out_bytes;
+    const Lift* lift;        // of this step, matrix 0
+    int lift_stride;
     // kLast
     MuonStack weight, out;
     bool update, out_bf16, tall;
     bool whole;              // tall, and four neighbouring elements of a row may be accessed at once
     float keep, rate;
 };
+
+// What a sum of products is multiplied by.
+template <Product kind>
+__device__ __forceinline__ float sum_factor(const ProductArgs& a, int matrix) {
+    if constexpr (kind == kPoly) return kDown;  // 2^28 C -> 2^14 C
+    const Lift* const l = a.lift + (size_t)matrix * a.lift_stride;
+    if constexpr (kind == kGram) return kDown * l->down * l->down;
+    else if constexpr (kind == kApply) return kDown * l->down * l[1].up;
+    else return kDown * kDown * l->down;
+}
 
 // byte offset of element (row, column) of an operand with `steps` fragments a group of rows
 __device__ __forceinline__ size_t operand_at(int row, int col, int steps) {
@@ -285,13 +315,13 @@ __device__ __forceinline__ void read_before(const ProductArgs& a, int matrix, in
 // Four elements of C, rows p0 .. p0 + 3 (p0 a multiple of 4) of column q, in f32.  `parts`: what was stored of them, hi | lo << 16.
 template <Product kind>
 __device__ __forceinline__ void write4(const ProductArgs& a, int matrix, int gp, int gq, int j, int at, int lane, const float (&sum)[4],
-                                       const Before<kind>& b, uint32_t (&parts)[4]) {
+                                       float factor, const Before<kind>& b, uint32_t (&parts)[4]) {
     const int p0 = gp * 32 + 8 * j + 4 * (lane >> 5), q = gq * 32 + (lane & 31);
     if constexpr (kind == kLast) {
         if (q >= a.s.n) return;
         float o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = sum[i] * (kDown * kDown);
+        for (int i = 0; i < 4; ++i) o[i] = sum[i] * factor;
         const bool four = a.whole && p0 + 3 < a.s.m;
         if (a.update) {
             float* const w = weight_at(a, matrix, p0, q);
@@ -332,7 +362,7 @@ __device__ __forceinline__ void write4(const ProductArgs& a, int matrix, int gp,
         halfx4 hi, lo;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float v = sum[i] * kDown;  // 2^28 C -> 2^14 C
+            float v = sum[i] * factor;
             if constexpr (kind == kPoly) {
                 v = fmaf(kB, (float)b.hi[at][i] + (float)b.lo[at][i], kC * v);
                 // (the padding's diagonal stays zero)
@@ -400,6 +430,7 @@ __global__ __launch_bounds__(64 * W) void muon_product_split_kernel(ProductArgs 
     }
     const char* const pm = a.p + (size_t)matrix * a.p_bytes;
     const char* const qm = a.q + (size_t)matrix * a.q_bytes;
+    const float factor = sum_factor<kind>(a, matrix);
     const __amdgpu_buffer_rsrc_t p_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pm), 0, (int)a.p_bytes, kRawBuffer);
     const __amdgpu_buffer_rsrc_t q_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qm), 0, (int)a.q_bytes, kRawBuffer);
     int ps[B], qs[B];
@@ -499,7 +530,7 @@ __global__ __launch_bounds__(64 * W) void muon_product_split_kernel(ProductArgs 
         int gp, gq, j;
         if (!block_of(t, gp, gq, j)) continue;
         uint32_t parts[4];
-        write4<kind>(a, matrix, gp, gq, j, 0, lane, sum[t], before[t], parts);
+        write4<kind>(a, matrix, gp, gq, j, 0, lane, sum[t], factor, before[t], parts);
         if constexpr (kind != kLast)
             *reinterpret_cast<uint4*>(turned + (((wave + t * W) / 4) * 32 + (lane & 31)) * kTurnedPitch + 8 * j + 4 * (lane >> 5)) =
                 make_uint4(parts[0], parts[1], parts[2], parts[3]);
@@ -570,6 +601,7 @@ __global__ __launch_bounds__(256, 2) void muon_product_kernel(ProductArgs a, int
     // Loads through a buffer descriptor: its base and the part of the offset that goes up with the reduction are scalars, so the loop
     // holds one vector register of addresses.  (An operand of one matrix has at most 2^30 bytes.)  A thread's pieces of a stage: piece i
     // of group i, whose two steps of 16 lie side by side.
+    const float factor = sum_factor<kind>(a, matrix);
     const __amdgpu_buffer_rsrc_t p_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pm), 0, (int)a.p_bytes, kRawBuffer);
     const __amdgpu_buffer_rsrc_t q_buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(qm), 0, (int)a.q_bytes, kRawBuffer);
     const int p_at = tid * 16, q_at = lane * 16;
@@ -700,7 +732,7 @@ __global__ __launch_bounds__(256, 2) void muon_product_kernel(ProductArgs a, int
         for (int j = 0; j < 4; ++j) {
             const float sum[4] = {acc[r][c][4 * j], acc[r][c][4 * j + 1], acc[r][c][4 * j + 2], acc[r][c][4 * j + 3]};
             uint32_t parts[4];
-            write4<kind>(a, matrix, gp, gq, j, j, lane, sum, before[b % 2], parts);
+            write4<kind>(a, matrix, gp, gq, j, j, lane, sum, factor, before[b % 2], parts);
             if (mirror)
                 *reinterpret_cast<uint4*>(turned + (lane & 31) * kTurnedPitch + 8 * j + 4 * (lane >> 5)) =
                     make_uint4(parts[0], parts[1], parts[2], parts[3]);
@@ -788,7 +820,8 @@ MuonTile muon_tile(int count, int rows, int cols, int product) {
 
 size_t muon_workspace_bytes(int count, int rows, int cols) {
     const Shape s = shape_of(rows, cols);
-    return rounded((size_t)count * norm_parts(rows, cols) * 8) + count * (3 * s.x_bytes() + 2 * s.a_bytes());
+    return rounded((size_t)count * norm_parts(rows, cols) * 8) + rounded((size_t)count * kMostMuonSteps * sizeof(Lift)) +
+           count * (3 * s.x_bytes() + 2 * s.a_bytes());
 }
 
 hipError_t launch_muon(const MuonCall& c, hipStream_t s) {
@@ -797,6 +830,8 @@ hipError_t launch_muon(const MuonCall& c, hipStream_t s) {
     Front f{c.grad, c.momentum, update, c.nesterov, c.mu, c.rows, c.cols, norm_parts(c.rows, c.cols),
             static_cast<double*>(c.workspace)};
     char* at = static_cast<char*>(c.workspace) + rounded((size_t)c.count * f.parts * 8);
+    Lift* const lift = reinterpret_cast<Lift*>(at);
+    at += rounded((size_t)c.count * kMostMuonSteps * sizeof(Lift));
     char *x, *xt[2], *am, *bm;
     x = at;  // (a step that writes X reads X^T alone, which lies in two places in turn)
     at += c.count * sh.x_bytes();
@@ -807,7 +842,7 @@ hipError_t launch_muon(const MuonCall& c, hipStream_t s) {
     am = at;
     bm = at + c.count * sh.a_bytes();
     const dim3 fg(f.parts, c.count), pgrid(sh.mg, (sh.ng + 1) / 2, c.count);
-    const Pack pk{f, sh, tall, x, xt[0]};
+    const Pack pk{f, sh, lift, c.steps, tall, x, xt[0]};
     const size_t elements = (size_t)c.rows * c.cols;
     auto fours = [&](const MuonStack& st, int size) {  // four neighbouring elements at once, wherever they stand
         return st.pitch == c.cols && elements % 4 == 0 && (c.count == 1 || st.stride % 4 == 0) && reinterpret_cast<uintptr_t>(st.p) % (4 * size) == 0;
@@ -831,6 +866,8 @@ hipError_t launch_muon(const MuonCall& c, hipStream_t s) {
         g.p_bytes = g.q_bytes = sh.x_bytes();
         g.pg = g.qg = sh.mg;
         g.steps = 2 * sh.ng;
+        g.lift = lift + k;
+        g.lift_stride = c.steps;
         g.direct = g.mirrored = am;
         g.out_bytes = sh.a_bytes();
         e = launch_product<kGram>(g, c.count, s);

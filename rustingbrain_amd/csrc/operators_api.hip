@@ -186,7 +186,7 @@ int rbmoe_orthogonalize(rbmoe_muon* m, const void* in, int32_t in_dtype, int32_t
     if (!in || !out) return fail(ctx, RBMOE_NULL_POINTER, "in or out is NULL");
     for (const int dt : {in_dtype, out_dtype})
         if (dt != RBMOE_F32 && dt != RBMOE_BF16) return fail(ctx, RBMOE_INVALID_CONFIG, "matrices must be f32 or bf16");
-    if (steps < 1 || steps > 64) return fail(ctx, RBMOE_INVALID_CONFIG, "the number of steps must be between 1 and 64");
+    if (steps < 1 || steps > kMostMuonSteps) return fail(ctx, RBMOE_INVALID_CONFIG, "the number of steps must be between 1 and 64");
     if (off_element(in, in_dtype) || off_element(out, out_dtype)) return fail(ctx, RBMOE_INVALID_INPUT, "matrices must start at an element");
     HIP_TRY(ctx, hipSetDevice(ctx->device));
     MuonCall c;
