@@ -295,7 +295,7 @@ struct rbmoe_layer {
     bool norm_set = false;
     // training through the block step (allocated once both the norm and training mode are there)
     Buf xraw, dxn, inv_rms, norm_partial, g_norm;  // [T, d] x2 activation dtype, [T], [T/32][d], [d] f32
-    bool last_was_block = false, last_kept_block = false;  // the last forward: the block step; in training mode, with its rows kept
+    bool last_was_block = false;
     // the block step's join where it is more than the residual add (rbmoe_set_block_join)
     Buf yj, join_post, join_gate;         // [max_T, d] the layer's rows, [d] f32 x2
     bool join_set = false, join_has_post = false, join_has_gate = false;
@@ -2339,7 +2339,6 @@ int rbmoe_forward_block(rbmoe_layer* L, const void* x, int32_t T, int32_t cols, 
         if (L->training && valid)  // the backward pass leaves padding rows out as well, and the caller's bytes may be gone by then
             HIP_TRY(ctx, hipMemcpyAsync(L->join_valid.p, valid, (size_t)T, hipMemcpyDeviceToDevice, ctx->stream));
     }
-    L->last_kept_block = L->training;
     L->last_joined = joined;
     L->last_join_valid = valid != nullptr;
     L->last_was_block = true;
@@ -2639,10 +2638,9 @@ int rbmoe_backward_block(rbmoe_layer* L, const void* grad_output, int32_t tokens
     const int T = L->last_T, d = L->cfg.d_model;
     if (T == 0) return RBMOE_OK;
     if (!grad_output || !grad_input) return fail(ctx, RBMOE_NULL_POINTER, "grad_output or grad_input is NULL");
-    // (a block step from before training mode has kept neither the rows in front of the norm nor the join's padding)
-    if (!L->last_kept_block) return fail(ctx, RBMOE_INVALID_INPUT, "no forward pass has run in training mode yet");
     const void* upstream = grad_output;
     if (L->last_joined) {  // ... through the join first (a training layer that has one holds its buffers)
+        if (!L->dyj.p) return fail(ctx, RBMOE_INVALID_INPUT, "no forward pass has run in training mode yet");
         HIP_TRY(ctx, hipSetDevice(ctx->device));
         JoinBackward j{};
         j.y = L->yj.p;
