@@ -271,8 +271,8 @@ int rbmoe_forward_block_host(rbmoe_layer* layer, const void* x, int32_t tokens, 
                              const uint8_t* valid, const float* router_bias, void* out);
 
 /* The block step's join, where it is more than the residual add: out = x + scale * gate * RmsNorm(layer(rmsnorm(x))) * post_weight, as
- * rbmoe_join_forward has it (below).  post_weight and gate are HOST [d_model] f32 or NULL; both NULL with scale 1 is the residual add
- * again.  From then on rbmoe_forward_block and rbmoe_backward_block (and their host forms) include it; padding rows pass x through, the
+ * rbmoe_join_forward has it (below), of the layer's rows rounded to its dtype.  post_weight and gate are HOST [d_model] f32 or NULL; both
+ * NULL with scale 1 is the residual add again.  From then on rbmoe_forward_block and rbmoe_backward_block (and their host forms) include it; padding rows pass x through, the
  * shared expert's rows included.  In training mode the gradients of post_weight and gate accumulate like the norm's
  * (RBMOE_W_POST_NORM, RBMOE_W_BLOCK_GATE).  Needs the feed-forward norm; a backward pass for a forward from before this call is refused.
  * (rbmoe_backward behind a joined block step is the layer's alone: its grad_output is that of the layer's rows.) */
@@ -334,15 +334,19 @@ int rbmoe_backward_block_host(rbmoe_layer* layer, const void* grad_output, int32
  *   normed = RmsNorm(out) * next_weight    (of the rows as they are stored; only with next_weight)
  * Rows [rows, cols] are of the join's dtype, weights [cols] f32; a gate by channel is [cols] f32, one by row [rows, cols] of the join's
  * dtype.  All of them DEVICE pointers.  `valid` [rows] bytes or NULL: a padding row (0) takes y as zero, so its `out` is its x; what
- * lies in its y and gate is not used, and it adds nothing to the gradients of weights and gate.  Statistics and sums are f32, each
- * output is rounded once.  `out` may be x, `normed` may be y; apart from that outputs must not overlap inputs or one another. */
+ * lies in its y and gate is not used, and it adds nothing to the gradients of weights and gate (its `normed` is that of its x, and
+ * grad_normed reaches its grad_x).  Statistics and sums are f32, each output is rounded once; a row's sum of squares is taken in f32, so
+ * a row whose squares pass its range has a norm of zeros, and with eps 0 one whose squares are below it none.  `out` may be x, `normed` may
+ * be y; apart from that outputs must not overlap inputs or one another. */
 typedef enum rbmoe_gate {
     RBMOE_GATE_NONE = 0,
     RBMOE_GATE_CHANNEL = 1, /* [cols] f32, a parameter */
     RBMOE_GATE_ROW = 2      /* [rows, cols] of the rows' dtype */
 } rbmoe_gate;
 typedef struct rbmoe_join rbmoe_join;
-/* Holds the workspace of the backward pass (counted against the context's budget).  1 to 65536 columns; calls take up to 2^30 rows. */
+/* Holds the workspace of the backward pass (counted against the context's budget), up to 12 bytes a column for each of 512 workgroups; weights
+ * come with a call, so one join serves every sub-layer of its width, dtype and gate, one call after the other.  1 to 65536 columns; calls take up
+ * to 2^30 rows. */
 int rbmoe_join_create(rbmoe_ctx* ctx, int32_t cols, int32_t dtype, int32_t gate, rbmoe_join** out);
 void rbmoe_join_destroy(rbmoe_join* join);
 /* Enqueued on the context's stream; allocates nothing. */

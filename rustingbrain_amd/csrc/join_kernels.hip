@@ -17,7 +17,7 @@
 // (never by the cube of s or t alone: it leaves f32's range, below for an RMS above 4e12 and above for one below 1e-13, where both h and n are
 // about one)
 //   grad_post = sum_rows db * y * t       grad_next = sum_rows grad_normed * out * s
-// us a call (bytes a second): forward 16384 x 1024 bf16 29.6 (4.5 TB/s; a copy of as much 5.2), 1 x 512 5.1, of which the launch is 2.8;
+// us a call (bytes a second): forward 16384 x 1024 bf16 29.6 (4.5 TB/s; a copy of as much 5.2), 1 x 512 5.2, of which the launch is 2.8;
 // backward 16384 x 1024 bf16 46.3 (4.3 TB/s), 1024 x 512 f32 9.2 (launches of 6 and 3).
 // Each of the three parameter gradients is a sum over rows: a wave (or workgroup) takes every n-th row and keeps the sums of
 // its columns in registers; workgroups then leave them in memory and a second, small launch adds them in a fixed order, so
@@ -578,7 +578,8 @@ bool on_pieces(int cols, int size, uintptr_t rows_at, uintptr_t parameters_at) {
 // f(A, P, G) as integral constants for rows of `cols` elements, or `any()` where registers do not hold them.  Rows off 16 bytes by whole
 // vectors too, against two (bf16) or one element an access, us forward / backward: 1533 x 1365 f32 8.7 / 25.3 -> 7.6 / 24.3, 2000 x 1365
 // bf16 10.2 / 41.6 -> 7.8 / 23.1, 2000 x 2047 bf16 13.5 / 48.7 -> 9.6 / 25.2; 1000 x 766 bf16 6.3 / 14.7 -> 6.0 / 15.6,
-// 4000 x 766 8.7 / 20.6 -> 8.7 / 22.9 (even widths gain in the forward pass only).  A wave takes a
+// 4000 x 766 8.7 / 20.6 -> 8.7 / 22.9.  (Even bf16 widths off 16 bytes lose 6 to 11 % in the backward pass where odd ones gain 1.8 times; there is no
+// third form of the kernels for those alone.)  A wave takes a
 // row of up to 16 elements a lane, a workgroup one of up to 32 a thread.  us a call, rows of 2048 bf16 by a wave / by a
 // workgroup: 200 rows 6.4 / 4.9, 2000 rows 9.2 / 8.0; rows of 768: 203 rows 4.9 / 4.9, 2000 rows 5.4 / 5.6, of 1024, 4096 rows 7.8 / 8.8.
 // Backward, 32 elements a thread (up to 423 registers, one wave a SIMD, nothing in memory) against rows read again: 1 x 5000 bf16

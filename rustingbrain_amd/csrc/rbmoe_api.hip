@@ -2328,6 +2328,7 @@ int rbmoe_forward_block(rbmoe_layer* L, const void* x, int32_t T, int32_t cols, 
     if (L->training && T > 0)  // TransformerBlockCache keeps the residual (src/transformer_block.rs:224-232)
         HIP_TRY(ctx, hipMemcpyAsync(L->xraw.p, x, (size_t)T * cols * dtype_size(L->cfg.act_dtype),
                                     hipMemcpyDeviceToDevice, ctx->stream));
+    // (behind a join the layer's rows are kept, in the layer's dtype: the backward pass reads them, and the operator on its own gives the same bits)
     const bool joined = L->join_set;
     const int rc = forward_impl(L, L->xn.p, T, cols, valid, router_bias, joined ? nullptr : x, joined ? L->yj.p : out, 0, x);
     if (rc != RBMOE_OK) return rc;
