@@ -214,7 +214,7 @@ def prepare(case, seed):
             else:
                 torch.cuda.synchronize()
                 s.cache.write_device(s.rows, s.k.data_ptr(), s.v.data_ptr(), s.slots.data_ptr())
-                s.handle = rb.DecodeAttention(s.cache, c["heads"], len(s.counts))
+                s.handle = rb.DecodeAttention(device, c["heads"], c["kv_heads"], c["head_dim"], len(s.counts), dtype=c["dtype"])
                 s.out = torch.empty_like(s.q)
                 device.synchronize()
     elif not c["kind"].startswith("prompt"):
@@ -375,8 +375,8 @@ def run(state):
             s.cache.read_device(s.rows, s.got_k.data_ptr(), s.got_v.data_ptr(), s.slots.data_ptr())
             return {"k": s.got_k, "v": s.got_v}
         s.cache.write_device(len(s.counts), s.new_k.data_ptr(), s.new_v.data_ptr(), s.new_slots.data_ptr())
-        s.handle.forward_device(len(s.counts), s.q.data_ptr(), s.out.data_ptr(), s.tables.data_ptr(), s.table_pages, s.lengths.data_ptr(),
-                                longest=max(s.counts), scale=s.scale)
+        s.handle.forward_device(s.cache, len(s.counts), s.q.data_ptr(), s.out.data_ptr(), s.tables.data_ptr(), s.table_pages,
+                                s.lengths.data_ptr(), longest=max(s.counts), scale=s.scale)
         return s.out
     if kind == "prompt":
         out, lse = _prompt_plain(s)
