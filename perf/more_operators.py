@@ -157,10 +157,8 @@ def _inputs(case, seed):
         else:
             s.q, s.k, s.v = q.to(t), k.to(t), v.to(t)
         if c["kind"] == "prompt_backward":
-            wide, s.lse = _prompt_plain(s)
-            # the forward's rows, and what their rounding took away
-            s.out = wide.to(t)
-            s.rest = (wide - s.out.float()).to(t) if c["dtype"] == "bf16" else None
+            s.out, s.lse = _prompt_plain(s)
+            s.out = s.out.to(t)
             s.grad_out = _normal(g, (s.rows, h, d), 1e-2).to(t)
         return s
     order.shuffle(counts)
@@ -367,8 +365,7 @@ def run(state):
                                         lse_ptr=s.lse.data_ptr(), **where)
                 return {"out": s.out, "lse": s.lse}
             s.handle.backward_device(len(s.counts), s.q.data_ptr(), s.k.data_ptr(), s.v.data_ptr(), s.out.data_ptr(), s.lse.data_ptr(),
-                                     s.grad_out.data_ptr(), s.grad_q.data_ptr(), s.grad_k.data_ptr(), s.grad_v.data_ptr(),
-                                     rest_ptr=0 if s.rest is None else s.rest.data_ptr(), **where)
+                                     s.grad_out.data_ptr(), s.grad_q.data_ptr(), s.grad_k.data_ptr(), s.grad_v.data_ptr(), **where)
             return {"grad_q": s.grad_q, "grad_k": s.grad_k, "grad_v": s.grad_v}
         if kind == "cache":
             s.cache.write_device(s.rows, s.k.data_ptr(), s.v.data_ptr(), s.slots.data_ptr())
@@ -461,7 +458,7 @@ def work(case):
         pairs = float(sum(n * e + (n * (n + 1) // 2 if c["causal"] else n * n) for n, e in zip(counts, earlier)))
         if c["kind"] == "prompt":
             return {"bytes": (2.0 * h * rows + 2.0 * kv * key_rows) * d * size + 4.0 * h * rows, "flops": 4.0 * d * h * pairs}
-        return {"bytes": ((4.0 + (c["dtype"] == "bf16")) * h * rows + 4.0 * kv * key_rows) * d * size + 4.0 * h * rows, "flops": 10.0 * d * h * pairs}
+        return {"bytes": (4.0 * h * rows + 4.0 * kv * key_rows) * d * size + 4.0 * h * rows, "flops": 10.0 * d * h * pairs}
     row = 2.0 * kv * d * _SIZE[c["cache"]] + (8.0 * kv if c["cache"] == "int8" else 0.0)  # of the cache
     if c["kind"] == "cache":
         return {"bytes": 2.0 * rows * (2.0 * kv * d * size + row + 8.0), "flops": 8.0 * rows * kv * d}
