@@ -398,6 +398,71 @@ int rbmoe_layer_muon_step(rbmoe_layer* layer, float lr, float momentum_factor, f
  * a checkpoint holds.  Synchronises. */
 int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* host, int32_t rows, int32_t cols);
 
+/* ---- attention ------------------------------------------------------------------------------------
+ * The attention half of a block, between its projections: whole sequences both ways (the reference's src/attention.rs, and
+ * src/cuda_flash.rs on its device), a paged cache of keys and values, and one new row a sequence over it.  Rows are [rows, heads, head_dim] of
+ * RBMOE_F32 or RBMOE_BF16 with consecutive elements; a stride says how many elements lie between two rows (0: no gap), so that
+ * q, k and v may lie side by side as one projection leaves them.  kv_heads divides heads: head h reads kv head
+ * h / (heads / kv_heads).  head_dim is a multiple of 8 up to 128, heads at most 1024.  Everything below are DEVICE pointers but the handles; every call is
+ * enqueued on the context's stream and allocates nothing, and the same call gives the same bits.  Outputs must not overlap inputs or one another.  Rows of 16-byte
+ * pieces (addresses and strides) are staged the fast way; any other element is as good a start. */
+
+/* Attention of whole sequences.  Sequence i has the queries query_begin[i] .. + query_count[i] and the keys key_begin[i] .. +
+ * key_count[i] (key arrays NULL: the queries'), of arrays of query_rows and key_rows rows: packed one behind the other, or padded,
+ * with rows between them that are left as they are.  Counts go up to longest_queries and longest_keys, which a launch is
+ * sized by (a longer sequence counts as that long, and what lies outside the arrays is cut off).  With causal != 0 query r of a sequence sees its keys up to
+ * r + key_count - query_count: the queries are the last of the keys, whose first may come from a cache.
+ *   s_ij = scale q_i . k_j,   lse_i = log sum_j exp s_ij,   out_i = sum_j exp(s_ij - lse_i) v_j    over the keys that row i sees
+ * A row that sees no key is zeros, its lse -inf.  What is not seen has no effect, whatever it holds.  scale is positive.  Two sequences may share keys
+ * (forward only), not queries.
+ *   out  [query_rows, heads, head_dim] without gaps      lse [heads, query_rows] f32 or NULL
+ * Sums and statistics are f32 (f32 rows: their products too); bf16 rows round exp(s_ij - m) to bf16 for the product with v. */
+typedef struct rbmoe_attention rbmoe_attention;
+/* backward_rows: the most query rows of a backward pass (0: forward only), 4 bytes a row and head, counted against the budget. */
+int rbmoe_attention_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t backward_rows,
+                           rbmoe_attention** out);
+void rbmoe_attention_destroy(rbmoe_attention* attention);
+int rbmoe_attention_forward(rbmoe_attention* attention, int32_t sequences, int32_t longest_queries, int32_t longest_keys,
+                            const int32_t* query_begin, const int32_t* query_count, const int32_t* key_begin, const int32_t* key_count,
+                            int32_t query_rows, int32_t key_rows, const void* q, int32_t q_stride, const void* k, int32_t k_stride,
+                            const void* v, int32_t v_stride, int32_t causal, float scale, void* out, float* lse);
+/* Gradients of q, k and v, each with its input's stride and of its type; the arguments up to scale are the forward's, out and lse
+ * what it wrote, grad_out is without gaps like out.  A kv head's gradients are the sums over its group;
+ * keys that no row sees get zeros.  Every sequence has keys of its own.  Calls on one attention must not overlap in time (the forward may be called
+ * any way). */
+int rbmoe_attention_backward(rbmoe_attention* attention, int32_t sequences, int32_t longest_queries, int32_t longest_keys,
+                             const int32_t* query_begin, const int32_t* query_count, const int32_t* key_begin, const int32_t* key_count,
+                             int32_t query_rows, int32_t key_rows, const void* q, int32_t q_stride, const void* k, int32_t k_stride,
+                             const void* v, int32_t v_stride, int32_t causal, float scale, const void* out, const float* lse,
+                             const void* grad_out, void* grad_q, void* grad_k, void* grad_v);
+
+/* A cache of keys and values in pages.  Slot page * page_rows + r is row r of a page; which pages belong to which sequence is the
+ * caller's affair.  Rows are of `dtype`, the cache holds them as they are (cache_dtype = dtype) or in 8 bits (RBMOE_I8): a scale max |x| / 127 a
+ * row and head, round(127 x / max |x|) with ties to even; a row with an infinity or NaN reads back as NaN.  page_rows is a power of two from 16 to
+ * 4096.  The pages (zeros at first, head_dim rounded up to 64 or 128, 8 bytes more a row and head in 8 bits) count against the budget. */
+typedef struct rbmoe_kv_cache rbmoe_kv_cache;
+int rbmoe_kv_cache_create(rbmoe_ctx* ctx, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t cache_dtype, int32_t page_rows,
+                          int32_t pages, rbmoe_kv_cache** out);
+void rbmoe_kv_cache_destroy(rbmoe_kv_cache* cache);
+/* Rows k and v [rows, kv_heads, head_dim] to their slots.  A row whose slot is negative or behind the last page is left out (padding).  The
+ * rows of one call go to different slots: two rows for one slot leave a mixture of both there. */
+int rbmoe_kv_cache_write(rbmoe_kv_cache* cache, int32_t rows, const void* k, int32_t k_stride, const void* v, int32_t v_stride,
+                         const int64_t* slots);
+/* And back, to any rows; those without a slot are zeros. */
+int rbmoe_kv_cache_read(rbmoe_kv_cache* cache, int32_t rows, void* k, int32_t k_stride, void* v, int32_t v_stride, const int64_t* slots);
+
+/* One query row a sequence over the cache: out[i] = attention of q[i] over the first lengths[i] rows of sequence i, whose pages are
+ * tables[i][0 .. table_pages).  The new row's own key is written before, and counts.  Lengths go up to `longest` (longer ones are cut), by which a
+ * launch is sized: a captured graph takes the longest that its replays will see.  A table entry that is no page of the cache has no rows; a
+ * sequence without any gives zeros.  The handle holds the workspace for up to max_sequences sequences, joins parts of long sequences in
+ * it, and serves any number of caches, one call after the other. */
+typedef struct rbmoe_decode rbmoe_decode;
+int rbmoe_decode_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t max_sequences,
+                        rbmoe_decode** out);
+void rbmoe_decode_destroy(rbmoe_decode* decode);
+int rbmoe_decode_attention(rbmoe_decode* decode, rbmoe_kv_cache* cache, int32_t sequences, const void* q, int32_t q_stride,
+                           const int32_t* tables, int32_t table_pages, const int32_t* lengths, int32_t longest, float scale, void* out);
+
 /* Per-stage timing of one forward with HIP events on the context's stream.
  * `ms` receives RBMOE_NUM_STAGES durations in milliseconds.  Synchronises.
  * Every stage has launches of its own here, one behind the other: a call that is not timed may have the dispatch inside the

@@ -92,6 +92,20 @@ pub struct rbmoe_join {
 pub struct rbmoe_muon {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct rbmoe_attention {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct rbmoe_kv_cache {
+    _private: [u8; 0],
+}
+
+#[repr(C)]
+pub struct rbmoe_decode {
+    _private: [u8; 0],
+}
 
 extern "C" {
     pub fn rbmoe_config_init(cfg: *mut rbmoe_config, d_model: i32, num_experts: i32, experts_per_token: i32,
@@ -138,6 +152,33 @@ extern "C" {
     pub fn rbmoe_muon_step(muon: *mut rbmoe_muon, grad: *const c_void, grad_dtype: i32, momentum: *mut f32, weight: *mut f32,
                            lr: f32, momentum_factor: f32, weight_decay: f32, update_scale: f32, nesterov: i32,
                            steps: i32) -> c_int;
+    pub fn rbmoe_attention_create(ctx: *mut rbmoe_ctx, heads: i32, kv_heads: i32, head_dim: i32, dtype: i32, backward_rows:
+                                  i32, out: *mut *mut rbmoe_attention) -> c_int;
+    pub fn rbmoe_attention_destroy(attention: *mut rbmoe_attention);
+    pub fn rbmoe_attention_forward(attention: *mut rbmoe_attention, sequences: i32, longest_queries: i32, longest_keys: i32,
+                                   query_begin: *const i32, query_count: *const i32, key_begin: *const i32, key_count:
+                                   *const i32, query_rows: i32, key_rows: i32, q: *const c_void, q_stride: i32, k: *const
+                                   c_void, k_stride: i32, v: *const c_void, v_stride: i32, causal: i32, scale: f32, out:
+                                   *mut c_void, lse: *mut f32) -> c_int;
+    pub fn rbmoe_attention_backward(attention: *mut rbmoe_attention, sequences: i32, longest_queries: i32, longest_keys:
+                                    i32, query_begin: *const i32, query_count: *const i32, key_begin: *const i32, key_count:
+                                    *const i32, query_rows: i32, key_rows: i32, q: *const c_void, q_stride: i32, k: *const
+                                    c_void, k_stride: i32, v: *const c_void, v_stride: i32, causal: i32, scale: f32, out:
+                                    *const c_void, lse: *const f32, grad_out: *const c_void, grad_q:
+                                    *mut c_void, grad_k: *mut c_void, grad_v: *mut c_void) -> c_int;
+    pub fn rbmoe_kv_cache_create(ctx: *mut rbmoe_ctx, kv_heads: i32, head_dim: i32, dtype: i32, cache_dtype: i32, page_rows:
+                                 i32, pages: i32, out: *mut *mut rbmoe_kv_cache) -> c_int;
+    pub fn rbmoe_kv_cache_destroy(cache: *mut rbmoe_kv_cache);
+    pub fn rbmoe_kv_cache_write(cache: *mut rbmoe_kv_cache, rows: i32, k: *const c_void, k_stride: i32, v: *const c_void,
+                                v_stride: i32, slots: *const i64) -> c_int;
+    pub fn rbmoe_kv_cache_read(cache: *mut rbmoe_kv_cache, rows: i32, k: *mut c_void, k_stride: i32, v: *mut c_void,
+                               v_stride: i32, slots: *const i64) -> c_int;
+    pub fn rbmoe_decode_create(ctx: *mut rbmoe_ctx, heads: i32, kv_heads: i32, head_dim: i32, dtype: i32, max_sequences:
+                               i32, out: *mut *mut rbmoe_decode) -> c_int;
+    pub fn rbmoe_decode_destroy(decode: *mut rbmoe_decode);
+    pub fn rbmoe_decode_attention(decode: *mut rbmoe_decode, cache: *mut rbmoe_kv_cache, sequences: i32, q: *const c_void,
+                                  q_stride: i32, tables: *const i32, table_pages: i32, lengths: *const i32, longest: i32,
+                                  scale: f32, out: *mut c_void) -> c_int;
     pub fn rbmoe_forward_timed(layer: *mut rbmoe_layer, x: *const c_void, tokens: i32, cols: i32, valid: *const u8,
                                router_bias: *const f32, residual: *const c_void, out: *mut c_void,
                                ms: *mut f32) -> c_int;

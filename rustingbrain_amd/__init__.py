@@ -1,4 +1,5 @@
 """MI355X (gfx950) mixture-of-experts layer behind RustingBrain's MoE interface."""
+from .attention import Attention, DecodeAttention, KvCache
 from .moe import (BackendUnavailable, Device, DeviceError, InvalidConfig, InvalidInput, Layout, MemoryBudget,
                   MoeCache, MoeConfig, MoeLayer, NetworkError, OutOfMemory, Unsupported, UNROUTED)
 from .operators import Muon, ResidualJoin
@@ -6,4 +7,4 @@ from .transformer import ParameterCounts, TransformerBuilder, TransformerConfig
 
 __all__ = ["BackendUnavailable", "Device", "DeviceError", "InvalidConfig", "InvalidInput", "Layout",
            "MemoryBudget", "MoeCache", "MoeConfig", "MoeLayer", "NetworkError", "OutOfMemory", "Unsupported",
-           "UNROUTED", "Muon", "ResidualJoin", "ParameterCounts", "TransformerBuilder", "TransformerConfig"]
+           "UNROUTED", "Attention", "DecodeAttention", "KvCache", "Muon", "ResidualJoin", "ParameterCounts", "TransformerBuilder", "TransformerConfig"]

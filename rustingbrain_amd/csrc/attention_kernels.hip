@@ -1,0 +1,681 @@
+// Attention of whole sequences with grouped heads, and its backward pass.
+//
+//   s_ij = scale q_i . k_j   for the keys j that row i sees: j < min(keys, i + keys - queries + 1) (causal), j < keys (not causal)
+//   out_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp s_ij
+//   backward, delta_i = dout_i . out_i:   dp_ij = dout_i . v_j,  ds_ij = p_ij (dp_ij - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij dout_i   (sums over the heads of a group too)
+//
+// All five products run on the matrix cores in blocks of 32 x 32 with f32 accumulators: bf16 rows 16 reduction elements an
+// instruction, f32 rows 2 (exact f32 products and sums).  A wave owns 32 rows (forward, dq) or 32 keys (dk, dv) and keeps
+// them as the instruction's B operand; the other side goes through LDS in tiles that a workgroup's four waves share.  A product of two
+// row arrays comes out with the lane's own row in its column and the tile's rows in its registers, in the order in which the next
+// product takes them as its B operand: scores never leave registers, and no lane hands a value to another except the row statistics.
+// The second product needs the tile with rows and columns exchanged, which the transposing LDS read gives (bf16), or a read
+// along the row (f32).  p and ds are rounded to bf16 for bf16 rows (the matrix cores take bf16 operands): 2^-9 a term at random, no more
+// than the rounding of the result itself; their sums, the running maximum and sum of the softmax and all accumulators are f32.
+//
+// Masked places: a masked score is replaced behind the product, whatever it was.  A masked p of zero times an infinity or NaN
+// in the tile would still be NaN, so a workgroup that ends with such a value goes over its tiles again and adds the blocks
+// on the diagonal row by row; nothing else is read twice.
+#include "attention_kernels.h"
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "rbmoe_kernels.h"
+
+namespace rbmoe {
+
+namespace {
+
+constexpr int kThreads = 256, kOwn = 128;  // a workgroup's threads, and rows or keys that it owns
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+__device__ uint32_t zero_piece[4];  // what is staged for rows and columns that are not there
+
+typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef uint32_t Any8 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+// 64 lanes' 16 bytes to consecutive LDS addresses (the same in all lanes) without registers on the way
+__device__ __forceinline__ void issue_dma(uint32_t lds_addr, const void* src) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
+}
+
+__device__ __forceinline__ float other_half_max(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// ---- a tile of rows in LDS ---------------------------------------------------------------------
+// Rows of D elements without padding, in 16-byte pieces; piece c of row r lies at place c ^ swizzle(r), so that the reads along rows
+// (eight rows, one piece) and the transposing reads (four rows, 32 bytes) both find their banks free.
+template <typename T, int D>
+struct Tile {
+    static constexpr int V = 16 / sizeof(T), CH = D / V, ROW = CH * 16;
+    static constexpr int KC = CH / 2;  // steps of a product along D: each takes two pieces of a row, one per half of the wave
+    static constexpr int DB = D / 32;  // blocks of 32 columns
+    static __device__ __forceinline__ int swizzle(int r) {
+        if constexpr (CH == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+        return (r & 3) << 2 | ((r >> 2) & 3);
+    }
+    static __device__ __forceinline__ const char* piece(const char* tile, int r, int c) { return tile + r * ROW + ((c ^ swizzle(r)) << 4); }
+
+    // ROWS rows from `first` on of a sequence's n; columns from head_dim on and rows from n on are zeros
+    template <int ROWS, bool A>
+    static __device__ __forceinline__ void stage(char* tile, const T* __restrict__ base, long long stride, int first, int n, int pieces) {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < ROWS * CH / kThreads; ++i) {
+            const int at = (i * (kThreads / 64) + wave) * 64, p = at + lane, r = p / CH, c = (p % CH) ^ swizzle(r);
+            const bool there = first + r < n && c < pieces;
+            const T* const src = base + (long long)(first + r) * stride + c * V;
+            if constexpr (A) {
+                issue_dma(lds_address(tile) + at * 16, there ? (const void*)src : (const void*)zero_piece);
+            } else {
+                Any16 x = {0, 0, 0, 0};
+                if (there) x = *reinterpret_cast<const Any16*>(src);
+                *reinterpret_cast<uint4*>(tile + p * 16) = make_uint4(x.x, x.y, x.z, x.w);
+            }
+        }
+    }
+    static __device__ __forceinline__ float element(const char* tile, int r, int d) {
+        return to_f32(*reinterpret_cast<const T*>(piece(tile, r, d / V) + d % V * sizeof(T)));
+    }
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16_t> {
+    typedef bf16x8 Rows;  // 8 elements of a row
+    struct Cols {         // a 32 x 32 block of scores as the second product takes it
+        bf16x8 c[2];
+    };
+    static __device__ __forceinline__ floatx16 rows(const Rows& a, const Rows& b, const floatx16& c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Cols cols(const floatx16& p) {
+        Cols r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            r.c[i] = __builtin_bit_cast(bf16x8, make_uint4(pack2(p[8 * i], p[8 * i + 1]), pack2(p[8 * i + 2], p[8 * i + 3]),
+                                                           pack2(p[8 * i + 4], p[8 * i + 5]), pack2(p[8 * i + 6], p[8 * i + 7])));
+        return r;
+    }
+    static __device__ __forceinline__ float total(const Cols& p, float sum) {  // of the lane's own values
+        typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+        const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint4 w = __builtin_bit_cast(uint4, p.c[i]);
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w.x), one, sum, false);
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w.y), one, sum, false);
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w.z), one, sum, false);
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w.w), one, sum, false);
+        }
+        return sum;
+    }
+    static __device__ __forceinline__ float rounded(float v) { return bf16_bits_to_f32(f32_to_bf16_bits(v)); }
+    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]
+    template <int D>
+    static __device__ __forceinline__ void add(floatx16 (&acc)[D / 32], const char* tile, int row0, const Cols& p) {
+        typedef Tile<bf16_t, D> T;
+        const int lane = threadIdx.x & 63, h = lane >> 5, j = (lane >> 2) & 3;
+        const int c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), in = (lane & 1) * 8;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                const int r = row0 + 16 * k + 4 * h + j;
+                union {
+                    v4i16 x[2];
+                    bf16x8 v;
+                } u;
+                u.x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(T::piece(tile, r, 4 * b + c0) + in));
+                u.x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(T::piece(tile, r + 8, 4 * b + c0) + in));
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, p.c[k], acc[b], 0, 0, 0);
+            }
+    }
+};
+template <>
+struct Mma<float> {
+    typedef float4 Rows;
+    typedef floatx16 Cols;
+    static __device__ __forceinline__ floatx16 rows(const Rows& a, const Rows& b, floatx16 c) {
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Cols cols(const floatx16& p) { return p; }
+    static __device__ __forceinline__ float rounded(float v) { return v; }
+    template <int D>
+    static __device__ __forceinline__ void add(floatx16 (&acc)[D / 32], const char* tile, int row0, const Cols& p) {
+        typedef Tile<float, D> T;
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int r = row0 + 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                const float x = *reinterpret_cast<const float*>(T::piece(tile, r, 8 * b + ((lane & 31) >> 2)) + (lane & 3) * 4);
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], acc[b], 0, 0, 0);
+            }
+        }
+    }
+};
+
+template <typename T>
+using RowsOf = typename Mma<T>::Rows;
+
+template <typename T, int D>
+__device__ __forceinline__ RowsOf<T> row_pieces(const char* tile, int row0, int kc) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const RowsOf<T>*>(Tile<T, D>::piece(tile, row0 + (lane & 31), 2 * kc + (lane >> 5)));
+}
+// The product of 32 of the tile's rows with the wave's own: register i of lane l holds tile row 8 (i / 4) + 4 (l / 32) + i % 4, own row l % 32.
+template <typename T, int D>
+__device__ __forceinline__ floatx16 product(const char* tile, int row0, const RowsOf<T> (&own)[Tile<T, D>::KC]) {
+    floatx16 c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+#pragma unroll
+    for (int kc = 0; kc < Tile<T, D>::KC; ++kc) c = Mma<T>::rows(row_pieces<T, D>(tile, row0, kc), own[kc], c);
+    return c;
+}
+__device__ __forceinline__ int block_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (i & 3); }
+
+// Mma::add for a block of which some places are masked, whatever the tile holds there: row by row, the places that `sees`(row) allows.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void add_seen(floatx16 (&acc)[D / 32], const char* tile, int row0, const floatx16& p, F sees) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma clang loop unroll(disable)
+    for (int r = 0; r < 32; ++r) {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x = i == (r >> 3) * 4 + (r & 3) ? p[i] : x;
+        x = Mma<T>::rounded(__shfl(x, (lane & 31) + 32 * ((r >> 2) & 1)));
+        const bool seen = sees(r);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float y = Tile<T, D>::element(tile, row0 + r, 32 * b + 8 * (e >> 2) + 4 * h + (e & 3));
+                acc[b][e] = seen ? __builtin_fmaf(x, y, acc[b][e]) : acc[b][e];
+            }
+    }
+}
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const floatx16 (&acc)[N]) {
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bad |= !(fabsf(acc[b][i]) < __builtin_inff());
+    return bad;
+}
+
+// ---- a wave's own rows ---------------------------------------------------------------------------
+// The row of lane l % 32 as the products' B operand, zeros where it or its columns are not there.
+template <typename T, int D>
+__device__ __forceinline__ void load_own(const T* __restrict__ row, bool there, int pieces, RowsOf<T> (&own)[Tile<T, D>::KC]) {
+    const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int kc = 0; kc < Tile<T, D>::KC; ++kc) {
+        Any16 x = {0, 0, 0, 0};
+        if (there && 2 * kc + h < pieces) x = *reinterpret_cast<const Any16*>(row + (2 * kc + h) * Tile<T, D>::V);
+        own[kc] = __builtin_bit_cast(RowsOf<T>, x);
+    }
+}
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<Any16*>(p) = Any16{__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)};
+}
+__device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
+    *reinterpret_cast<Any8*>(p) = Any8{pack2(a, b), pack2(c, d)};
+}
+// acc[d][own] of lane l's own row to `row`, times `factor`
+template <typename T, int D>
+__device__ __forceinline__ void store_own(const floatx16 (&acc)[D / 32], T* row, float factor, int head_dim) {
+    const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = 32 * b + 8 * e + 4 * h;
+            if (d >= head_dim) continue;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = acc[b][4 * e + i] * factor;
+            store4(row + d, x[0], x[1], x[2], x[3]);
+        }
+}
+
+// ---- sequences -------------------------------------------------------------------------------------
+struct Sequence {
+    int q0, nq, k0, nk;
+};
+// (whatever the arrays hold, a sequence lies inside the rows that the call names)
+__device__ __forceinline__ Sequence sequence_of(const AttentionCall& a, int i) {
+    Sequence s;
+    s.q0 = min(max(a.query_begin[i], 0), a.query_rows);
+    s.nq = min(max(a.query_count[i], 0), min(a.longest_queries, a.query_rows - s.q0));
+    s.k0 = min(max(a.key_begin[i], 0), a.key_rows);
+    s.nk = min(max(a.key_count[i], 0), min(a.longest_keys, a.key_rows - s.k0));
+    return s;
+}
+// Which tile, head and sequence a workgroup takes.  Workgroup i runs on XCD i % 8: where the heads divide among them, every XCD has
+// its own heads (neighbours, so that a group's heads share their keys in one L2), otherwise all take turns.  Tiles in descending order: the last are the
+// longest where later rows see more keys.
+struct Place {
+    int tile, head, sequence;
+};
+__device__ __forceinline__ Place place_of(int heads, int sequences, int tiles, bool descending) {
+    int i = blockIdx.x;
+    Place p;
+    if (heads % 8 == 0) {
+        const int per = heads / 8, xcd = i & 7;
+        i >>= 3;
+        p.head = xcd * per + i % per;
+        i /= per;
+    } else {
+        p.head = i % heads;
+        i /= heads;
+    }
+    p.sequence = i % sequences;
+    p.tile = i / sequences;
+    if (descending) p.tile = tiles - 1 - p.tile;
+    return p;
+}
+
+// ---- forward ----------------------------------------------------------------------------------------
+template <typename T>
+constexpr int tile_rows() {
+    return sizeof(T) == 2 ? 64 : 32;
+}
+
+template <typename T, int D, bool A>
+__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(AttentionCall a) {
+    typedef Tile<T, D> Tl;
+    constexpr int N = tile_rows<T>(), NB = N / 32, BYTES = N * Tl::ROW;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of keys and values
+    const int tiles = (a.longest_queries + kOwn - 1) / kOwn;
+    const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
+    const Sequence s = sequence_of(a, at.sequence);
+    const int first = at.tile * kOwn;
+    if (first >= s.nq) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
+    const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / Tl::V;
+    const T* const k = static_cast<const T*>(a.k) + (long long)s.k0 * a.k_stride + (long long)kv * a.head_dim;
+    const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
+    const int wave_first = first + 32 * wave, row = wave_first + (lane & 31);
+    const bool there = row < s.nq;
+    RowsOf<T> q[Tl::KC];
+    load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
+
+    // the keys that a row sees are those below its limit
+    auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
+    const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
+    const int end = limit(min(first + kOwn, s.nq) - 1);
+    const float c = a.scale * kLog2e;
+    floatx16 acc[Tl::DB];
+    float m, l;
+
+    auto pass = [&](auto careful) {
+#pragma unroll
+        for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][i] = 0.0f;
+        m = -__builtin_inff();
+        l = 0.0f;
+        auto stage = [&](int buf, int t) {
+            char* const to = attention_lds + buf * 2 * BYTES;
+            Tl::template stage<N, A>(to, k, a.k_stride, t, s.nk, pieces);
+            Tl::template stage<N, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
+        };
+        if (end > 0) stage(0, 0);
+        for (int t = 0, buf = 0; t < end; t += N, buf ^= 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile has landed
+            __syncthreads();                                  // and the others'; all are done with the other stage
+            if (t + N < end) stage(buf ^ 1, t + N);
+            if (t >= most || wave_first >= s.nq) continue;
+            const char* const kt = attention_lds + buf * 2 * BYTES;
+            const char* const vt = kt + BYTES;
+            floatx16 p[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) p[b] = product<T, D>(kt, 32 * b, q);
+            if (t + N > least) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t + 32 * b + block_row(i) >= own_limit) p[b][i] = -__builtin_inff();
+            }
+            float top = p[0][0];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, p[b][i]);
+            top = other_half_max(top) * c;
+            // The reference of the exponents moves only when a score passes it by 2^8: the results are the same, sums and accumulators
+            // have room for it, and after a few tiles nothing has to be scaled.
+            if (__any(top > m + 8.0f)) {
+                const float next = fmaxf(m, top), down = next == m ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+                m = next;
+                l *= down;
+#pragma unroll
+                for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[b][i] *= down;
+            }
+            const float reference = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[b][i], c, -reference));
+                    l += p[b][i];
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (decltype(careful)::value && t + N > least)
+                    add_seen<T, D>(acc, vt, 32 * b, p[b], [&](int r) { return t + 32 * b + r < own_limit; });
+                else
+                    Mma<T>::template add<D>(acc, vt, 32 * b, Mma<T>::cols(p[b]));
+            }
+        }
+    };
+    pass(std::false_type{});
+    if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
+
+    l = other_half_sum(l);
+    if (!there) return;
+    const long long to = (long long)(s.q0 + row) * a.heads + at.head;
+    store_own<T, D>(acc, static_cast<T*>(a.out) + to * a.head_dim, l == 0.0f ? 0.0f : 1.0f / l, a.head_dim);
+    if (a.lse && h == 0)
+        a.lse[(long long)at.head * a.query_rows + s.q0 + row] =
+            l == 0.0f ? -__builtin_inff() : ((m == -__builtin_inff() ? 0.0f : m) + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---- backward: gradients of the queries ------------------------------------------------------------------
+template <typename T, int D, bool A>
+__global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_kernel(AttentionCall a) {
+    typedef Tile<T, D> Tl;
+    constexpr int N = tile_rows<T>(), NB = N / 32, BYTES = N * Tl::ROW;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];
+    const int tiles = (a.longest_queries + kOwn - 1) / kOwn;
+    const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
+    const Sequence s = sequence_of(a, at.sequence);
+    const int first = at.tile * kOwn;
+    if (first >= s.nq) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
+    const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / Tl::V;
+    const T* const k = static_cast<const T*>(a.k) + (long long)s.k0 * a.k_stride + (long long)kv * a.head_dim;
+    const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
+    const int wave_first = first + 32 * wave, row = wave_first + (lane & 31);
+    const bool there = row < s.nq;
+    const long long in_out = ((long long)(s.q0 + row) * a.heads + at.head) * a.head_dim, in_lse = (long long)at.head * a.query_rows + s.q0 + row;
+    RowsOf<T> q[Tl::KC], dout[Tl::KC];
+    load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
+    load_own<T, D>(static_cast<const T*>(a.grad_out) + in_out, there, pieces, dout);
+
+    float delta = 0.0f;
+#pragma unroll
+    for (int kc = 0; kc < Tl::KC; ++kc) {
+        if (!there || 2 * kc + h >= pieces) continue;
+        float x[Tl::V], y[Tl::V];
+        const long long at_piece = in_out + (2 * kc + h) * Tl::V;
+        const Any16 o = *reinterpret_cast<const Any16*>(static_cast<const T*>(a.out) + at_piece);
+        Vec16<T>::widen(make_uint4(o.x, o.y, o.z, o.w), x);
+        Vec16<T>::widen(__builtin_bit_cast(uint4, dout[kc]), y);
+#pragma unroll
+        for (int i = 0; i < Tl::V; ++i) delta = __builtin_fmaf(x[i], y[i], delta);
+    }
+    delta = other_half_sum(delta);
+    const float lse2 = there ? a.lse[in_lse] * kLog2e : 0.0f;
+
+    auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
+    const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
+    const int end = limit(min(first + kOwn, s.nq) - 1);
+    const float c = a.scale * kLog2e;
+    // For bf16 rows delta comes from rounded rows of `out`, and ds is rounded.  Both errors make a row's ds add up to something
+    // else than its true sum of zero, and where keys share a direction that goes along it.  So the sum of the rounded ds is taken
+    // off again in proportion to p (grad_q -= sum * mean key), and delta handed on as what makes the sum of the unrounded ones zero.
+    constexpr bool mend = sizeof(T) == 2;
+    floatx16 acc[Tl::DB], mean[mend ? Tl::DB : 1];
+    float sum, rounded_sum;
+
+    auto pass = [&](auto careful) {
+#pragma unroll
+        for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][i] = mean[mend ? b : 0][i] = 0.0f;
+        sum = rounded_sum = 0.0f;
+        auto stage = [&](int buf, int t) {
+            char* const to = attention_lds + buf * 2 * BYTES;
+            Tl::template stage<N, A>(to, k, a.k_stride, t, s.nk, pieces);
+            Tl::template stage<N, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
+        };
+        if (end > 0) stage(0, 0);
+        for (int t = 0, buf = 0; t < end; t += N, buf ^= 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (t + N < end) stage(buf ^ 1, t + N);
+            if (t >= most || wave_first >= s.nq) continue;
+            const char* const kt = attention_lds + buf * 2 * BYTES;
+            const char* const vt = kt + BYTES;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                floatx16 p = product<T, D>(kt, 32 * b, q), dp = product<T, D>(vt, 32 * b, dout);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -lse2));
+                    dp[i] = p[i] * (dp[i] - delta);
+                }
+                if (t + N > least) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t + 32 * b + block_row(i) >= own_limit) p[i] = dp[i] = 0.0f;
+                }
+                const auto ds = Mma<T>::cols(dp);
+                if constexpr (mend) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum += dp[i];
+                    rounded_sum = Mma<T>::total(ds, rounded_sum);
+                }
+                if (decltype(careful)::value && t + N > least) {
+                    auto sees = [&](int r) { return t + 32 * b + r < own_limit; };
+                    add_seen<T, D>(acc, kt, 32 * b, dp, sees);
+                    if constexpr (mend) add_seen<T, D>(mean, kt, 32 * b, p, sees);
+                } else {
+                    Mma<T>::template add<D>(acc, kt, 32 * b, ds);
+                    if constexpr (mend) Mma<T>::template add<D>(mean, kt, 32 * b, Mma<T>::cols(p));
+                }
+            }
+        }
+    };
+    pass(std::false_type{});
+    if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
+    if constexpr (mend) {
+        rounded_sum = other_half_sum(rounded_sum);
+        delta += other_half_sum(sum);
+#pragma unroll
+        for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_fmaf(-rounded_sum, mean[b][i], acc[b][i]);
+    }
+    if (there && h == 0) a.delta[in_lse] = delta;
+    if (there)
+        store_own<T, D>(acc, static_cast<T*>(a.grad_q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, a.scale, a.head_dim);
+}
+
+// ---- backward: gradients of keys and values -------------------------------------------------------------
+template <typename T, int D, bool A>
+__global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_kv_kernel(AttentionCall a) {
+    typedef Tile<T, D> Tl;
+    constexpr int N = tile_rows<T>(), NB = N / 32, BYTES = N * Tl::ROW, STAGE = 2 * BYTES + 2 * N * 4;
+    extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
+    const int tiles = (a.longest_keys + kOwn - 1) / kOwn;
+    const Place at = place_of(a.kv_heads, a.sequences, tiles, false);
+    const Sequence s = sequence_of(a, at.sequence);
+    const int first = at.tile * kOwn, kv = at.head, group = a.heads / a.kv_heads;
+    if (first >= s.nk) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int pieces = a.head_dim / Tl::V;
+    const int wave_first = first + 32 * wave, key = wave_first + (lane & 31);
+    const bool there = key < s.nk;
+    RowsOf<T> k[Tl::KC], v[Tl::KC];
+    load_own<T, D>(static_cast<const T*>(a.k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there, pieces, k);
+    load_own<T, D>(static_cast<const T*>(a.v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, pieces, v);
+
+    // the rows that see a key are those from its start on
+    auto start = [&](int j) { return a.causal ? max(j - (s.nk - s.nq), 0) : 0; };
+    const int own_start = start(key), least = start(wave_first), most = start(wave_first + 31);
+    const int begin = start(first) / N * N, turns = begin < s.nq ? (s.nq - begin + N - 1) / N : 0, all = turns * group;
+    const float c = a.scale * kLog2e;
+    floatx16 dk[Tl::DB], dv[Tl::DB];
+
+    auto pass = [&](auto careful) {
+#pragma unroll
+        for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.0f;
+        // turn i: head i / turns of the group, rows from begin + N (i % turns) on
+        auto stage = [&](int buf, int i) {
+            const int head = kv * group + i / turns, t = begin + i % turns * N;
+            char* const to = attention_lds + buf * STAGE;
+            if (threadIdx.x < 2 * N) {
+                const int r = threadIdx.x % N;
+                const float* const from = threadIdx.x < N ? a.lse : a.delta;
+                float x = 0.0f;
+                if (t + r < s.nq) x = from[(long long)head * a.query_rows + s.q0 + t + r];
+                *reinterpret_cast<float*>(to + 2 * BYTES + threadIdx.x * 4) = threadIdx.x < N ? x * kLog2e : x;
+            }
+            Tl::template stage<N, A>(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
+            Tl::template stage<N, A>(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
+                                     (long long)a.heads * a.head_dim, t, s.nq, pieces);
+        };
+        if (all > 0) stage(0, 0);
+        for (int i = 0, buf = 0; i < all; ++i, buf ^= 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (i + 1 < all) stage(buf ^ 1, i + 1);
+            const int t = begin + i % turns * N;
+            if (t + N <= least || wave_first >= s.nk) continue;
+            const char* const qt = attention_lds + buf * STAGE;
+            const char* const ot = qt + BYTES;
+            const float* const lse2 = reinterpret_cast<const float*>(ot + BYTES);
+            const bool masked = t < most || t + N > s.nq;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                floatx16 p = product<T, D>(qt, 32 * b, k), dp = product<T, D>(ot, 32 * b, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 32 * b + block_row(4 * e);
+                    const float4 x = *reinterpret_cast<const float4*>(lse2 + r), y = *reinterpret_cast<const float4*>(lse2 + N + r);
+                    const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        p[4 * e + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[4 * e + j], c, -xs[j]));
+                        dp[4 * e + j] = p[4 * e + j] * (dp[4 * e + j] - ys[j]);
+                    }
+                }
+                auto sees = [&](int r) { return t + 32 * b + r >= own_start && t + 32 * b + r < s.nq; };
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (!sees(block_row(e))) p[e] = dp[e] = 0.0f;
+                }
+                if (decltype(careful)::value && masked) {
+                    add_seen<T, D>(dv, ot, 32 * b, p, sees);
+                    add_seen<T, D>(dk, qt, 32 * b, dp, sees);
+                } else {
+                    Mma<T>::template add<D>(dv, ot, 32 * b, Mma<T>::cols(p));
+                    Mma<T>::template add<D>(dk, qt, 32 * b, Mma<T>::cols(dp));
+                }
+            }
+        }
+    };
+    pass(std::false_type{});
+    if (__syncthreads_or(any_not_finite(dk) || any_not_finite(dv))) pass(std::true_type{});
+    if (there) {
+        store_own<T, D>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, a.scale, a.head_dim);
+        store_own<T, D>(dv, static_cast<T*>(a.grad_v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, 1.0f, a.head_dim);
+    }
+}
+
+bool whole_pieces(const void* p, long long stride, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+}
+
+// f(element type, padded head width, rows start on 16-byte boundaries)
+template <typename F>
+hipError_t with_kernel(bool bf16, int head_dim, bool aligned, F f) {
+    auto wide = [&](auto type) -> hipError_t {
+        typedef decltype(type) T;
+        if (head_dim <= 64)
+            return aligned ? f(T{}, std::integral_constant<int, 64>{}, std::true_type{}) : f(T{}, std::integral_constant<int, 64>{}, std::false_type{});
+        return aligned ? f(T{}, std::integral_constant<int, 128>{}, std::true_type{}) : f(T{}, std::integral_constant<int, 128>{}, std::false_type{});
+    };
+    return bf16 ? wide(bf16_t{}) : wide(float{});
+}
+
+template <typename K>
+hipError_t launch(K kernel, std::atomic<unsigned long long>& once, const AttentionCall& a, int tiles, int heads, int lds, hipStream_t s) {
+    const hipError_t e = once_per_device(once, [&] {
+        return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    });
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles * heads * a.sequences), dim3(kThreads), lds, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream_t s) {
+    const int size = bf16 ? 2 : 4;
+    const bool aligned = whole_pieces(a.k, a.k_stride, size) && whole_pieces(a.v, a.v_stride, size);
+    return with_kernel(bf16, a.head_dim, aligned, [&](auto type, auto width, auto whole) {
+        typedef decltype(type) T;
+        constexpr int D = decltype(width)::value;
+        static std::atomic<unsigned long long> once{0};
+        return launch(attention_forward_kernel<T, D, decltype(whole)::value>, once, a, (a.longest_queries + kOwn - 1) / kOwn, a.heads,
+                      4 * tile_rows<T>() * Tile<T, D>::ROW, s);
+    });
+}
+
+hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStream_t s) {
+    const int size = bf16 ? 2 : 4;
+    hipError_t e = hipSuccess;
+    if (a.longest_queries > 0) {
+        const bool aligned = whole_pieces(a.k, a.k_stride, size) && whole_pieces(a.v, a.v_stride, size);
+        e = with_kernel(bf16, a.head_dim, aligned, [&](auto type, auto width, auto whole) {
+            typedef decltype(type) T;
+            constexpr int D = decltype(width)::value;
+            static std::atomic<unsigned long long> once{0};
+            return launch(attention_grad_q_kernel<T, D, decltype(whole)::value>, once, a, (a.longest_queries + kOwn - 1) / kOwn, a.heads,
+                          4 * tile_rows<T>() * Tile<T, D>::ROW, s);
+        });
+    }
+    if (e != hipSuccess || a.longest_keys == 0) return e;
+    const bool aligned = whole_pieces(a.q, a.q_stride, size) && whole_pieces(a.grad_out, a.head_dim, size);
+    return with_kernel(bf16, a.head_dim, aligned, [&](auto type, auto width, auto whole) {
+        typedef decltype(type) T;
+        constexpr int D = decltype(width)::value;
+        static std::atomic<unsigned long long> once{0};
+        return launch(attention_grad_kv_kernel<T, D, decltype(whole)::value>, once, a, (a.longest_keys + kOwn - 1) / kOwn, a.kv_heads,
+                      4 * tile_rows<T>() * Tile<T, D>::ROW + 4 * tile_rows<T>() * 4, s);
+    });
+}
+
+}  // namespace rbmoe

@@ -1,0 +1,635 @@
+// A paged cache of keys and values: rows written to it, read back from it, and the attention of one new row a sequence over it.
+//
+// int8 rows have a scale each (per token and head): a = max |x|, scale = a / 127, stored round(127 x / a), ties to even, read back as
+// stored * scale.  (127 x is exact for bf16 rows, so one division decides the rounding, and ties are ties.)  A row with an
+// infinity or NaN reads back as NaN whole.
+#include "kv_cache_kernels.h"
+
+#include <algorithm>
+
+#include "rbmoe_kernels.h"
+
+namespace rbmoe {
+
+namespace {
+
+typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+
+__device__ __forceinline__ unsigned char* cache_block(const CachePool& p, long long page, int head) {
+    return p.base + ((size_t)page * p.kv_heads + head) * p.block_bytes();
+}
+// where element d of row r (within its page) of the values stands, in elements
+template <int W, int G>
+__device__ __forceinline__ int value_at(int r, int d) {
+    return ((r / G) * W + d) * G + r % G;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const Any16 x = *reinterpret_cast<const Any16*>(p);
+        Vec16<T>::widen(make_uint4(x.x, x.y, x.z, x.w), v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Any16 x = *reinterpret_cast<const Any16*>(p + 4 * i);
+            v[4 * i] = __uint_as_float(x.x); v[4 * i + 1] = __uint_as_float(x.y);
+            v[4 * i + 2] = __uint_as_float(x.z); v[4 * i + 3] = __uint_as_float(x.w);
+        }
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<Any16*>(p + 4 * i) = Any16{__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])};
+}
+__device__ __forceinline__ void store8(bf16_t* p, const float (&v)[8]) {
+    *reinterpret_cast<Any16*>(p) = Any16{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
+}
+__device__ __forceinline__ void store8(int8_t* p, const float (&v)[8]) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w[i] = ((uint32_t)(int)v[4 * i] & 255) | ((uint32_t)(int)v[4 * i + 1] & 255) << 8 | ((uint32_t)(int)v[4 * i + 2] & 255) << 16 |
+               (uint32_t)(int)v[4 * i + 3] << 24;
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+// The 8 values of each of a row's TR threads, rounded to whole numbers of the returned scale.
+template <int TR>
+__device__ __forceinline__ float quantize(float (&v)[8]) {
+    float most = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        most = fmaxf(most, fabsf(v[i]));
+        bad |= !(fabsf(v[i]) < __builtin_inff());
+    }
+    // (a mark that the maximum hands on: infinities come out of it anyway)
+    most = group_fmax(bad ? __builtin_inff() : most, TR);
+    if (!(most < __builtin_inff())) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        return __builtin_nanf("");
+    }
+    const float small = most > 0x1p100f ? 0x1p-20f : 1.0f;  // 127 x stays in range
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = most > 0.0f ? rintf(__fdiv_rn(__fmul_rn(127.0f, v[i] * small), most * small)) : 0.0f;
+    return __fdiv_rn(most, 127.0f);
+}
+
+// A workgroup takes ROWS rows of one head, 8 elements a thread.  Keys go to their places at once; values pass through LDS, where a
+// thread picks up a column's elements of neighbouring places: runs of rows in neighbouring places are written in
+// pieces of up to 16 bytes.
+template <int W>
+constexpr int cache_rows() {
+    return 16 * (256 / W);
+}
+// run: how many rows from this one on lie in neighbouring places (a mask of "the next row lies behind this one")
+__device__ __forceinline__ int run_from(uint64_t next, int r) {
+    const uint64_t stops = ~(next >> r);
+    return stops ? (int)__builtin_ctzll(stops) + 1 : 64;
+}
+
+template <typename T, typename C, int W>
+__global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
+    constexpr int R = cache_rows<W>(), TR = W / 8, G = 16 / sizeof(C);
+    __shared__ C values[R][W + 16 / sizeof(C)];
+    __shared__ long long places[R];
+    __shared__ uint64_t neighbours;
+    const CachePool& p = a.pool;
+    const int head = blockIdx.y, first = blockIdx.x * R, tid = threadIdx.x;
+    const long long slots = (long long)p.pages << p.page_shift;
+    if (tid < 64) {
+        long long at = -1;
+        if (tid < R && first + tid < a.rows) at = a.slots[first + tid];
+        if (at < 0 || at >= slots) at = -1;
+        const long long next = __shfl_down(at, 1);
+        const uint64_t mask = __ballot(tid + 1 < R && at >= 0 && next == at + 1);
+        if (tid < R) places[tid] = at;
+        if (tid == 0) neighbours = mask;
+    }
+    __syncthreads();
+    const int page_mask = (1 << p.page_shift) - 1, c = tid % TR * 8;
+#pragma unroll
+    for (int i = 0; i < R * TR / 256; ++i) {
+        const int r = i * (256 / TR) + tid / TR;
+        const long long at = places[r];
+        float k[8] = {}, v[8] = {};
+        if (at >= 0 && c < p.head_dim) {
+            load8(static_cast<const T*>(a.k) + (long long)(first + r) * a.k_stride + (long long)head * p.head_dim + c, k);
+            load8(static_cast<const T*>(a.v) + (long long)(first + r) * a.v_stride + (long long)head * p.head_dim + c, v);
+        }
+        unsigned char* const block = cache_block(p, at >= 0 ? at >> p.page_shift : 0, head);
+        const int row = (int)(at & page_mask);
+        if constexpr (sizeof(C) == 1) {
+            const float k_scale = quantize<TR>(k), v_scale = quantize<TR>(v);
+            if (at >= 0 && tid % TR == 0) {
+                float* const scales = reinterpret_cast<float*>(block + 2 * p.half_bytes());
+                scales[row] = k_scale;
+                scales[(1 << p.page_shift) + row] = v_scale;
+            }
+        }
+        if (at >= 0) store8(reinterpret_cast<C*>(block) + (size_t)row * W + c, k);
+        store8(&values[r][c], v);
+    }
+    __syncthreads();
+    // column d of 16 rows
+    const int d = tid % W, end = tid / W * 16 + 16;
+    const uint64_t next = neighbours;
+    for (int r = end - 16; r < end;) {
+        const long long at = places[r];
+        if (at < 0) {
+            ++r;
+            continue;
+        }
+        const int row = (int)(at & page_mask), run = min(run_from(next, r), end - r);
+        C* const to = reinterpret_cast<C*>(cache_block(p, at >> p.page_shift, head) + p.half_bytes()) + value_at<W, G>(row, d);
+        int n = G;
+        while (n > 1 && (n > run || (row & (n - 1)))) n >>= 1;
+        auto put = [&](auto piece, auto count) {
+            typedef decltype(piece) P;
+            constexpr int N = decltype(count)::value;
+            union {
+                P p;
+                C c[N];
+            } u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) u.c[i] = values[r + i][d];
+            *reinterpret_cast<P*>(to) = u.p;
+        };
+        constexpr int E = sizeof(C);
+        if (n * E == 16) put(uint4{}, std::integral_constant<int, 16 / E>{});
+        else if (n * E == 8) put(uint2{}, std::integral_constant<int, 8 / E>{});
+        else if (n * E == 4) put(uint32_t{}, std::integral_constant<int, 4 / E>{});
+        else if constexpr (E <= 2) {
+            if (n * E == 2) put(uint16_t{}, std::integral_constant<int, 2 / E>{});
+            else if constexpr (E == 1) put(uint8_t{}, std::integral_constant<int, 1>{});
+        }
+        r += n;
+    }
+}
+
+__device__ __forceinline__ void widen8(const float* p, float (&v)[8]) { load8(p, v); }
+__device__ __forceinline__ void widen8(const bf16_t* p, float (&v)[8]) { load8(p, v); }
+__device__ __forceinline__ void widen8(const int8_t* p, float (&v)[8]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = (float)(int8_t)(w.x >> (8 * i));
+        v[4 + i] = (float)(int8_t)(w.y >> (8 * i));
+    }
+}
+
+// The way back: columns' runs to LDS, then rows.  Rows without a place are zeros.
+template <typename T, typename C, int W>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheRows a) {
+    constexpr int R = cache_rows<W>(), TR = W / 8, G = 16 / sizeof(C);
+    __shared__ C values[R][W + 16 / sizeof(C)];
+    __shared__ long long places[R];
+    __shared__ uint64_t neighbours;
+    const CachePool& p = a.pool;
+    const int head = blockIdx.y, first = blockIdx.x * R, tid = threadIdx.x;
+    const long long slots = (long long)p.pages << p.page_shift;
+    if (tid < 64) {
+        long long at = -1;
+        if (tid < R && first + tid < a.rows) at = a.slots[first + tid];
+        if (at < 0 || at >= slots) at = -1;
+        const long long next = __shfl_down(at, 1);
+        const uint64_t mask = __ballot(tid + 1 < R && at >= 0 && next == at + 1);
+        if (tid < R) places[tid] = at;
+        if (tid == 0) neighbours = mask;
+    }
+    __syncthreads();
+    const int page_mask = (1 << p.page_shift) - 1;
+    const int d = tid % W, end = tid / W * 16 + 16;
+    const uint64_t next = neighbours;
+    for (int r = end - 16; r < end;) {
+        const long long at = places[r];
+        if (at < 0) {
+            ++r;
+            continue;
+        }
+        const int row = (int)(at & page_mask), run = min(run_from(next, r), end - r);
+        const C* const from = reinterpret_cast<const C*>(cache_block(p, at >> p.page_shift, head) + p.half_bytes()) + value_at<W, G>(row, d);
+        int n = G;
+        while (n > 1 && (n > run || (row & (n - 1)))) n >>= 1;
+        auto take = [&](auto piece, auto count) {
+            typedef decltype(piece) P;
+            constexpr int N = decltype(count)::value;
+            union {
+                P p;
+                C c[N];
+            } u;
+            u.p = *reinterpret_cast<const P*>(from);
+#pragma unroll
+            for (int i = 0; i < N; ++i) values[r + i][d] = u.c[i];
+        };
+        constexpr int E = sizeof(C);
+        if (n * E == 16) take(uint4{}, std::integral_constant<int, 16 / E>{});
+        else if (n * E == 8) take(uint2{}, std::integral_constant<int, 8 / E>{});
+        else if (n * E == 4) take(uint32_t{}, std::integral_constant<int, 4 / E>{});
+        else if constexpr (E <= 2) {
+            if (n * E == 2) take(uint16_t{}, std::integral_constant<int, 2 / E>{});
+            else if constexpr (E == 1) take(uint8_t{}, std::integral_constant<int, 1>{});
+        }
+        r += n;
+    }
+    __syncthreads();
+    const int c = tid % TR * 8;
+    if (c >= p.head_dim) return;
+#pragma unroll
+    for (int i = 0; i < R * TR / 256; ++i) {
+        const int r = i * (256 / TR) + tid / TR;
+        if (first + r >= a.rows) continue;
+        const long long at = places[r];
+        float k[8] = {}, v[8] = {};
+        if (at >= 0) {
+            const unsigned char* const block = cache_block(p, at >> p.page_shift, head);
+            const int row = (int)(at & page_mask);
+            widen8(reinterpret_cast<const C*>(block) + (size_t)row * W + c, k);
+            widen8(&values[r][c], v);
+            if constexpr (sizeof(C) == 1) {
+                const float* const scales = reinterpret_cast<const float*>(block + 2 * p.half_bytes());
+                const float k_scale = scales[row], v_scale = scales[(1 << p.page_shift) + row];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    k[j] *= k_scale;
+                    v[j] *= v_scale;
+                }
+            }
+        }
+        store8(static_cast<T*>(a.k) + (long long)(first + r) * a.k_stride + (long long)head * p.head_dim + c, k);
+        store8(static_cast<T*>(a.v) + (long long)(first + r) * a.v_stride + (long long)head * p.head_dim + c, v);
+    }
+}
+
+// f(type of the rows, type of the cache, width)
+template <typename F>
+hipError_t with_types(const CachePool& p, bool bf16_rows, F f) {
+    auto wide = [&](auto row, auto cache) -> hipError_t {
+        return p.width() == 64 ? f(row, cache, std::integral_constant<int, 64>{}) : f(row, cache, std::integral_constant<int, 128>{});
+    };
+    if (bf16_rows) return p.dtype == RBMOE_I8 ? wide(bf16_t{}, int8_t{}) : wide(bf16_t{}, bf16_t{});
+    return p.dtype == RBMOE_I8 ? wide(float{}, int8_t{}) : wide(float{}, float{});
+}
+
+}  // namespace
+
+size_t cache_bytes(const CachePool& p) { return (size_t)p.pages * p.kv_heads * p.block_bytes(); }
+
+hipError_t launch_cache_write(const CacheRows& a, bool bf16_rows, hipStream_t s) {
+    return with_types(a.pool, bf16_rows, [&](auto row, auto cache, auto width) {
+        constexpr int W = decltype(width)::value, R = cache_rows<W>();
+        hipLaunchKernelGGL((cache_write_kernel<decltype(row), decltype(cache), W>), dim3((a.rows + R - 1) / R, a.pool.kv_heads), dim3(256), 0, s, a);
+        return hipGetLastError();
+    });
+}
+hipError_t launch_cache_read(const CacheRows& a, bool bf16_rows, hipStream_t s) {
+    return with_types(a.pool, bf16_rows, [&](auto row, auto cache, auto width) {
+        constexpr int W = decltype(width)::value, R = cache_rows<W>();
+        hipLaunchKernelGGL((cache_read_kernel<decltype(row), decltype(cache), W>), dim3((a.rows + R - 1) / R, a.pool.kv_heads), dim3(256), 0, s, a);
+        return hipGetLastError();
+    });
+}
+
+// ---- decode -------------------------------------------------------------------------------------------
+//
+// A workgroup takes the heads of one group (up to 16) of one sequence over a part of its keys; its four waves take tiles of
+// keys in turn and load them straight into registers in operand order, a tile ahead.  Both products run on the matrix cores: a block
+// of 16 keys times the heads' rows (unused columns are zeros: there is nothing else for them to do, the loads decide), then the values' columns times
+// the scores.  A tile has four groups of g = 16 / element bytes neighbouring keys, one a row of 16 lanes: key g (m / 4) + 4 b + m % 4 of the
+// tile is row m of its block b, so that a lane's scores belong to the g keys whose values it loads as one piece.
+// Products of bf16 operands: bf16 and int8 values are such exactly; f32 rows over int8 are cut into three bf16 parts, p (times the
+// value's scale) into two for bf16 rows and three for f32 rows.  An f32 cache takes the f32 instruction.
+template <int N>
+__device__ __forceinline__ void cut(const float (&x)[8], bf16x8 (&part)[N]) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const uint4 w = make_uint4(pack2(rest[0], rest[1]), pack2(rest[2], rest[3]), pack2(rest[4], rest[5]), pack2(rest[6], rest[7]));
+        part[n] = __builtin_bit_cast(bf16x8, w);
+        float back[8];
+        Vec16<bf16_t>::widen(w, back);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[i] -= back[i];
+    }
+}
+
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
+
+template <typename T, typename C, int W>
+struct Decode {
+    static constexpr int G = 16 / sizeof(C), KT = 4 * G, NB = G / 4;  // keys of a piece, of a tile; blocks of 16 keys
+    static constexpr int KP = W / G / 4;                             // pieces of a key's row that a lane loads
+    static constexpr int VP = W / 16;                                // pieces of values (a column each)
+    static constexpr int QP = sizeof(C) == 4 ? 1 : sizeof(T) == 4 ? 3 : 1, PP = sizeof(T) == 4 ? 3 : 2;
+    struct Keys {
+        uint4 k[NB][KP], v[VP];
+        float ks[sizeof(C) == 1 ? G : 1], vs[sizeof(C) == 1 ? G : 1];
+    };
+};
+
+__device__ __forceinline__ float over_rows_max(float v) {  // over the four rows of 16 lanes
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float over_rows_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+constexpr int kDecodeWaves = 4;
+
+template <typename T, typename C, int W>
+__global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(DecodeCall a) {
+    typedef Decode<T, C, W> X;
+    constexpr int G = X::G, KT = X::KT, NB = X::NB, KP = X::KP, VP = X::VP;
+    __shared__ float joined[kDecodeWaves][16][W + 4];
+    __shared__ float wave_m[kDecodeWaves][16], wave_l[kDecodeWaves][16];
+    const CachePool& p = a.pool;
+    const int group = a.heads / p.kv_heads, blocks = (group + 15) / 16;
+    const int kv = blockIdx.x / blocks, head0 = kv * group + blockIdx.x % blocks * 16, heads = min(16, (kv + 1) * group - head0);
+    const int sequence = blockIdx.z, split = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15;
+    const int length = (int)min((long long)min(max(a.lengths[sequence], 0), a.longest), (long long)a.table_pages << p.page_shift);
+    const int tiles = (length + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
+    const int from = min(split * per, tiles), to = min(from + per, tiles);
+    const int32_t* const table = a.tables + (long long)sequence * a.table_pages;
+    const int page_mask = (1 << p.page_shift) - 1;
+
+    // the heads' rows as B operand: lane l holds head l % 16
+    float q[W / 4];
+    bf16x8 qb[sizeof(C) == 4 ? 1 : W / 32][X::QP];
+    {
+        const T* const row = static_cast<const T*>(a.q) + (long long)sequence * a.q_stride + (long long)(head0 + m16) * p.head_dim;
+        const bool there = m16 < heads;
+        if constexpr (sizeof(C) == 4) {
+#pragma unroll
+            for (int c = 0; c < W / 16; ++c) {
+                const int d = 16 * c + 4 * g;
+                Any16 x = {0, 0, 0, 0};
+                if (there && d < p.head_dim) x = *reinterpret_cast<const Any16*>(row + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[4 * c + i] = __uint_as_float(x[i]);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < W / 32; ++c) {
+                // bf16 keys: piece 4 c + g of 8; int8: half c % 2 of piece 4 (c / 2) + g of 16
+                const int d = sizeof(C) == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
+                float x[8] = {};
+                if (there && d < p.head_dim) load8(row + d, x);
+                cut<X::QP>(x, qb[c]);
+            }
+        }
+    }
+
+    auto entry = [&](int t, int quarter) {  // the page of a tile's quarter; -1: none
+        const int key = t * KT + quarter * G;
+        if (key >= length) return -1;
+        const int e = table[key >> p.page_shift];
+        return e >= 0 && e < p.pages ? e : -1;
+    };
+    // (a lane loads keys of quarter m16 / 4 and values of quarter g)
+    auto load = [&](typename X::Keys& x, int t, int k_page, int v_page) {
+        const unsigned char* const kb = cache_block(p, max(k_page, 0), kv);
+        const unsigned char* const vb = cache_block(p, max(v_page, 0), kv);
+        const int k_row = ((t * KT + (m16 >> 2) * G) & page_mask) + (m16 & 3), v_row = (t * KT + g * G) & page_mask;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int c = 0; c < KP; ++c)
+                x.k[b][c] = *reinterpret_cast<const uint4*>(kb + ((size_t)(k_row + 4 * b) * W + (4 * c + g) * G) * sizeof(C));
+        const unsigned char* const vals = vb + p.half_bytes() + ((size_t)v_row * W + m16 * G) * sizeof(C);
+#pragma unroll
+        for (int c = 0; c < VP; ++c) x.v[c] = *reinterpret_cast<const uint4*>(vals + c * 256);
+        if constexpr (sizeof(C) == 1) {
+            const float* const scales = reinterpret_cast<const float*>(vb + 2 * p.half_bytes()) + v_row;
+#pragma unroll
+            for (int i = 0; i < G / 4; ++i) {
+                const float4 s = *reinterpret_cast<const float4*>(scales + 4 * i), r = *reinterpret_cast<const float4*>(scales + page_mask + 1 + 4 * i);
+                x.ks[4 * i] = s.x; x.ks[4 * i + 1] = s.y; x.ks[4 * i + 2] = s.z; x.ks[4 * i + 3] = s.w;
+                x.vs[4 * i] = r.x; x.vs[4 * i + 1] = r.y; x.vs[4 * i + 2] = r.z; x.vs[4 * i + 3] = r.w;
+            }
+        }
+    };
+
+    const float c = a.scale * 1.44269504088896340736f;
+    floatx4 acc[VP];
+#pragma unroll
+    for (int i = 0; i < VP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+
+    auto compute = [&](typename X::Keys& x, int t, int v_page) {
+        float s[G];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            floatx4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KP; ++k) {
+                if constexpr (sizeof(C) == 4) {
+                    const float y[4] = {__uint_as_float(x.k[b][k].x), __uint_as_float(x.k[b][k].y), __uint_as_float(x.k[b][k].z), __uint_as_float(x.k[b][k].w)};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r = __builtin_amdgcn_mfma_f32_16x16x4f32(y[i], q[4 * k + i], r, 0, 0, 0);
+                } else if constexpr (sizeof(C) == 2) {
+#pragma unroll
+                    for (int n = X::QP - 1; n >= 0; --n)
+                        r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[b][k]), qb[k][n], r, 0, 0, 0);
+                } else {
+                    const bf16x8 lo = widen_i8(make_uint2(x.k[b][k].x, x.k[b][k].y)), hi = widen_i8(make_uint2(x.k[b][k].z, x.k[b][k].w));
+#pragma unroll
+                    for (int n = X::QP - 1; n >= 0; --n) {
+                        r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qb[2 * k][n], r, 0, 0, 0);
+                        r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qb[2 * k + 1][n], r, 0, 0, 0);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * b + i] = r[i] * c;
+        }
+        if constexpr (sizeof(C) == 1) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) s[i] *= x.ks[i];
+        }
+        // keys behind the end and keys without a page: no score, and nothing of what their values' places hold
+        const int left = v_page < 0 ? 0 : length - (t * KT + g * G);
+        const bool ragged = __any(left < G);
+        if (ragged) {
+#pragma unroll
+            for (int i = 0; i < G; ++i) s[i] = i < left ? s[i] : -__builtin_inff();
+            if constexpr (sizeof(C) != 1) {
+                uint4 keep;
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = sizeof(C) == 4 ? (i < left ? ~0u : 0u) : (2 * i < left ? 0xffffu : 0u) | (2 * i + 1 < left ? 0xffff0000u : 0u);
+                keep = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int i = 0; i < VP; ++i) {
+                    x.v[i].x &= keep.x; x.v[i].y &= keep.y; x.v[i].z &= keep.z; x.v[i].w &= keep.w;
+                }
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < G; ++i) top = fmaxf(top, s[i]);
+        if (__any(top > m + 8.0f)) {  // (as in the kernels over whole sequences)
+            const float next = fmaxf(m, over_rows_max(top)), down = next == m ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= down;
+#pragma unroll
+            for (int i = 0; i < VP; ++i) acc[i] *= down;
+        }
+        const float reference = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - reference);
+            l += s[i];
+        }
+        if constexpr (sizeof(C) == 4) {
+#pragma unroll
+            for (int k = 0; k < VP; ++k) {
+                const float y[4] = {__uint_as_float(x.v[k].x), __uint_as_float(x.v[k].y), __uint_as_float(x.v[k].z), __uint_as_float(x.v[k].w)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[i], s[i], acc[k], 0, 0, 0);
+            }
+        } else {
+            bf16x8 part[G / 8][X::PP];
+#pragma unroll
+            for (int h = 0; h < G / 8; ++h) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[i] = s[8 * h + i];
+                    if constexpr (sizeof(C) == 1) y[i] = !ragged || 8 * h + i < left ? y[i] * x.vs[8 * h + i] : 0.0f;
+                }
+                cut<X::PP>(y, part[h]);
+            }
+#pragma unroll
+            for (int k = 0; k < VP; ++k) {
+                if constexpr (sizeof(C) == 2) {
+#pragma unroll
+                    for (int n = X::PP - 1; n >= 0; --n)
+                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.v[k]), part[0][n], acc[k], 0, 0, 0);
+                } else {
+                    const bf16x8 lo = widen_i8(make_uint2(x.v[k].x, x.v[k].y)), hi = widen_i8(make_uint2(x.v[k].z, x.v[k].w));
+#pragma unroll
+                    for (int n = X::PP - 1; n >= 0; --n) {
+                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, part[0][n], acc[k], 0, 0, 0);
+                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, part[1][n], acc[k], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+
+    int t = from + wave;
+    if (t < to) {
+        typename X::Keys now;
+        int k_page = entry(t, m16 >> 2), v_page = entry(t, g);
+        load(now, t, k_page, v_page);
+        int k_next = entry(t + kDecodeWaves, m16 >> 2), v_next = entry(t + kDecodeWaves, g);
+        for (; t < to; t += kDecodeWaves) {
+            typename X::Keys ahead;
+            if (t + kDecodeWaves < to) load(ahead, t + kDecodeWaves, k_next, v_next);
+            const int k_after = entry(t + 2 * kDecodeWaves, m16 >> 2), v_after = entry(t + 2 * kDecodeWaves, g);
+            compute(now, t, v_page);
+            now = ahead;
+            v_page = v_next;
+            k_next = k_after;
+            v_next = v_after;
+        }
+    }
+    l = over_rows_sum(l);
+
+    // the waves' parts
+    if (g == 0) {
+        wave_m[wave][m16] = m;
+        wave_l[wave][m16] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < VP; ++i)
+        *reinterpret_cast<floatx4*>(&joined[wave][m16][16 * i + 4 * g]) = acc[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * W; i += 64 * kDecodeWaves) {
+        const int h = i / W, d = i % W;
+        if (d >= p.head_dim) continue;
+        float top = wave_m[0][h];
+#pragma unroll
+        for (int w = 1; w < kDecodeWaves; ++w) top = fmaxf(top, wave_m[w][h]);
+        float o = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kDecodeWaves; ++w) {
+            const float f = wave_m[w][h] == top ? 1.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
+            o = __builtin_fmaf(f, joined[w][h][d], o);
+            sum = __builtin_fmaf(f, wave_l[w][h], sum);
+        }
+        const long long row = (long long)sequence * a.heads + head0 + h;
+        if (a.splits == 1) {
+            static_cast<T*>(a.out)[row * p.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
+        } else {
+            a.partial[(row * a.splits + split) * W + d] = o;
+            if (d == 0) {
+                a.statistics[(row * a.splits + split) * 2] = top;
+                a.statistics[(row * a.splits + split) * 2 + 1] = sum;
+            }
+        }
+    }
+}
+
+// One wave a row: the parts of its keys, in their order.
+template <typename T, int W>
+__global__ __launch_bounds__(64) void decode_join_kernel(DecodeCall a) {
+    const long long row = blockIdx.x;
+    const int lane = threadIdx.x;
+    const float* const st = a.statistics + row * a.splits * 2;
+    float top = -__builtin_inff();
+    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, st[2 * i]);
+    top = group_fmax(top, 64);
+    float o[W / 64] = {}, sum = 0.0f;
+    for (int i = 0; i < a.splits; ++i) {
+        const float m = st[2 * i], f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+        sum = __builtin_fmaf(f, st[2 * i + 1], sum);
+#pragma unroll
+        for (int j = 0; j < W / 64; ++j) {
+            const int d = lane + 64 * j;
+            if (d < a.pool.head_dim) o[j] = __builtin_fmaf(f, a.partial[(row * a.splits + i) * W + d], o[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < W / 64; ++j) {
+        const int d = lane + 64 * j;
+        if (d < a.pool.head_dim) static_cast<T*>(a.out)[row * a.pool.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o[j] / sum);
+    }
+}
+
+constexpr int kDecodeWorkgroups = 1024, kLeastPart = 512;
+
+int decode_splits(int sequences, int kv_heads, int group, int longest) {
+    const long long rows = (long long)sequences * kv_heads * ((group + 15) / 16);
+    const long long wanted = (kDecodeWorkgroups + rows - 1) / rows;
+    return (int)std::max<long long>(1, std::min<long long>(wanted, (longest + kLeastPart - 1) / kLeastPart));
+}
+size_t decode_partials(int sequences, int kv_heads, int group) {
+    // sequences * heads * ceil(kDecodeWorkgroups / (sequences kv_heads blocks)) is less than both terms together
+    return (size_t)kDecodeWorkgroups * std::min(group, 16) + (size_t)sequences * kv_heads * group;
+}
+
+hipError_t launch_decode_attention(const DecodeCall& a, bool bf16_rows, hipStream_t s) {
+    const int group = a.heads / a.pool.kv_heads;
+    return with_types(a.pool, bf16_rows, [&](auto row, auto cache, auto width) -> hipError_t {
+        typedef decltype(row) T;
+        constexpr int W = decltype(width)::value;
+        hipLaunchKernelGGL((decode_attention_kernel<T, decltype(cache), W>), dim3(a.pool.kv_heads * ((group + 15) / 16), a.splits, a.sequences),
+                           dim3(64 * kDecodeWaves), 0, s, a);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess || a.splits == 1) return e;
+        hipLaunchKernelGGL((decode_join_kernel<T, W>), dim3(a.sequences * a.heads), dim3(64), 0, s, a);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace rbmoe

@@ -1,8 +1,8 @@
 """The part of RustingBrain's ``TransformerLm`` builder surface that selects and
 sizes the sparse layers (reference src/transformer.rs:60-227, :278-447).
 
-Only the mixture-of-experts feed-forward of a block is built here; attention,
-embeddings and the rest of the model are outside this package.  The builder
+The mixture-of-experts feed-forward of a block and the operators of its attention
+are built here; projections, embeddings and the rest of the model are outside this package.  The builder
 keeps the reference's method names — ``.experts(n, k)``, ``.moe_layers(..)``,
 ``.shared_expert(b)``, ``.moe_d_ff(f)``, ``.aux_loss_weight(w)``,
 ``.router_z_loss_weight(w)`` — validates like ``TransformerConfig::validate``
@@ -13,6 +13,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field, replace
 from typing import Dict, Iterable, List, Optional
 
+from .attention import Attention, DecodeAttention, KvCache
 from .moe import (DEFAULT_AUX_LOSS_WEIGHT, DEFAULT_ROUTER_Z_LOSS_WEIGHT, Device, InvalidConfig, MoeConfig,
                   MoeLayer)
 
@@ -134,3 +135,24 @@ class TransformerBuilder:
         tokens = max_tokens if max_tokens is not None else cfg.max_seq_len
         return {i: MoeLayer(cfg.d_model, cfg.moe_config(), device, act_dtype=act_dtype,
                             weight_dtype=weight_dtype, max_tokens=tokens) for i in cfg.moe_layers}
+
+    def build_attention(self, device: Device, *, dtype: str = "f32", backward_rows: int = 0) -> Attention:
+        """Attention over whole sequences with this model's heads; one serves every layer."""
+        self._config.validate()
+        cfg = self._config
+        return Attention(device, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, dtype=dtype, backward_rows=backward_rows)
+
+    def build_caches(self, device: Device, *, sequences: int, dtype: str = "f32", cache_dtype: str = "",
+                     page_rows: int = 16) -> List[KvCache]:
+        """One cache a layer, each with room for ``sequences`` of ``max_seq_len`` rows."""
+        self._config.validate()
+        cfg = self._config
+        pages = sequences * -(-cfg.max_seq_len // page_rows)
+        return [KvCache(device, cfg.n_kv_heads, cfg.head_dim, pages, page_rows=page_rows, dtype=dtype, cache_dtype=cache_dtype)
+                for _ in range(cfg.n_layers)]
+
+    def build_decode_attention(self, device: Device, *, max_sequences: int, dtype: str = "f32") -> DecodeAttention:
+        """A decode step's attention over such caches; one serves every layer."""
+        self._config.validate()
+        cfg = self._config
+        return DecodeAttention(device, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, max_sequences, dtype=dtype)
