@@ -116,7 +116,7 @@ int rbmoe_attention_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int3
     a->head_dim = head_dim;
     a->dtype = dtype;
     a->backward_rows = backward_rows;
-    a->delta_bytes = (size_t)backward_rows * heads * 4;
+    a->delta_bytes = (size_t)backward_rows * heads * 8;
     if (a->delta_bytes)
         if (const int rc = ctx_alloc(ctx, a->delta_bytes, "the backward pass's row sums", &a->delta)) {
             delete a;

@@ -34,7 +34,7 @@ struct AttentionCall {
     void* grad_q;
     void* grad_k;
     void* grad_v;
-    float* delta;  // [heads, query_rows]: written by the queries' gradients, read by the keys'
+    float* delta;  // [2][heads, query_rows], references of the exponents and deltas: written by the queries' gradients, read by the keys'
 };
 hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream_t s);
 hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStream_t s);

@@ -29,7 +29,7 @@ namespace rbmoe {
 
 namespace {
 
-constexpr int kThreads = 256, kOwn = 128;  // a workgroup's threads, and rows or keys that it owns
+constexpr int kThreads = 256, kWaves = 4;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 __device__ uint32_t zero_piece[4];  // what is staged for rows and columns that are not there
@@ -45,6 +45,10 @@ __device__ __forceinline__ uint32_t lds_address(const char* p) {
 // 64 lanes' 16 bytes to consecutive LDS addresses (the same in all lanes) without registers on the way
 __device__ __forceinline__ void issue_dma(uint32_t lds_addr, const void* src) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
+}
+
+__device__ __forceinline__ void issue_dma_word(uint32_t lds_addr, const void* src) {  // and their 4 bytes
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_addr), "v"(src) : "memory");
 }
 
 __device__ __forceinline__ float other_half_max(float v) {
@@ -70,13 +74,13 @@ struct Tile {
     }
     static __device__ __forceinline__ const char* piece(const char* tile, int r, int c) { return tile + r * ROW + ((c ^ swizzle(r)) << 4); }
 
-    // ROWS rows from `first` on of a sequence's n; columns from head_dim on and rows from n on are zeros
-    template <int ROWS, bool A>
+    // ROWS rows from `first` on of a sequence's n, by TEAM waves; columns from head_dim on and rows from n on are zeros
+    template <int ROWS, int TEAM, bool A>
     static __device__ __forceinline__ void stage(char* tile, const T* __restrict__ base, long long stride, int first, int n, int pieces) {
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const int wave = TEAM == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < ROWS * CH / kThreads; ++i) {
-            const int at = (i * (kThreads / 64) + wave) * 64, p = at + lane, r = p / CH, c = (p % CH) ^ swizzle(r);
+        for (int i = 0; i < ROWS * CH / (64 * TEAM); ++i) {
+            const int at = (i * TEAM + wave) * 64, p = at + lane, r = p / CH, c = (p % CH) ^ swizzle(r);
             const bool there = first + r < n && c < pieces;
             const T* const src = base + (long long)(first + r) * stride + c * V;
             if constexpr (A) {
@@ -126,6 +130,11 @@ struct Mma<bf16_t> {
         return sum;
     }
     static __device__ __forceinline__ float rounded(float v) { return bf16_bits_to_f32(f32_to_bf16_bits(v)); }
+    // exp of a score by its factor `c`, less the reference: both times log2 e, for the base-2 exponential
+    static constexpr float unit = kLog2e, natural = kLn2;
+    static __device__ __forceinline__ float exponential(float s, float c, float reference) {
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -reference));
+    }
     // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]
     template <int D>
     static __device__ __forceinline__ void add(floatx16 (&acc)[D / 32], const char* tile, int row0, const Cols& p) {
@@ -159,6 +168,11 @@ struct Mma<float> {
     }
     static __device__ __forceinline__ Cols cols(const floatx16& p) { return p; }
     static __device__ __forceinline__ float rounded(float v) { return v; }
+    // (the factor is the caller's scale as it is, and only the difference is rounded with log2 e)
+    static constexpr float unit = 1.0f, natural = 1.0f;
+    static __device__ __forceinline__ float exponential(float s, float c, float reference) {
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -reference) * kLog2e);
+    }
     template <int D>
     static __device__ __forceinline__ void add(floatx16 (&acc)[D / 32], const char* tile, int row0, const Cols& p) {
         typedef Tile<float, D> T;
@@ -243,21 +257,52 @@ __device__ __forceinline__ void store4(float* p, float a, float b, float c, floa
 __device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
     *reinterpret_cast<Any8*>(p) = Any8{pack2(a, b), pack2(c, d)};
 }
-// acc[d][own] of lane l's own row to `row`, times `factor`
-template <typename T, int D>
-__device__ __forceinline__ void store_own(const floatx16 (&acc)[D / 32], T* row, float factor, int head_dim) {
-    const int h = (threadIdx.x >> 5) & 1;
+// acc[d][own] of lane l's own row to `row`, times `factor`.  TEAM 1: the sum over the workgroup's four waves, in their order, each of which stores a
+// quarter; all threads call, `room` is 4 x D x 128 bytes of LDS that nobody reads any more.
+template <typename T, int D, int TEAM>
+__device__ __forceinline__ void store_own(const floatx16 (&acc)[D / 32], T* row, bool there, float factor, int head_dim, char* room) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (TEAM == 1) {
+        const int wave = threadIdx.x >> 6;
+        float4* const parts = reinterpret_cast<float4*>(room) + lane;
 #pragma unroll
-    for (int b = 0; b < D / 32; ++b)
+        for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int d = 32 * b + 8 * e + 4 * h;
-            if (d >= head_dim) continue;
-            float x[4];
+            for (int e = 0; e < 4; ++e)
+                parts[((wave * (D / 32) + b) * 4 + e) * 64] = make_float4(acc[b][4 * e], acc[b][4 * e + 1], acc[b][4 * e + 2], acc[b][4 * e + 3]);
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = acc[b][4 * e + i] * factor;
-            store4(row + d, x[0], x[1], x[2], x[3]);
+        for (int b = 0; b < D / 32; ++b) {
+            float x[4] = {};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float4 y = parts[((w * (D / 32) + b) * 4 + wave) * 64];
+                x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
+            }
+            const int d = 32 * b + 8 * wave + 4 * h;
+            if (there && d < head_dim) store4(row + d, x[0] * factor, x[1] * factor, x[2] * factor, x[3] * factor);
         }
+        __syncthreads();
+    } else {
+        if (!there) return;
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 32 * b + 8 * e + 4 * h;
+                if (d < head_dim) store4(row + d, acc[b][4 * e] * factor, acc[b][4 * e + 1] * factor, acc[b][4 * e + 2] * factor, acc[b][4 * e + 3] * factor);
+            }
+    }
+}
+// The sum (or maximum) of a lane's value over the four waves; all threads call.
+template <bool MAX>
+__device__ __forceinline__ float over_waves(float v, char* room) {
+    float* const parts = reinterpret_cast<float*>(room);
+    parts[threadIdx.x] = v;
+    __syncthreads();
+    const float x[kWaves] = {parts[threadIdx.x & 63], parts[64 + (threadIdx.x & 63)], parts[128 + (threadIdx.x & 63)], parts[192 + (threadIdx.x & 63)]};
+    __syncthreads();
+    return MAX ? fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) : (x[0] + x[1]) + (x[2] + x[3]);
 }
 
 // ---- sequences -------------------------------------------------------------------------------------
@@ -297,27 +342,43 @@ __device__ __forceinline__ Place place_of(int heads, int sequences, int tiles, b
     return p;
 }
 
-// ---- forward ----------------------------------------------------------------------------------------
-template <typename T>
+// How a workgroup's four waves share the work.  TEAM 4: each owns 32 rows, the tiles are common.  TEAM 1: all own the same 32 rows, each takes every
+// fourth tile, stages it for itself, and their sums are added at the end: four times the workgroups, for calls that have few.
+template <typename T, int TEAM>
 constexpr int tile_rows() {
-    return sizeof(T) == 2 ? 64 : 32;
+    return sizeof(T) == 2 && TEAM == 4 ? 64 : 32;
+}
+// Stages of tiles: the next is loaded while one is used, where four teams' find room in the LDS of 160 KB.
+template <typename T, int D, int TEAM>
+constexpr int tile_stages() {
+    return TEAM == 1 && sizeof(T) * D > 256 ? 1 : 2;
+}
+template <typename T, int D, int TEAM>
+constexpr int tiles_lds(int extra) {  // of two tiles and `extra` bytes a stage
+    return (kWaves / TEAM) * tile_stages<T, D, TEAM>() * (2 * tile_rows<T, TEAM>() * Tile<T, D>::ROW + extra);
+}
+__device__ __forceinline__ void wait_for_tile(bool common) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's part of the tile has landed, its reads of the other stage are done
+    if (common) __syncthreads();                                 // and the other waves'
 }
 
-template <typename T, int D, bool A>
-__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(AttentionCall a) {
+// ---- forward ----------------------------------------------------------------------------------------
+
+template <typename T, int D, int TEAM, bool A>
+__global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attention_forward_kernel(AttentionCall a) {
     typedef Tile<T, D> Tl;
-    constexpr int N = tile_rows<T>(), NB = N / 32, BYTES = N * Tl::ROW;
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, BYTES = N * Tl::ROW, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM>();
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of keys and values
-    const int tiles = (a.longest_queries + kOwn - 1) / kOwn;
+    const int tiles = (a.longest_queries + OWN - 1) / OWN;
     const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
     const Sequence s = sequence_of(a, at.sequence);
-    const int first = at.tile * kOwn;
+    const int first = at.tile * OWN;
     if (first >= s.nq) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
     const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / Tl::V;
     const T* const k = static_cast<const T*>(a.k) + (long long)s.k0 * a.k_stride + (long long)kv * a.head_dim;
     const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
-    const int wave_first = first + 32 * wave, row = wave_first + (lane & 31);
+    const int wave_first = TEAM == 1 ? first : first + 32 * wave, row = wave_first + (lane & 31);
     const bool there = row < s.nq;
     RowsOf<T> q[Tl::KC];
     load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
@@ -325,8 +386,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
     // the keys that a row sees are those below its limit
     auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
-    const int end = limit(min(first + kOwn, s.nq) - 1);
-    const float c = a.scale * kLog2e;
+    const int end = limit(min(first + OWN, s.nq) - 1);
+    constexpr int STEP = TEAM == 1 ? kWaves * N : N;
+    const int start = TEAM == 1 ? wave * N : 0;
+    char* const tiles_at = attention_lds + (TEAM == 1 ? wave * STAGES * 2 * BYTES : 0);
+    const float c = a.scale * Mma<T>::unit;
     floatx16 acc[Tl::DB];
     float m, l;
 
@@ -338,17 +402,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
         m = -__builtin_inff();
         l = 0.0f;
         auto stage = [&](int buf, int t) {
-            char* const to = attention_lds + buf * 2 * BYTES;
-            Tl::template stage<N, A>(to, k, a.k_stride, t, s.nk, pieces);
-            Tl::template stage<N, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
+            char* const to = tiles_at + buf * 2 * BYTES;
+            Tl::template stage<N, TEAM, A>(to, k, a.k_stride, t, s.nk, pieces);
+            Tl::template stage<N, TEAM, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
         };
-        if (end > 0) stage(0, 0);
-        for (int t = 0, buf = 0; t < end; t += N, buf ^= 1) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile has landed
-            __syncthreads();                                  // and the others'; all are done with the other stage
-            if (t + N < end) stage(buf ^ 1, t + N);
+        if (STAGES == 2 && start < end) stage(0, start);
+        for (int t = start, buf = 0; t < end; t += STEP, buf ^= STAGES - 1) {
+            if (STAGES == 1) {
+                wait_for_tile(false);
+                stage(0, t);
+            }
+            wait_for_tile(TEAM == 4);
+            if (STAGES == 2 && t + STEP < end) stage(buf ^ 1, t + STEP);
             if (t >= most || wave_first >= s.nq) continue;
-            const char* const kt = attention_lds + buf * 2 * BYTES;
+            const char* const kt = tiles_at + buf * 2 * BYTES;
             const char* const vt = kt + BYTES;
             floatx16 p[NB];
 #pragma unroll
@@ -369,7 +436,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
             // The reference of the exponents moves only when a score passes it by 2^8: the results are the same, sums and accumulators
             // have room for it, and after a few tiles nothing has to be scaled.
             if (__any(top > m + 8.0f)) {
-                const float next = fmaxf(m, top), down = next == m ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+                const float next = fmaxf(m, top), down = next == m ? 1.0f : Mma<T>::exponential(1.0f, m, next);
                 m = next;
                 l *= down;
 #pragma unroll
@@ -382,7 +449,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[b][i], c, -reference));
+                    p[b][i] = Mma<T>::exponential(p[b][i], c, reference);
                     l += p[b][i];
                 }
             }
@@ -399,30 +466,39 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
     if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
 
     l = other_half_sum(l);
-    if (!there) return;
+    if constexpr (TEAM == 1) {  // to one reference
+        __syncthreads();
+        const float all = over_waves<true>(m, attention_lds), down = m == all ? 1.0f : Mma<T>::exponential(1.0f, m, all);
+        m = all;
+        l = over_waves<false>(l * down, attention_lds);
+#pragma unroll
+        for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][i] *= down;
+    }
     const long long to = (long long)(s.q0 + row) * a.heads + at.head;
-    store_own<T, D>(acc, static_cast<T*>(a.out) + to * a.head_dim, l == 0.0f ? 0.0f : 1.0f / l, a.head_dim);
-    if (a.lse && h == 0)
+    store_own<T, D, TEAM>(acc, static_cast<T*>(a.out) + to * a.head_dim, there, l == 0.0f ? 0.0f : 1.0f / l, a.head_dim, attention_lds);
+    if (there && a.lse && h == 0 && (TEAM == 4 || wave == 0))
         a.lse[(long long)at.head * a.query_rows + s.q0 + row] =
-            l == 0.0f ? -__builtin_inff() : ((m == -__builtin_inff() ? 0.0f : m) + __builtin_amdgcn_logf(l)) * kLn2;
+            l == 0.0f ? -__builtin_inff() : (m == -__builtin_inff() ? 0.0f : m * Mma<T>::natural) + __builtin_amdgcn_logf(l) * kLn2;
 }
 
 // ---- backward: gradients of the queries ------------------------------------------------------------------
-template <typename T, int D, bool A>
+template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_kernel(AttentionCall a) {
     typedef Tile<T, D> Tl;
-    constexpr int N = tile_rows<T>(), NB = N / 32, BYTES = N * Tl::ROW;
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, BYTES = N * Tl::ROW, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM>();
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    const int tiles = (a.longest_queries + kOwn - 1) / kOwn;
+    const int tiles = (a.longest_queries + OWN - 1) / OWN;
     const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
     const Sequence s = sequence_of(a, at.sequence);
-    const int first = at.tile * kOwn;
+    const int first = at.tile * OWN;
     if (first >= s.nq) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
     const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / Tl::V;
     const T* const k = static_cast<const T*>(a.k) + (long long)s.k0 * a.k_stride + (long long)kv * a.head_dim;
     const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
-    const int wave_first = first + 32 * wave, row = wave_first + (lane & 31);
+    const int wave_first = TEAM == 1 ? first : first + 32 * wave, row = wave_first + (lane & 31);
     const bool there = row < s.nq;
     const long long in_out = ((long long)(s.q0 + row) * a.heads + at.head) * a.head_dim, in_lse = (long long)at.head * a.query_rows + s.q0 + row;
     RowsOf<T> q[Tl::KC], dout[Tl::KC];
@@ -442,12 +518,15 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
         for (int i = 0; i < Tl::V; ++i) delta = __builtin_fmaf(x[i], y[i], delta);
     }
     delta = other_half_sum(delta);
-    const float lse2 = there ? a.lse[in_lse] * kLog2e : 0.0f;
+    const float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
 
     auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
-    const int end = limit(min(first + kOwn, s.nq) - 1);
-    const float c = a.scale * kLog2e;
+    const int end = limit(min(first + OWN, s.nq) - 1);
+    constexpr int STEP = TEAM == 1 ? kWaves * N : N;
+    const int start = TEAM == 1 ? wave * N : 0;
+    char* const tiles_at = attention_lds + (TEAM == 1 ? wave * STAGES * 2 * BYTES : 0);
+    const float c = a.scale * Mma<T>::unit;
     // For bf16 rows delta comes from rounded rows of `out`, and ds is rounded.  Both errors make a row's ds add up to something
     // else than its true sum of zero, and where keys share a direction that goes along it.  So the sum of the rounded ds is taken
     // off again in proportion to p (grad_q -= sum * mean key), and delta handed on as what makes the sum of the unrounded ones zero.
@@ -462,24 +541,27 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
             for (int i = 0; i < 16; ++i) acc[b][i] = mean[mend ? b : 0][i] = 0.0f;
         sum = rounded_sum = 0.0f;
         auto stage = [&](int buf, int t) {
-            char* const to = attention_lds + buf * 2 * BYTES;
-            Tl::template stage<N, A>(to, k, a.k_stride, t, s.nk, pieces);
-            Tl::template stage<N, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
+            char* const to = tiles_at + buf * 2 * BYTES;
+            Tl::template stage<N, TEAM, A>(to, k, a.k_stride, t, s.nk, pieces);
+            Tl::template stage<N, TEAM, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
         };
-        if (end > 0) stage(0, 0);
-        for (int t = 0, buf = 0; t < end; t += N, buf ^= 1) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (t + N < end) stage(buf ^ 1, t + N);
+        if (STAGES == 2 && start < end) stage(0, start);
+        for (int t = start, buf = 0; t < end; t += STEP, buf ^= STAGES - 1) {
+            if (STAGES == 1) {
+                wait_for_tile(false);
+                stage(0, t);
+            }
+            wait_for_tile(TEAM == 4);
+            if (STAGES == 2 && t + STEP < end) stage(buf ^ 1, t + STEP);
             if (t >= most || wave_first >= s.nq) continue;
-            const char* const kt = attention_lds + buf * 2 * BYTES;
+            const char* const kt = tiles_at + buf * 2 * BYTES;
             const char* const vt = kt + BYTES;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 floatx16 p = product<T, D>(kt, 32 * b, q), dp = product<T, D>(vt, 32 * b, dout);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], c, -lse2));
+                    p[i] = Mma<T>::exponential(p[i], c, reference);
                     dp[i] = p[i] * (dp[i] - delta);
                 }
                 if (t + N > least) {
@@ -506,33 +588,42 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
     };
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
+    if constexpr (TEAM == 1) __syncthreads();
     if constexpr (mend) {
         rounded_sum = other_half_sum(rounded_sum);
-        delta += other_half_sum(sum);
+        sum = other_half_sum(sum);
+        if constexpr (TEAM == 1) {
+            rounded_sum = over_waves<false>(rounded_sum, attention_lds);
+            sum = over_waves<false>(sum, attention_lds);
+        }
+        delta += sum;
 #pragma unroll
         for (int b = 0; b < Tl::DB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_fmaf(-rounded_sum, mean[b][i], acc[b][i]);
     }
-    if (there && h == 0) a.delta[in_lse] = delta;
-    if (there)
-        store_own<T, D>(acc, static_cast<T*>(a.grad_q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, a.scale, a.head_dim);
+    if (there && h == 0 && (TEAM == 4 || wave == 0)) {
+        a.delta[in_lse] = reference;
+        a.delta[(long long)a.heads * a.query_rows + in_lse] = delta;
+    }
+    store_own<T, D, TEAM>(acc, static_cast<T*>(a.grad_q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, a.scale,
+                          a.head_dim, attention_lds);
 }
 
 // ---- backward: gradients of keys and values -------------------------------------------------------------
-template <typename T, int D, bool A>
+template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_kv_kernel(AttentionCall a) {
     typedef Tile<T, D> Tl;
-    constexpr int N = tile_rows<T>(), NB = N / 32, BYTES = N * Tl::ROW, STAGE = 2 * BYTES + 2 * N * 4;
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, BYTES = N * Tl::ROW, STAGE = 2 * BYTES + 2 * N * 4, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM>();
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
-    const int tiles = (a.longest_keys + kOwn - 1) / kOwn;
+    const int tiles = (a.longest_keys + OWN - 1) / OWN;
     const Place at = place_of(a.kv_heads, a.sequences, tiles, false);
     const Sequence s = sequence_of(a, at.sequence);
-    const int first = at.tile * kOwn, kv = at.head, group = a.heads / a.kv_heads;
+    const int first = at.tile * OWN, kv = at.head, group = a.heads / a.kv_heads;
     if (first >= s.nk) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int pieces = a.head_dim / Tl::V;
-    const int wave_first = first + 32 * wave, key = wave_first + (lane & 31);
+    const int wave_first = TEAM == 1 ? first : first + 32 * wave, key = wave_first + (lane & 31);
     const bool there = key < s.nk;
     RowsOf<T> k[Tl::KC], v[Tl::KC];
     load_own<T, D>(static_cast<const T*>(a.k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there, pieces, k);
@@ -542,7 +633,10 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     auto start = [&](int j) { return a.causal ? max(j - (s.nk - s.nq), 0) : 0; };
     const int own_start = start(key), least = start(wave_first), most = start(wave_first + 31);
     const int begin = start(first) / N * N, turns = begin < s.nq ? (s.nq - begin + N - 1) / N : 0, all = turns * group;
-    const float c = a.scale * kLog2e;
+    constexpr int STEP = TEAM == 1 ? kWaves : 1;
+    const int mine = TEAM == 1 ? wave : 0;
+    char* const tiles_at = attention_lds + (TEAM == 1 ? wave * STAGES * STAGE : 0);
+    const float c = a.scale * Mma<T>::unit;
     floatx16 dk[Tl::DB], dv[Tl::DB];
 
     auto pass = [&](auto careful) {
@@ -553,28 +647,29 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
         // turn i: head i / turns of the group, rows from begin + N (i % turns) on
         auto stage = [&](int buf, int i) {
             const int head = kv * group + i / turns, t = begin + i % turns * N;
-            char* const to = attention_lds + buf * STAGE;
-            if (threadIdx.x < 2 * N) {
-                const int r = threadIdx.x % N;
-                const float* const from = threadIdx.x < N ? a.lse : a.delta;
-                float x = 0.0f;
-                if (t + r < s.nq) x = from[(long long)head * a.query_rows + s.q0 + t + r];
-                *reinterpret_cast<float*>(to + 2 * BYTES + threadIdx.x * 4) = threadIdx.x < N ? x * kLog2e : x;
+            char* const to = tiles_at + buf * STAGE;
+            if (TEAM == 1 || wave < 2 * N / 64) {  // references, then deltas
+                const int i = TEAM == 1 ? lane : threadIdx.x, r = t + i % N;
+                const float* const from = a.delta + (i < N ? 0 : (long long)a.heads * a.query_rows) + (long long)head * a.query_rows + s.q0 + r;
+                issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), r < s.nq ? (const void*)from : (const void*)zero_piece);
             }
-            Tl::template stage<N, A>(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
-            Tl::template stage<N, A>(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
+            Tl::template stage<N, TEAM, A>(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
+            Tl::template stage<N, TEAM, A>(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
                                      (long long)a.heads * a.head_dim, t, s.nq, pieces);
         };
-        if (all > 0) stage(0, 0);
-        for (int i = 0, buf = 0; i < all; ++i, buf ^= 1) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (i + 1 < all) stage(buf ^ 1, i + 1);
+        if (STAGES == 2 && mine < all) stage(0, mine);
+        for (int i = mine, buf = 0; i < all; i += STEP, buf ^= STAGES - 1) {
+            if (STAGES == 1) {
+                wait_for_tile(false);
+                stage(0, i);
+            }
+            wait_for_tile(TEAM == 4);
+            if (STAGES == 2 && i + STEP < all) stage(buf ^ 1, i + STEP);
             const int t = begin + i % turns * N;
             if (t + N <= least || wave_first >= s.nk) continue;
-            const char* const qt = attention_lds + buf * STAGE;
+            const char* const qt = tiles_at + buf * STAGE;
             const char* const ot = qt + BYTES;
-            const float* const lse2 = reinterpret_cast<const float*>(ot + BYTES);
+            const float* const references = reinterpret_cast<const float*>(ot + BYTES);
             const bool masked = t < most || t + N > s.nq;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -582,11 +677,11 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 32 * b + block_row(4 * e);
-                    const float4 x = *reinterpret_cast<const float4*>(lse2 + r), y = *reinterpret_cast<const float4*>(lse2 + N + r);
+                    const float4 x = *reinterpret_cast<const float4*>(references + r), y = *reinterpret_cast<const float4*>(references + N + r);
                     const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        p[4 * e + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[4 * e + j], c, -xs[j]));
+                        p[4 * e + j] = Mma<T>::exponential(p[4 * e + j], c, xs[j]);
                         dp[4 * e + j] = p[4 * e + j] * (dp[4 * e + j] - ys[j]);
                     }
                 }
@@ -608,27 +703,38 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     };
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(dk) || any_not_finite(dv))) pass(std::true_type{});
-    if (there) {
-        store_own<T, D>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, a.scale, a.head_dim);
-        store_own<T, D>(dv, static_cast<T*>(a.grad_v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, 1.0f, a.head_dim);
-    }
+    if constexpr (TEAM == 1) __syncthreads();
+    store_own<T, D, TEAM>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there, a.scale, a.head_dim,
+                          attention_lds);
+    store_own<T, D, TEAM>(dv, static_cast<T*>(a.grad_v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, 1.0f, a.head_dim,
+                          attention_lds);
 }
 
 bool whole_pieces(const void* p, long long stride, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
 }
 
-// f(element type, padded head width, rows start on 16-byte boundaries)
+// f(element type, padded head width, waves a team, rows start on 16-byte boundaries)
 template <typename F>
-hipError_t with_kernel(bool bf16, int head_dim, bool aligned, F f) {
-    auto wide = [&](auto type) -> hipError_t {
-        typedef decltype(type) T;
-        if (head_dim <= 64)
-            return aligned ? f(T{}, std::integral_constant<int, 64>{}, std::true_type{}) : f(T{}, std::integral_constant<int, 64>{}, std::false_type{});
-        return aligned ? f(T{}, std::integral_constant<int, 128>{}, std::true_type{}) : f(T{}, std::integral_constant<int, 128>{}, std::false_type{});
+hipError_t with_kernel(bool bf16, int head_dim, bool few, bool aligned, F f) {
+    auto rows = [&](auto type, auto width, auto team) -> hipError_t {
+        return aligned ? f(type, width, team, std::true_type{}) : f(type, width, team, std::false_type{});
     };
-    return bf16 ? wide(bf16_t{}) : wide(float{});
+    auto team = [&](auto type, auto width) -> hipError_t {
+        return few ? rows(type, width, std::integral_constant<int, 1>{}) : rows(type, width, std::integral_constant<int, 4>{});
+    };
+    auto width = [&](auto type) -> hipError_t {
+        return head_dim <= 64 ? team(type, std::integral_constant<int, 64>{}) : team(type, std::integral_constant<int, 128>{});
+    };
+    return bf16 ? width(bf16_t{}) : width(float{});
 }
+
+#ifndef RBMOE_ATTENTION_FEW
+#define RBMOE_ATTENTION_FEW 512
+#endif
+constexpr int kFew = RBMOE_ATTENTION_FEW;
+// Whether a launch over `longest` rows of `heads` heads a sequence would have few workgroups of 128 rows.
+bool few_workgroups(const AttentionCall& a, int longest, int heads) { return (long long)((longest + 127) / 128) * heads * a.sequences < kFew; }
 
 template <typename K>
 hipError_t launch(K kernel, std::atomic<unsigned long long>& once, const AttentionCall& a, int tiles, int heads, int lds, hipStream_t s) {
@@ -645,12 +751,12 @@ hipError_t launch(K kernel, std::atomic<unsigned long long>& once, const Attenti
 hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream_t s) {
     const int size = bf16 ? 2 : 4;
     const bool aligned = whole_pieces(a.k, a.k_stride, size) && whole_pieces(a.v, a.v_stride, size);
-    return with_kernel(bf16, a.head_dim, aligned, [&](auto type, auto width, auto whole) {
+    return with_kernel(bf16, a.head_dim, few_workgroups(a, a.longest_queries, a.heads), aligned, [&](auto type, auto width, auto team, auto whole) {
         typedef decltype(type) T;
-        constexpr int D = decltype(width)::value;
+        constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
-        return launch(attention_forward_kernel<T, D, decltype(whole)::value>, once, a, (a.longest_queries + kOwn - 1) / kOwn, a.heads,
-                      4 * tile_rows<T>() * Tile<T, D>::ROW, s);
+        return launch(attention_forward_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
+                      tiles_lds<T, D, TEAM>(0), s);
     });
 }
 
@@ -659,22 +765,22 @@ hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStrea
     hipError_t e = hipSuccess;
     if (a.longest_queries > 0) {
         const bool aligned = whole_pieces(a.k, a.k_stride, size) && whole_pieces(a.v, a.v_stride, size);
-        e = with_kernel(bf16, a.head_dim, aligned, [&](auto type, auto width, auto whole) {
+        e = with_kernel(bf16, a.head_dim, few_workgroups(a, a.longest_queries, a.heads), aligned, [&](auto type, auto width, auto team, auto whole) {
             typedef decltype(type) T;
-            constexpr int D = decltype(width)::value;
+            constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
             static std::atomic<unsigned long long> once{0};
-            return launch(attention_grad_q_kernel<T, D, decltype(whole)::value>, once, a, (a.longest_queries + kOwn - 1) / kOwn, a.heads,
-                          4 * tile_rows<T>() * Tile<T, D>::ROW, s);
+            return launch(attention_grad_q_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
+                          tiles_lds<T, D, TEAM>(0), s);
         });
     }
     if (e != hipSuccess || a.longest_keys == 0) return e;
     const bool aligned = whole_pieces(a.q, a.q_stride, size) && whole_pieces(a.grad_out, a.head_dim, size);
-    return with_kernel(bf16, a.head_dim, aligned, [&](auto type, auto width, auto whole) {
+    return with_kernel(bf16, a.head_dim, few_workgroups(a, a.longest_keys, a.kv_heads), aligned, [&](auto type, auto width, auto team, auto whole) {
         typedef decltype(type) T;
-        constexpr int D = decltype(width)::value;
+        constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
-        return launch(attention_grad_kv_kernel<T, D, decltype(whole)::value>, once, a, (a.longest_keys + kOwn - 1) / kOwn, a.kv_heads,
-                      4 * tile_rows<T>() * Tile<T, D>::ROW + 4 * tile_rows<T>() * 4, s);
+        return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_keys + OWN - 1) / OWN, a.kv_heads,
+                      tiles_lds<T, D, TEAM>(8 * tile_rows<T, TEAM>()), s);
     });
 }
 
