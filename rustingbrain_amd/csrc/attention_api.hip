@@ -341,7 +341,9 @@ int rbmoe_decode_attention(rbmoe_decode* d, rbmoe_kv_cache* c, int32_t sequences
     a.heads = d->heads;
     a.table_pages = table_pages;
     a.longest = longest;
-    a.splits = decode_splits(sequences, d->kv_heads, d->heads / d->kv_heads, longest);
+    const DecodePlan plan = decode_plan(sequences, d->kv_heads, d->heads / d->kv_heads, longest);
+    a.ranges = plan.ranges;
+    a.many = plan.many;
     a.scale = scale;
     a.partial = static_cast<float*>(d->workspace);
     a.statistics = a.partial + d->partials * (d->head_dim <= 64 ? 64 : 128);
@@ -349,9 +351,9 @@ int rbmoe_decode_attention(rbmoe_decode* d, rbmoe_kv_cache* c, int32_t sequences
     return RBMOE_OK;
 }
 
-// How many parts a call cuts its sequences into: for tests (no GPU needed).
-int rbmoe_internal_decode_splits(int32_t sequences, int32_t kv_heads, int32_t group, int32_t longest) {
-    return decode_splits(sequences, kv_heads, group, longest);
+// Into how many ranges a call cuts its sequences: for tests (no GPU needed).
+int rbmoe_internal_decode_ranges(int32_t sequences, int32_t kv_heads, int32_t group, int32_t longest) {
+    return decode_plan(sequences, kv_heads, group, longest).ranges;
 }
 
 }  // extern "C"

@@ -43,13 +43,20 @@ struct DecodeCall {
     long long q_stride;
     const int32_t* tables;  // [sequences][table_stride]
     const int32_t* lengths;
-    int sequences, heads, table_pages, longest, splits;
+    int sequences, heads, table_pages, longest;
+    int ranges;  // decode_plan's
+    bool many;
     float scale;
-    float* partial;     // [sequences, heads, splits][width]
-    float* statistics;  // [sequences, heads, splits][2]: reference of the exponents, sum
+    float* partial;     // [ranges + sequences][heads][width]: part range + sequence
+    float* statistics;  // [ranges + sequences][heads][2]: reference of the exponents, sum
 };
-int decode_splits(int sequences, int kv_heads, int group, int longest);
-size_t decode_partials(int sequences, int kv_heads, int group);  // the most that decode_splits leads to for up to so many sequences
+// ranges > 0: the tiles of all sequences in so many equal ranges; 0: a workgroup a sequence, `many`: of many waves.
+struct DecodePlan {
+    int ranges;
+    bool many;
+};
+DecodePlan decode_plan(int sequences, int kv_heads, int group, int longest);
+size_t decode_partials(int sequences, int kv_heads, int group);  // parts of heads at most, for up to so many sequences
 hipError_t launch_decode_attention(const DecodeCall& a, bool bf16_rows, hipStream_t s);
 
 }  // namespace rbmoe

@@ -55,6 +55,12 @@ __device__ __forceinline__ void store8(int8_t* p, const float (&v)[8]) {
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
+template <typename C>
+__device__ __forceinline__ C stored_as(float v) {
+    if constexpr (sizeof(C) == 1) return (int8_t)(int)v;
+    else return from_f32<C>(v);
+}
+
 // The 8 values of each of a row's TR threads, rounded to whole numbers of the returned scale.
 template <int TR>
 __device__ __forceinline__ float quantize(float (&v)[8]) {
@@ -111,9 +117,11 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
     }
     __syncthreads();
     const int page_mask = (1 << p.page_shift) - 1, c = tid % TR * 8;
+    const bool scattered = neighbours == 0;  // (new rows of many sequences: the way through LDS would gain nothing)
 #pragma unroll
     for (int i = 0; i < R * TR / 256; ++i) {
         const int r = i * (256 / TR) + tid / TR;
+        if (first + r >= a.rows) break;
         const long long at = places[r];
         float k[8] = {}, v[8] = {};
         if (at >= 0 && c < p.head_dim) {
@@ -131,8 +139,15 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
             }
         }
         if (at >= 0) store8(reinterpret_cast<C*>(block) + (size_t)row * W + c, k);
-        store8(&values[r][c], v);
+        if (!scattered) {
+            store8(&values[r][c], v);
+        } else if (at >= 0) {
+            C* const to = reinterpret_cast<C*>(block + p.half_bytes()) + value_at<W, G>(row, c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[j * G] = stored_as<C>(v[j]);
+        }
     }
+    if (scattered) return;
     __syncthreads();
     // column d of 16 rows
     const int d = tid % W, end = tid / W * 16 + 16;
@@ -327,8 +342,12 @@ struct Decode {
     static constexpr int VP = W / 16;                                // pieces of values (a column each)
     static constexpr int QP = sizeof(C) == 4 ? 1 : sizeof(T) == 4 ? 3 : 1, PP = sizeof(T) == 4 ? 3 : 2;
     struct Keys {
-        uint4 k[NB][KP], v[VP];
-        float ks[sizeof(C) == 1 ? G : 1], vs[sizeof(C) == 1 ? G : 1];
+        uint4 k[NB][KP];
+        float4 scale[sizeof(C) == 1 ? G / 4 : 1];
+    };
+    struct Values {
+        uint4 v[VP];
+        float4 scale[sizeof(C) == 1 ? G / 4 : 1];
     };
 };
 
@@ -341,24 +360,48 @@ __device__ __forceinline__ float over_rows_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-constexpr int kDecodeWaves = 4;
+#ifndef RBMOE_DECODE_OCC
+#define RBMOE_DECODE_OCC 2
+#endif
+// Waves of a workgroup: 4, or as many as registers allow where a call is so small that one workgroup a group of heads takes all of its keys (no
+// parts, no second launch).
+template <typename C, int W>
+constexpr int many_waves() {
+    return W == 64 && sizeof(C) != 1 ? 16 : 8;
+}
+//
+// STREAM: the tiles of all sequences, one behind the other, are cut into as many equal ranges as there are workgroups for a group of heads, whatever
+// the sequences' lengths are.  A workgroup works off the sequences of its range; it writes rows of those that lie within it, and parts of those that
+// pass its ends (number: its own plus the sequence's), which a second launch joins.  Otherwise a workgroup takes one sequence whole.
+template <typename C>
+constexpr int tile_keys() {
+    return 64 / sizeof(C);
+}
+constexpr int kMostStreamed = 1024;  // sequences: their prefix sums lie in LDS
+__device__ __forceinline__ int sequence_length(const DecodeCall& a, int i) {
+    return (int)min((long long)min(max(a.lengths[i], 0), a.longest), (long long)a.table_pages << a.pool.page_shift);
+}
+__device__ __forceinline__ int sequence_tiles(const DecodeCall& a, int i, int keys) {  // (a sequence without keys has one: zeros are written for it)
+    return max(1, (sequence_length(a, i) + keys - 1) / keys);
+}
+__device__ __forceinline__ long long range_start(long long tiles, int i, int n) { return tiles * i / n; }
 
-template <typename T, typename C, int W>
-__global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(DecodeCall a) {
+template <typename T, typename C, int W, int NW, bool STREAM>
+__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : RBMOE_DECODE_OCC) void decode_attention_kernel(DecodeCall a) {
     typedef Decode<T, C, W> X;
     constexpr int G = X::G, KT = X::KT, NB = X::NB, KP = X::KP, VP = X::VP;
-    __shared__ float joined[kDecodeWaves][16][W + 4];
-    __shared__ float wave_m[kDecodeWaves][16], wave_l[kDecodeWaves][16];
+    __shared__ float joined[NW][16][W + 4];
+    __shared__ float wave_m[NW][16], wave_l[NW][16];
     const CachePool& p = a.pool;
     const int group = a.heads / p.kv_heads, blocks = (group + 15) / 16;
     const int kv = blockIdx.x / blocks, head0 = kv * group + blockIdx.x % blocks * 16, heads = min(16, (kv + 1) * group - head0);
-    const int sequence = blockIdx.z, split = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, m16 = lane & 15;
-    const int length = (int)min((long long)min(max(a.lengths[sequence], 0), a.longest), (long long)a.table_pages << p.page_shift);
-    const int tiles = (length + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
-    const int from = min(split * per, tiles), to = min(from + per, tiles);
-    const int32_t* const table = a.tables + (long long)sequence * a.table_pages;
     const int page_mask = (1 << p.page_shift) - 1;
+
+    // the tiles `from` to `to` of a sequence; `part`: where they go if they are not all of it, or -1
+    auto work = [&](const int sequence, const int from, const int to, const long long part) {
+    const int length = sequence_length(a, sequence);
+    const int32_t* const table = a.tables + (long long)sequence * a.table_pages;
 
     // the heads' rows as B operand: lane l holds head l % 16
     float q[W / 4];
@@ -394,26 +437,30 @@ __global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(
         return e >= 0 && e < p.pages ? e : -1;
     };
     // (a lane loads keys of quarter m16 / 4 and values of quarter g)
-    auto load = [&](typename X::Keys& x, int t, int k_page, int v_page) {
-        const unsigned char* const kb = cache_block(p, max(k_page, 0), kv);
-        const unsigned char* const vb = cache_block(p, max(v_page, 0), kv);
-        const int k_row = ((t * KT + (m16 >> 2) * G) & page_mask) + (m16 & 3), v_row = (t * KT + g * G) & page_mask;
+    auto load_keys = [&](typename X::Keys& x, int t, int page, int scale_page) {
+        const unsigned char* const block = cache_block(p, max(page, 0), kv);
+        const int row = ((t * KT + (m16 >> 2) * G) & page_mask) + (m16 & 3);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int c = 0; c < KP; ++c)
-                x.k[b][c] = *reinterpret_cast<const uint4*>(kb + ((size_t)(k_row + 4 * b) * W + (4 * c + g) * G) * sizeof(C));
-        const unsigned char* const vals = vb + p.half_bytes() + ((size_t)v_row * W + m16 * G) * sizeof(C);
-#pragma unroll
-        for (int c = 0; c < VP; ++c) x.v[c] = *reinterpret_cast<const uint4*>(vals + c * 256);
+                x.k[b][c] = *reinterpret_cast<const uint4*>(block + ((size_t)(row + 4 * b) * W + (4 * c + g) * G) * sizeof(C));
         if constexpr (sizeof(C) == 1) {
-            const float* const scales = reinterpret_cast<const float*>(vb + 2 * p.half_bytes()) + v_row;
+            const float* const scales = reinterpret_cast<const float*>(cache_block(p, max(scale_page, 0), kv) + 2 * p.half_bytes()) + ((t * KT + g * G) & page_mask);
 #pragma unroll
-            for (int i = 0; i < G / 4; ++i) {
-                const float4 s = *reinterpret_cast<const float4*>(scales + 4 * i), r = *reinterpret_cast<const float4*>(scales + page_mask + 1 + 4 * i);
-                x.ks[4 * i] = s.x; x.ks[4 * i + 1] = s.y; x.ks[4 * i + 2] = s.z; x.ks[4 * i + 3] = s.w;
-                x.vs[4 * i] = r.x; x.vs[4 * i + 1] = r.y; x.vs[4 * i + 2] = r.z; x.vs[4 * i + 3] = r.w;
-            }
+            for (int i = 0; i < G / 4; ++i) x.scale[i] = *reinterpret_cast<const float4*>(scales + 4 * i);
+        }
+    };
+    auto load_values = [&](typename X::Values& x, int t, int page) {
+        const unsigned char* const block = cache_block(p, max(page, 0), kv);
+        const int row = (t * KT + g * G) & page_mask;
+        const unsigned char* const values = block + p.half_bytes() + ((size_t)row * W + m16 * G) * sizeof(C);
+#pragma unroll
+        for (int c = 0; c < VP; ++c) x.v[c] = *reinterpret_cast<const uint4*>(values + c * 256);
+        if constexpr (sizeof(C) == 1) {
+            const float* const scales = reinterpret_cast<const float*>(block + 2 * p.half_bytes()) + page_mask + 1 + row;
+#pragma unroll
+            for (int i = 0; i < G / 4; ++i) x.scale[i] = *reinterpret_cast<const float4*>(scales + 4 * i);
         }
     };
 
@@ -423,8 +470,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(
     for (int i = 0; i < VP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -__builtin_inff(), l = 0.0f;
 
-    auto compute = [&](typename X::Keys& x, int t, int v_page) {
-        float s[G];
+    auto score = [&](const typename X::Keys& x, float (&s)[G]) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             floatx4 r = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -452,8 +498,12 @@ __global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(
         }
         if constexpr (sizeof(C) == 1) {
 #pragma unroll
-            for (int i = 0; i < G; ++i) s[i] *= x.ks[i];
+            for (int i = 0; i < G / 4; ++i) {
+                s[4 * i] *= x.scale[i].x; s[4 * i + 1] *= x.scale[i].y; s[4 * i + 2] *= x.scale[i].z; s[4 * i + 3] *= x.scale[i].w;
+            }
         }
+    };
+    auto add = [&](float (&s)[G], typename X::Values& x, int t, int v_page) {
         // keys behind the end and keys without a page: no score, and nothing of what their values' places hold
         const int left = v_page < 0 ? 0 : length - (t * KT + g * G);
         const bool ragged = __any(left < G);
@@ -504,7 +554,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     y[i] = s[8 * h + i];
-                    if constexpr (sizeof(C) == 1) y[i] = !ragged || 8 * h + i < left ? y[i] * x.vs[8 * h + i] : 0.0f;
+                    if constexpr (sizeof(C) == 1) {
+                        const float4 f = x.scale[2 * h + i / 4];
+                        y[i] = !ragged || 8 * h + i < left ? y[i] * (i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w) : 0.0f;
+                    }
                 }
                 cut<X::PP>(y, part[h]);
             }
@@ -526,21 +579,31 @@ __global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(
         }
     };
 
+    // A tile's values are under way while its scores are made, the next tile's keys while its values are added; page numbers come a tile
+    // earlier.  (Behind the last tile that one is loaded again: no load depends on a branch, so that each is waited for alone.)
     int t = from + wave;
     if (t < to) {
-        typename X::Keys now;
-        int k_page = entry(t, m16 >> 2), v_page = entry(t, g);
-        load(now, t, k_page, v_page);
-        int k_next = entry(t + kDecodeWaves, m16 >> 2), v_next = entry(t + kDecodeWaves, g);
-        for (; t < to; t += kDecodeWaves) {
-            typename X::Keys ahead;
-            if (t + kDecodeWaves < to) load(ahead, t + kDecodeWaves, k_next, v_next);
-            const int k_after = entry(t + 2 * kDecodeWaves, m16 >> 2), v_after = entry(t + 2 * kDecodeWaves, g);
-            compute(now, t, v_page);
-            now = ahead;
+        typename X::Keys keys;
+        typename X::Values values;
+        int v_page = entry(t, g);
+        load_keys(keys, t, entry(t, m16 >> 2), v_page);
+        int next = min(t + NW, to - 1);
+        int k_next = entry(next, m16 >> 2), v_next = entry(next, g);
+        for (; t < to; t += NW) {
+            load_values(values, t, v_page);
+            const int after = min(t + 2 * NW, to - 1);
+            const int k_after = entry(after, m16 >> 2), v_after = entry(after, g);
+            __builtin_amdgcn_sched_barrier(0);
+            float s[G];
+            score(keys, s);
+            __builtin_amdgcn_sched_barrier(0);
+            load_keys(keys, next, k_next, v_next);
+            __builtin_amdgcn_sched_barrier(0);
+            add(s, values, t, v_page);
             v_page = v_next;
             k_next = k_after;
             v_next = v_after;
+            next = after;
         }
     }
     l = over_rows_sum(l);
@@ -554,80 +617,178 @@ __global__ __launch_bounds__(64 * kDecodeWaves, 2) void decode_attention_kernel(
     for (int i = 0; i < VP; ++i)
         *reinterpret_cast<floatx4*>(&joined[wave][m16][16 * i + 4 * g]) = acc[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * W; i += 64 * kDecodeWaves) {
+    for (int i = threadIdx.x; i < heads * W; i += 64 * NW) {
         const int h = i / W, d = i % W;
         if (d >= p.head_dim) continue;
         float top = wave_m[0][h];
 #pragma unroll
-        for (int w = 1; w < kDecodeWaves; ++w) top = fmaxf(top, wave_m[w][h]);
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, wave_m[w][h]);
         float o = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kDecodeWaves; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = wave_m[w][h] == top ? 1.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
             o = __builtin_fmaf(f, joined[w][h][d], o);
             sum = __builtin_fmaf(f, wave_l[w][h], sum);
         }
-        const long long row = (long long)sequence * a.heads + head0 + h;
-        if (a.splits == 1) {
-            static_cast<T*>(a.out)[row * p.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
+        if (part < 0) {
+            static_cast<T*>(a.out)[((long long)sequence * a.heads + head0 + h) * p.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
         } else {
-            a.partial[(row * a.splits + split) * W + d] = o;
+            const long long row = part * a.heads + head0 + h;
+            a.partial[row * W + d] = o;
             if (d == 0) {
-                a.statistics[(row * a.splits + split) * 2] = top;
-                a.statistics[(row * a.splits + split) * 2 + 1] = sum;
+                a.statistics[row * 2] = top;
+                a.statistics[row * 2 + 1] = sum;
             }
         }
     }
-}
+    };  // work
 
-// One wave a row: the parts of its keys, in their order.
-template <typename T, int W>
-__global__ __launch_bounds__(64) void decode_join_kernel(DecodeCall a) {
-    const long long row = blockIdx.x;
-    const int lane = threadIdx.x;
-    const float* const st = a.statistics + row * a.splits * 2;
-    float top = -__builtin_inff();
-    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, st[2 * i]);
-    top = group_fmax(top, 64);
-    float o[W / 64] = {}, sum = 0.0f;
-    for (int i = 0; i < a.splits; ++i) {
-        const float m = st[2 * i], f = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-        sum = __builtin_fmaf(f, st[2 * i + 1], sum);
+    if constexpr (!STREAM) {
+        work(blockIdx.y, 0, (sequence_length(a, blockIdx.y) + KT - 1) / KT, -1);
+    } else {
+        __shared__ long long starts[kMostStreamed + 1], wave_sums[NW];
+        constexpr int PER = kMostStreamed / (64 * NW);
+        long long own[PER], upto = 0;
 #pragma unroll
-        for (int j = 0; j < W / 64; ++j) {
-            const int d = lane + 64 * j;
-            if (d < a.pool.head_dim) o[j] = __builtin_fmaf(f, a.partial[(row * a.splits + i) * W + d], o[j]);
+        for (int i = 0; i < PER; ++i) {
+            const int s = threadIdx.x * PER + i;
+            own[i] = upto;
+            upto += s < a.sequences ? sequence_tiles(a, s, KT) : 0;
+        }
+        long long before = upto;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const long long y = __shfl_up(before, o);
+            before += lane >= o ? y : 0;
+        }
+        if (lane == 63) wave_sums[wave] = before;
+        __syncthreads();
+        before -= upto;
+        for (int w = 0; w < wave; ++w) before += wave_sums[w];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) starts[threadIdx.x * PER + i] = before + own[i];
+        if (threadIdx.x == 64 * NW - 1) starts[kMostStreamed] = before + upto;
+        __syncthreads();
+        const long long tiles = starts[kMostStreamed];
+        const int ranges = (int)min((long long)gridDim.y, tiles);  // (none without a tile)
+        if ((int)blockIdx.y >= ranges) return;
+        const long long end = range_start(tiles, blockIdx.y + 1, ranges);
+        long long at = range_start(tiles, blockIdx.y, ranges);
+        int sequence = 0;  // the last that starts at `at` or before (each has a tile)
+        for (int o = kMostStreamed / 2; o > 0; o >>= 1)
+            if (sequence + o < a.sequences && starts[sequence + o] <= at) sequence += o;
+        for (; at < end; ++sequence) {
+            const long long first = starts[sequence], last = starts[sequence + 1], stop = min(end, last);
+            work(sequence, (int)(at - first), (int)(stop - first), at == first && stop == last ? -1 : (long long)blockIdx.y + sequence);
+            at = stop;
+            __syncthreads();  // (the waves' parts have been read)
         }
     }
-#pragma unroll
-    for (int j = 0; j < W / 64; ++j) {
-        const int d = lane + 64 * j;
-        if (d < a.pool.head_dim) static_cast<T*>(a.out)[row * a.pool.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o[j] / sum);
+}
+
+// One workgroup a row whose sequence passes the ends of ranges: its parts.  256 / W threads share a column, each takes every so many parts; their
+// sums are added in order.
+#ifndef RBMOE_DECODE_WG
+#define RBMOE_DECODE_WG 512
+#endif
+#ifndef RBMOE_DECODE_PART
+#define RBMOE_DECODE_PART 512
+#endif
+#ifndef RBMOE_DECODE_ONE
+#define RBMOE_DECODE_ONE 1024
+#endif
+constexpr int kDecodeWorkgroups = RBMOE_DECODE_WG, kLeastPart = RBMOE_DECODE_PART, kOnePart = RBMOE_DECODE_ONE;
+
+template <typename T, typename C, int W>
+__global__ __launch_bounds__(256) void decode_join_kernel(DecodeCall a) {
+    constexpr int S = 256 / W;
+    __shared__ float factor[kDecodeWorkgroups], tops[4], columns[S][W], sums[S];
+    __shared__ long long wave_sums[2][4];
+    const int sequence = blockIdx.x / a.heads, head = blockIdx.x % a.heads, tid = threadIdx.x;
+    long long before = 0, tiles = 0;
+    for (int i = tid; i < a.sequences; i += 256) {
+        const int n = sequence_tiles(a, i, tile_keys<C>());
+        tiles += n;
+        before += i < sequence ? n : 0;
     }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        before += __shfl_xor(before, o);
+        tiles += __shfl_xor(tiles, o);
+    }
+    if ((tid & 63) == 0) {
+        wave_sums[0][tid >> 6] = before;
+        wave_sums[1][tid >> 6] = tiles;
+    }
+    __syncthreads();
+    before = wave_sums[0][0] + wave_sums[0][1] + wave_sums[0][2] + wave_sums[0][3];
+    tiles = wave_sums[1][0] + wave_sums[1][1] + wave_sums[1][2] + wave_sums[1][3];
+    const int ranges = (int)min((long long)a.ranges, tiles);
+    auto range_of = [&](long long tile) {
+        int i = (int)(tile * ranges / tiles);
+        while (range_start(tiles, i + 1, ranges) <= tile) ++i;
+        return i;
+    };
+    const int first_range = range_of(before), last_range = range_of(before + sequence_tiles(a, sequence, tile_keys<C>()) - 1);
+    const int parts = last_range - first_range + 1;
+    if (parts == 1) return;  // written already
+    // consecutive parts are a.heads rows apart
+    const long long row = ((long long)first_range + sequence) * a.heads + head;
+    const float* const st = a.statistics + row * 2;
+    float top = -__builtin_inff();
+    for (int i = tid; i < parts; i += 256) top = fmaxf(top, st[(long long)i * 2 * a.heads]);
+    top = group_fmax(top, 64);
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    for (int i = tid; i < parts; i += 256) {
+        const float m = st[(long long)i * 2 * a.heads];
+        factor[i] = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    }
+    __syncthreads();
+    const int d = tid % W, slice = tid / W;
+    const float* const column = a.partial + row * W + d;
+    float o = 0.0f, sum = 0.0f;
+#pragma unroll 8
+    for (int i = slice; i < parts; i += S) {
+        o = __builtin_fmaf(factor[i], column[(long long)i * a.heads * W], o);
+        sum = __builtin_fmaf(factor[i], st[(long long)i * 2 * a.heads + 1], sum);
+    }
+    columns[slice][d] = o;
+    if (d == 0) sums[slice] = sum;
+    __syncthreads();
+    if (tid >= a.pool.head_dim) return;
+#pragma unroll
+    for (int i = 1; i < S; ++i) o += columns[i][tid];
+    sum = sums[0];
+#pragma unroll
+    for (int i = 1; i < S; ++i) sum += sums[i];
+    static_cast<T*>(a.out)[((long long)sequence * a.heads + head) * a.pool.head_dim + tid] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
 }
 
-constexpr int kDecodeWorkgroups = 1024, kLeastPart = 512;
-
-int decode_splits(int sequences, int kv_heads, int group, int longest) {
-    const long long rows = (long long)sequences * kv_heads * ((group + 15) / 16);
-    const long long wanted = (kDecodeWorkgroups + rows - 1) / rows;
-    return (int)std::max<long long>(1, std::min<long long>(wanted, (longest + kLeastPart - 1) / kLeastPart));
+DecodePlan decode_plan(int sequences, int kv_heads, int group, int longest) {
+    const long long groups = (long long)kv_heads * ((group + 15) / 16), rows = groups * sequences;
+    if (longest <= kOnePart || sequences > kMostStreamed) return {0, rows <= 256};
+    const long long least = ((long long)sequences * longest + kLeastPart - 1) / kLeastPart;
+    return {(int)std::max<long long>(1, std::min(kDecodeWorkgroups / groups, least)), false};
 }
-size_t decode_partials(int sequences, int kv_heads, int group) {
-    // sequences * heads * ceil(kDecodeWorkgroups / (sequences kv_heads blocks)) is less than both terms together
-    return (size_t)kDecodeWorkgroups * std::min(group, 16) + (size_t)sequences * kv_heads * group;
+size_t decode_partials(int sequences, int kv_heads, int group) {  // (ranges + sequences) * heads, of parts that begin or end within a sequence
+    return (size_t)kDecodeWorkgroups * std::min(group, 16) + (size_t)std::min(sequences, kMostStreamed) * kv_heads * group;
 }
 
 hipError_t launch_decode_attention(const DecodeCall& a, bool bf16_rows, hipStream_t s) {
     const int group = a.heads / a.pool.kv_heads;
     return with_types(a.pool, bf16_rows, [&](auto row, auto cache, auto width) -> hipError_t {
         typedef decltype(row) T;
+        typedef decltype(cache) C;
         constexpr int W = decltype(width)::value;
-        hipLaunchKernelGGL((decode_attention_kernel<T, decltype(cache), W>), dim3(a.pool.kv_heads * ((group + 15) / 16), a.splits, a.sequences),
-                           dim3(64 * kDecodeWaves), 0, s, a);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess || a.splits == 1) return e;
-        hipLaunchKernelGGL((decode_join_kernel<T, W>), dim3(a.sequences * a.heads), dim3(64), 0, s, a);
+        const int groups = a.pool.kv_heads * ((group + 15) / 16);
+        if (a.ranges > 0) hipLaunchKernelGGL((decode_attention_kernel<T, C, W, 4, true>), dim3(groups, a.ranges), dim3(256), 0, s, a);
+        else if (a.many) hipLaunchKernelGGL((decode_attention_kernel<T, C, W, many_waves<C, W>(), false>), dim3(groups, a.sequences), dim3(64 * many_waves<C, W>()), 0, s, a);
+        else hipLaunchKernelGGL((decode_attention_kernel<T, C, W, 4, false>), dim3(groups, a.sequences), dim3(256), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || a.ranges <= 1) return e;
+        hipLaunchKernelGGL((decode_join_kernel<T, C, W>), dim3(a.sequences * a.heads), dim3(256), 0, s, a);
         return hipGetLastError();
     });
 }
