@@ -60,54 +60,49 @@ __device__ __forceinline__ float other_half_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// ---- a tile of rows in LDS ---------------------------------------------------------------------
-// Rows of D elements without padding, in 16-byte pieces; piece c of row r lies at place c ^ swizzle(r), so that the reads along rows
-// (eight rows, one piece) and the transposing reads (four rows, 32 bytes) both find their banks free.
-template <typename T, int D>
-struct Tile {
-    static constexpr int V = 16 / sizeof(T), CH = D / V, ROW = CH * 16;
-    static constexpr int KC = CH / 2;  // steps of a product along D: each takes two pieces of a row, one per half of the wave
-    static constexpr int DB = D / 32;  // blocks of 32 columns
-    static __device__ __forceinline__ int swizzle(int r) {
-        if constexpr (CH == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
-        return (r & 3) << 2 | ((r >> 2) & 3);
-    }
-    static __device__ __forceinline__ const char* piece(const char* tile, int r, int c) { return tile + r * ROW + ((c ^ swizzle(r)) << 4); }
-
-    // ROWS rows from `first` on of a sequence's n, by TEAM waves; columns from head_dim on and rows from n on are zeros
-    template <int ROWS, int TEAM, bool A>
-    static __device__ __forceinline__ void stage(char* tile, const T* __restrict__ base, long long stride, int first, int n, int pieces) {
-        const int wave = TEAM == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+// ---- operands ------------------------------------------------------------------------------------
+// f32 rows as matrix operands: three bf16 parts of 8 bits each, cut off one behind the other, which add up to the value exactly.
+// Of the nine products of two values' parts the six largest are taken; the others are below 2^-22 of the product.
+// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  `guard`: an infinity has no rest, where inf - inf would make it NaN.
+struct Parts8 {
+    bf16x8 part[3];
+};
+template <bool GUARD>
+__device__ __forceinline__ Parts8 cut8(const float (&x)[8]) {
+    Parts8 r;
+    float rest[8];
 #pragma unroll
-        for (int i = 0; i < ROWS * CH / (64 * TEAM); ++i) {
-            const int at = (i * TEAM + wave) * 64, p = at + lane, r = p / CH, c = (p % CH) ^ swizzle(r);
-            const bool there = first + r < n && c < pieces;
-            const T* const src = base + (long long)(first + r) * stride + c * V;
-            if constexpr (A) {
-                issue_dma(lds_address(tile) + at * 16, there ? (const void*)src : (const void*)zero_piece);
-            } else {
-                Any16 x = {0, 0, 0, 0};
-                if (there) x = *reinterpret_cast<const Any16*>(src);
-                *reinterpret_cast<uint4*>(tile + p * 16) = make_uint4(x.x, x.y, x.z, x.w);
-            }
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // the upper halves of two
+            w[i] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * i + 1]), __float_as_uint(rest[2 * i]), 0x07060302);
+        r.part[n] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+        if (n == 2) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool stop = GUARD && n == 0 && fabsf(rest[i]) == __builtin_inff();
+            rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
+            if (stop) rest[i] = 0.0f;
         }
     }
-    static __device__ __forceinline__ float element(const char* tile, int r, int d) {
-        return to_f32(*reinterpret_cast<const T*>(piece(tile, r, d / V) + d % V * sizeof(T)));
-    }
-};
+    return r;
+}
 
 template <typename T>
 struct Mma;
 template <>
 struct Mma<bf16_t> {
-    typedef bf16x8 Rows;  // 8 elements of a row
-    struct Cols {         // a 32 x 32 block of scores as the second product takes it
+    static constexpr int P = 1;  // parts
+    typedef bf16x8 Rows;         // 8 elements of a row
+    struct Cols {                // a 32 x 32 block of scores as the second product takes it
         bf16x8 c[2];
     };
-    static __device__ __forceinline__ floatx16 rows(const Rows& a, const Rows& b, const floatx16& c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    }
+    static __device__ __forceinline__ bf16x8 part(const Rows& r, int) { return r; }
+    static __device__ __forceinline__ bf16x8 part(const Cols& p, int k, int) { return p.c[k]; }
+    template <bool GUARD>
     static __device__ __forceinline__ Cols cols(const floatx16& p) {
         Cols r;
 #pragma unroll
@@ -135,82 +130,161 @@ struct Mma<bf16_t> {
     static __device__ __forceinline__ float exponential(float s, float c, float reference) {
         return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -reference));
     }
-    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]
-    template <int D>
-    static __device__ __forceinline__ void add(floatx16 (&acc)[D / 32], const char* tile, int row0, const Cols& p) {
-        typedef Tile<bf16_t, D> T;
-        const int lane = threadIdx.x & 63, h = lane >> 5, j = (lane >> 2) & 3;
-        const int c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), in = (lane & 1) * 8;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-                const int r = row0 + 16 * k + 4 * h + j;
-                union {
-                    v4i16 x[2];
-                    bf16x8 v;
-                } u;
-                u.x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(T::piece(tile, r, 4 * b + c0) + in));
-                u.x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(T::piece(tile, r + 8, 4 * b + c0) + in));
-                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, p.c[k], acc[b], 0, 0, 0);
-            }
-    }
 };
 template <>
 struct Mma<float> {
-    typedef float4 Rows;
-    typedef floatx16 Cols;
-    static __device__ __forceinline__ floatx16 rows(const Rows& a, const Rows& b, floatx16 c) {
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, c, 0, 0, 0);
+    static constexpr int P = 3;
+    typedef Parts8 Rows;
+    struct Cols {
+        Parts8 c[2];
+    };
+    static __device__ __forceinline__ bf16x8 part(const Rows& r, int i) { return r.part[i]; }
+    static __device__ __forceinline__ bf16x8 part(const Cols& p, int k, int i) { return p.c[k].part[i]; }
+    template <bool GUARD>
+    static __device__ __forceinline__ Cols cols(const floatx16& p) {
+        Cols r;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float x[8] = {p[8 * k], p[8 * k + 1], p[8 * k + 2], p[8 * k + 3], p[8 * k + 4], p[8 * k + 5], p[8 * k + 6], p[8 * k + 7]};
+            r.c[k] = cut8<GUARD>(x);
+        }
+        return r;
     }
-    static __device__ __forceinline__ Cols cols(const floatx16& p) { return p; }
     static __device__ __forceinline__ float rounded(float v) { return v; }
     // (the factor is the caller's scale as it is, and only the difference is rounded with log2 e)
     static constexpr float unit = 1.0f, natural = 1.0f;
     static __device__ __forceinline__ float exponential(float s, float c, float reference) {
         return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -reference) * kLog2e);
     }
-    template <int D>
-    static __device__ __forceinline__ void add(floatx16 (&acc)[D / 32], const char* tile, int row0, const Cols& p) {
-        typedef Tile<float, D> T;
-        const int lane = threadIdx.x & 63, h = lane >> 5;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = row0 + 8 * (i >> 2) + 4 * h + (i & 3);
-#pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-                const float x = *reinterpret_cast<const float*>(T::piece(tile, r, 8 * b + ((lane & 31) >> 2)) + (lane & 3) * 4);
-                acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], acc[b], 0, 0, 0);
-            }
-        }
-    }
 };
-
 template <typename T>
 using RowsOf = typename Mma<T>::Rows;
 
-template <typename T, int D>
-__device__ __forceinline__ RowsOf<T> row_pieces(const char* tile, int row0, int kc) {
-    const int lane = threadIdx.x & 63;
-    return *reinterpret_cast<const RowsOf<T>*>(Tile<T, D>::piece(tile, row0 + (lane & 31), 2 * kc + (lane >> 5)));
+__device__ __forceinline__ void load8(const bf16_t* p, float (&v)[8]) {
+    const Any16 x = *reinterpret_cast<const Any16*>(p);
+    Vec16<bf16_t>::widen(make_uint4(x.x, x.y, x.z, x.w), v);
 }
-// The product of 32 of the tile's rows with the wave's own: register i of lane l holds tile row 8 (i / 4) + 4 (l / 32) + i % 4, own row l % 32.
-template <typename T, int D>
-__device__ __forceinline__ floatx16 product(const char* tile, int row0, const RowsOf<T> (&own)[Tile<T, D>::KC]) {
-    floatx16 c;
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) c[i] = 0.0f;
-#pragma unroll
-    for (int kc = 0; kc < Tile<T, D>::KC; ++kc) c = Mma<T>::rows(row_pieces<T, D>(tile, row0, kc), own[kc], c);
-    return c;
+    for (int i = 0; i < 2; ++i) {
+        const Any16 x = *reinterpret_cast<const Any16*>(p + 4 * i);
+        v[4 * i] = __uint_as_float(x.x); v[4 * i + 1] = __uint_as_float(x.y); v[4 * i + 2] = __uint_as_float(x.z); v[4 * i + 3] = __uint_as_float(x.w);
+    }
 }
+
+// ---- a tile of rows in LDS ---------------------------------------------------------------------
+// N rows of D elements as bf16 parts, one part behind the other, without padding, in 16-byte pieces; piece c of row r lies at place c ^ swizzle(r), so
+// that the reads along rows (eight rows, one piece) and the transposing reads (four rows, 32 bytes) both find their banks free.
+template <typename T, int D, int N>
+struct Tile {
+    static constexpr int P = Mma<T>::P, CH = D / 8, ROW = D * 2, PART = N * ROW, BYTES = P * PART;
+    static constexpr int KC = D / 16;  // steps of a product along D: each takes two pieces of a row, one per half of the wave
+    static constexpr int DB = D / 32;  // blocks of 32 columns
+    static __device__ __forceinline__ int swizzle(int r) {
+        if constexpr (CH == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+        return (r & 3) << 2 | ((r >> 2) & 3);
+    }
+    static __device__ __forceinline__ const char* piece(const char* tile, int r, int c) { return tile + r * ROW + ((c ^ swizzle(r)) << 4); }
+    static __device__ __forceinline__ float element(const char* tile, int r, int d) {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = P - 1; i >= 0; --i) x += to_f32(*reinterpret_cast<const bf16_t*>(piece(tile + i * PART, r, d / 8) + d % 8 * 2));
+        return x;
+    }
+
+    // The rows from `first` on of a sequence's n, by TEAM waves; columns from head_dim on and rows from n on are zeros.  begin() has the loads
+    // under way, finish() leaves them in the tile: bf16 rows on 16-byte boundaries get there without it.
+    template <int TEAM, bool A>
+    struct Stager {
+        static constexpr int UNITS = N * CH / (64 * TEAM);  // pieces of 8 elements a lane
+        float x[P == 3 ? UNITS : 1][8];
+        Any16 raw[P == 1 && !A ? UNITS : 1];
+        __device__ __forceinline__ void begin(char* tile, const T* __restrict__ base, long long stride, int first, int n, int pieces) {
+            const int wave = TEAM == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const int at = (i * TEAM + wave) * 64, p = at + lane, r = p / CH, c = (p % CH) ^ swizzle(r);
+                const bool there = first + r < n && c < pieces;
+                const T* const src = base + (long long)(first + r) * stride + c * 8;
+                if constexpr (P == 3) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+                    if (there) load8(src, x[i]);
+                } else if constexpr (A) {
+                    issue_dma(lds_address(tile) + at * 16, there ? (const void*)src : (const void*)zero_piece);
+                } else {
+                    raw[i] = Any16{0, 0, 0, 0};
+                    if (there) raw[i] = *reinterpret_cast<const Any16*>(src);
+                }
+            }
+        }
+        template <bool GUARD>
+        __device__ __forceinline__ void finish(char* tile) {
+            if constexpr (P == 3 || !A) {
+#pragma unroll
+                for (int i = 0; i < UNITS; ++i) {
+                    char* const to = tile + (i * TEAM * 64 + (int)(threadIdx.x & (64 * TEAM - 1))) * 16;
+                    if constexpr (P == 3) {
+                        const Parts8 parts = cut8<GUARD>(x[i]);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(to + k * PART) = parts.part[k];
+                    } else {
+                        *reinterpret_cast<uint4*>(to) = make_uint4(raw[i].x, raw[i].y, raw[i].z, raw[i].w);
+                    }
+                }
+            }
+        }
+    };
+
+    // The product of 32 of the tile's rows with the wave's own: register i of lane l holds tile row 8 (i / 4) + 4 (l / 32) + i % 4, own row l % 32.
+    static __device__ __forceinline__ floatx16 product(const char* tile, int row0, const RowsOf<T> (&own)[KC]) {
+        const int lane = threadIdx.x & 63;
+        floatx16 c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            bf16x8 rows[P];
+#pragma unroll
+            for (int i = 0; i < P; ++i) rows[i] = *reinterpret_cast<const bf16x8*>(piece(tile + i * PART, row0 + (lane & 31), 2 * kc + (lane >> 5)));
+#pragma unroll
+            for (int s = P - 1; s >= 0; --s)  // small ones first
+#pragma unroll
+                for (int i = 0; i <= s; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows[i], Mma<T>::part(own[kc], s - i), c, 0, 0, 0);
+        }
+        return c;
+    }
+    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]
+    static __device__ __forceinline__ void add(floatx16 (&acc)[DB], const char* tile, int row0, const typename Mma<T>::Cols& p) {
+        const int lane = threadIdx.x & 63, h = lane >> 5, j = (lane >> 2) & 3;
+        const int c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), in = (lane & 1) * 8;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int b = 0; b < DB; ++b) {
+                const int r = row0 + 16 * k + 4 * h + j;
+                bf16x8 cols[P];
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    union {
+                        v4i16 x[2];
+                        bf16x8 v;
+                    } u;
+                    u.x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(piece(tile + i * PART, r, 4 * b + c0) + in));
+                    u.x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(piece(tile + i * PART, r + 8, 4 * b + c0) + in));
+                    cols[i] = u.v;
+                }
+#pragma unroll
+                for (int s = P - 1; s >= 0; --s)
+#pragma unroll
+                    for (int i = 0; i <= s; ++i) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols[i], Mma<T>::part(p, k, s - i), acc[b], 0, 0, 0);
+            }
+    }
+};
 __device__ __forceinline__ int block_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (i & 3); }
 
-// Mma::add for a block of which some places are masked, whatever the tile holds there: row by row, the places that `sees`(row) allows.
-template <typename T, int D, typename F>
+// Tile::add for a block of which some places are masked, whatever the tile holds there: row by row, the places that `sees`(row) allows.
+template <typename T, int D, int N, typename F>
 __device__ __forceinline__ void add_seen(floatx16 (&acc)[D / 32], const char* tile, int row0, const floatx16& p, F sees) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma clang loop unroll(disable)
@@ -224,7 +298,7 @@ __device__ __forceinline__ void add_seen(floatx16 (&acc)[D / 32], const char* ti
         for (int b = 0; b < D / 32; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float y = Tile<T, D>::element(tile, row0 + r, 32 * b + 8 * (e >> 2) + 4 * h + (e & 3));
+                const float y = Tile<T, D, N>::element(tile, row0 + r, 32 * b + 8 * (e >> 2) + 4 * h + (e & 3));
                 acc[b][e] = seen ? __builtin_fmaf(x, y, acc[b][e]) : acc[b][e];
             }
     }
@@ -242,13 +316,20 @@ __device__ __forceinline__ bool any_not_finite(const floatx16 (&acc)[N]) {
 // ---- a wave's own rows ---------------------------------------------------------------------------
 // The row of lane l % 32 as the products' B operand, zeros where it or its columns are not there.
 template <typename T, int D>
-__device__ __forceinline__ void load_own(const T* __restrict__ row, bool there, int pieces, RowsOf<T> (&own)[Tile<T, D>::KC]) {
+__device__ __forceinline__ void load_own(const T* __restrict__ row, bool there, int pieces, RowsOf<T> (&own)[D / 16]) {
     const int h = (threadIdx.x >> 5) & 1;
 #pragma unroll
-    for (int kc = 0; kc < Tile<T, D>::KC; ++kc) {
-        Any16 x = {0, 0, 0, 0};
-        if (there && 2 * kc + h < pieces) x = *reinterpret_cast<const Any16*>(row + (2 * kc + h) * Tile<T, D>::V);
-        own[kc] = __builtin_bit_cast(RowsOf<T>, x);
+    for (int kc = 0; kc < D / 16; ++kc) {
+        const bool in = there && 2 * kc + h < pieces;
+        if constexpr (sizeof(T) == 4) {
+            float x[8] = {};
+            if (in) load8(row + (2 * kc + h) * 8, x);
+            own[kc] = cut8<true>(x);
+        } else {
+            Any16 x = {0, 0, 0, 0};
+            if (in) x = *reinterpret_cast<const Any16*>(row + (2 * kc + h) * 8);
+            own[kc] = __builtin_bit_cast(bf16x8, x);
+        }
     }
 }
 __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
@@ -348,26 +429,54 @@ template <typename T, int TEAM>
 constexpr int tile_rows() {
     return sizeof(T) == 2 && TEAM == 4 ? 64 : 32;
 }
-// Stages of tiles: the next is loaded while one is used, where four teams' find room in the LDS of 160 KB.
-template <typename T, int D, int TEAM>
+// Stages of tiles.  TEAM 4: two, one is filled while the other is used.  TEAM 1: one, the workgroups beside this one on its compute unit are busy meanwhile.
+template <int TEAM>
 constexpr int tile_stages() {
-    return TEAM == 1 && sizeof(T) * D > 256 ? 1 : 2;
+    return TEAM == 1 ? 1 : 2;
 }
 template <typename T, int D, int TEAM>
 constexpr int tiles_lds(int extra) {  // of two tiles and `extra` bytes a stage
-    return (kWaves / TEAM) * tile_stages<T, D, TEAM>() * (2 * tile_rows<T, TEAM>() * Tile<T, D>::ROW + extra);
+    return (kWaves / TEAM) * tile_stages<TEAM>() * (2 * Tile<T, D, tile_rows<T, TEAM>()>::BYTES + extra);
 }
 __device__ __forceinline__ void wait_for_tile(bool common) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's part of the tile has landed, its reads of the other stage are done
     if (common) __syncthreads();                                 // and the other waves'
 }
 
+// A wave's or workgroup's tiles from `start` to `end`, `step` apart: the next one's loads are under way while one is used.  With one stage
+// f32 rows wait in registers meanwhile; bf16 rows, which are loaded straight into it, are waited for.
+template <int STAGES, int PARTS, int TEAM, typename B, typename F, typename U>
+__device__ __forceinline__ void over_tiles(int start, int end, int step, B begin, F finish, U use) {
+    if constexpr (STAGES == 1 && PARTS == 1) {
+        for (int t = start; t < end; t += step) {
+            wait_for_tile(false);
+            begin(0, t);
+            finish(0);
+            wait_for_tile(false);
+            use(0, t);
+        }
+    } else {
+        if (start < end) {
+            begin(0, start);
+            finish(0);
+        }
+        for (int t = start, buf = 0; t < end; t += step, buf ^= STAGES - 1) {
+            wait_for_tile(TEAM == 4);
+            const bool more = t + step < end;
+            if (more) begin(buf ^ (STAGES - 1), t + step);
+            use(buf, t);
+            if (more) finish(buf ^ (STAGES - 1));
+        }
+    }
+}
+
 // ---- forward ----------------------------------------------------------------------------------------
 
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attention_forward_kernel(AttentionCall a) {
-    typedef Tile<T, D> Tl;
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, BYTES = N * Tl::ROW, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM>();
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<TEAM>();
+    typedef Tile<T, D, N> Tl;
+    constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of keys and values
     const int tiles = (a.longest_queries + OWN - 1) / OWN;
     const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
@@ -375,7 +484,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attenti
     const int first = at.tile * OWN;
     if (first >= s.nq) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
-    const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / Tl::V;
+    const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / 8;
     const T* const k = static_cast<const T*>(a.k) + (long long)s.k0 * a.k_stride + (long long)kv * a.head_dim;
     const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
     const int wave_first = TEAM == 1 ? first : first + 32 * wave, row = wave_first + (lane & 31);
@@ -401,25 +510,24 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attenti
             for (int i = 0; i < 16; ++i) acc[b][i] = 0.0f;
         m = -__builtin_inff();
         l = 0.0f;
-        auto stage = [&](int buf, int t) {
+        typename Tl::template Stager<TEAM, A> keys, values;
+        auto begin = [&](int buf, int t) {
             char* const to = tiles_at + buf * 2 * BYTES;
-            Tl::template stage<N, TEAM, A>(to, k, a.k_stride, t, s.nk, pieces);
-            Tl::template stage<N, TEAM, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
+            keys.begin(to, k, a.k_stride, t, s.nk, pieces);
+            values.begin(to + BYTES, v, a.v_stride, t, s.nk, pieces);
         };
-        if (STAGES == 2 && start < end) stage(0, start);
-        for (int t = start, buf = 0; t < end; t += STEP, buf ^= STAGES - 1) {
-            if (STAGES == 1) {
-                wait_for_tile(false);
-                stage(0, t);
-            }
-            wait_for_tile(TEAM == 4);
-            if (STAGES == 2 && t + STEP < end) stage(buf ^ 1, t + STEP);
-            if (t >= most || wave_first >= s.nq) continue;
+        auto finish = [&](int buf) {
+            char* const to = tiles_at + buf * 2 * BYTES;
+            keys.template finish<decltype(careful)::value>(to);
+            values.template finish<decltype(careful)::value>(to + BYTES);
+        };
+        auto use = [&](int buf, int t) {
+            if (t >= most || wave_first >= s.nq) return;
             const char* const kt = tiles_at + buf * 2 * BYTES;
             const char* const vt = kt + BYTES;
             floatx16 p[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) p[b] = product<T, D>(kt, 32 * b, q);
+            for (int b = 0; b < NB; ++b) p[b] = Tl::product(kt, 32 * b, q);
             if (t + N > least) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -456,11 +564,12 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attenti
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (decltype(careful)::value && t + N > least)
-                    add_seen<T, D>(acc, vt, 32 * b, p[b], [&](int r) { return t + 32 * b + r < own_limit; });
+                    add_seen<T, D, N>(acc, vt, 32 * b, p[b], [&](int r) { return t + 32 * b + r < own_limit; });
                 else
-                    Mma<T>::template add<D>(acc, vt, 32 * b, Mma<T>::cols(p[b]));
+                    Tl::add(acc, vt, 32 * b, Mma<T>::template cols<decltype(careful)::value>(p[b]));
             }
-        }
+        };
+        over_tiles<STAGES, Tl::P, TEAM>(start, end, STEP, begin, finish, use);
     };
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
@@ -486,8 +595,9 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attenti
 // ---- backward: gradients of the queries ------------------------------------------------------------------
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_kernel(AttentionCall a) {
-    typedef Tile<T, D> Tl;
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, BYTES = N * Tl::ROW, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM>();
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<TEAM>();
+    typedef Tile<T, D, N> Tl;
+    constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
     const int tiles = (a.longest_queries + OWN - 1) / OWN;
     const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
@@ -495,7 +605,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
     const int first = at.tile * OWN;
     if (first >= s.nq) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5;
-    const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / Tl::V;
+    const int kv = at.head / (a.heads / a.kv_heads), pieces = a.head_dim / 8;
     const T* const k = static_cast<const T*>(a.k) + (long long)s.k0 * a.k_stride + (long long)kv * a.head_dim;
     const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
     const int wave_first = TEAM == 1 ? first : first + 32 * wave, row = wave_first + (lane & 31);
@@ -509,13 +619,11 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
 #pragma unroll
     for (int kc = 0; kc < Tl::KC; ++kc) {
         if (!there || 2 * kc + h >= pieces) continue;
-        float x[Tl::V], y[Tl::V];
-        const long long at_piece = in_out + (2 * kc + h) * Tl::V;
-        const Any16 o = *reinterpret_cast<const Any16*>(static_cast<const T*>(a.out) + at_piece);
-        Vec16<T>::widen(make_uint4(o.x, o.y, o.z, o.w), x);
-        Vec16<T>::widen(__builtin_bit_cast(uint4, dout[kc]), y);
+        float x[8], y[8];
+        load8(static_cast<const T*>(a.out) + in_out + (2 * kc + h) * 8, x);
+        load8(static_cast<const T*>(a.grad_out) + in_out + (2 * kc + h) * 8, y);
 #pragma unroll
-        for (int i = 0; i < Tl::V; ++i) delta = __builtin_fmaf(x[i], y[i], delta);
+        for (int i = 0; i < 8; ++i) delta = __builtin_fmaf(x[i], y[i], delta);
     }
     delta = other_half_sum(delta);
     const float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
@@ -540,25 +648,24 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[b][i] = mean[mend ? b : 0][i] = 0.0f;
         sum = rounded_sum = 0.0f;
-        auto stage = [&](int buf, int t) {
+        typename Tl::template Stager<TEAM, A> keys, values;
+        auto begin = [&](int buf, int t) {
             char* const to = tiles_at + buf * 2 * BYTES;
-            Tl::template stage<N, TEAM, A>(to, k, a.k_stride, t, s.nk, pieces);
-            Tl::template stage<N, TEAM, A>(to + BYTES, v, a.v_stride, t, s.nk, pieces);
+            keys.begin(to, k, a.k_stride, t, s.nk, pieces);
+            values.begin(to + BYTES, v, a.v_stride, t, s.nk, pieces);
         };
-        if (STAGES == 2 && start < end) stage(0, start);
-        for (int t = start, buf = 0; t < end; t += STEP, buf ^= STAGES - 1) {
-            if (STAGES == 1) {
-                wait_for_tile(false);
-                stage(0, t);
-            }
-            wait_for_tile(TEAM == 4);
-            if (STAGES == 2 && t + STEP < end) stage(buf ^ 1, t + STEP);
-            if (t >= most || wave_first >= s.nq) continue;
+        auto finish = [&](int buf) {
+            char* const to = tiles_at + buf * 2 * BYTES;
+            keys.template finish<decltype(careful)::value>(to);
+            values.template finish<decltype(careful)::value>(to + BYTES);
+        };
+        auto use = [&](int buf, int t) {
+            if (t >= most || wave_first >= s.nq) return;
             const char* const kt = tiles_at + buf * 2 * BYTES;
             const char* const vt = kt + BYTES;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                floatx16 p = product<T, D>(kt, 32 * b, q), dp = product<T, D>(vt, 32 * b, dout);
+                floatx16 p = Tl::product(kt, 32 * b, q), dp = Tl::product(vt, 32 * b, dout);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     p[i] = Mma<T>::exponential(p[i], c, reference);
@@ -569,7 +676,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
                     for (int i = 0; i < 16; ++i)
                         if (t + 32 * b + block_row(i) >= own_limit) p[i] = dp[i] = 0.0f;
                 }
-                const auto ds = Mma<T>::cols(dp);
+                const auto ds = Mma<T>::template cols<decltype(careful)::value>(dp);
                 if constexpr (mend) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sum += dp[i];
@@ -577,14 +684,15 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
                 }
                 if (decltype(careful)::value && t + N > least) {
                     auto sees = [&](int r) { return t + 32 * b + r < own_limit; };
-                    add_seen<T, D>(acc, kt, 32 * b, dp, sees);
-                    if constexpr (mend) add_seen<T, D>(mean, kt, 32 * b, p, sees);
+                    add_seen<T, D, N>(acc, kt, 32 * b, dp, sees);
+                    if constexpr (mend) add_seen<T, D, N>(mean, kt, 32 * b, p, sees);
                 } else {
-                    Mma<T>::template add<D>(acc, kt, 32 * b, ds);
-                    if constexpr (mend) Mma<T>::template add<D>(mean, kt, 32 * b, Mma<T>::cols(p));
+                    Tl::add(acc, kt, 32 * b, ds);
+                    if constexpr (mend) Tl::add(mean, kt, 32 * b, Mma<T>::template cols<false>(p));
                 }
             }
-        }
+        };
+        over_tiles<STAGES, Tl::P, TEAM>(start, end, STEP, begin, finish, use);
     };
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
@@ -613,8 +721,9 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
 // ---- backward: gradients of keys and values -------------------------------------------------------------
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_kv_kernel(AttentionCall a) {
-    typedef Tile<T, D> Tl;
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, BYTES = N * Tl::ROW, STAGE = 2 * BYTES + 2 * N * 4, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM>();
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<TEAM>();
+    typedef Tile<T, D, N> Tl;
+    constexpr int BYTES = Tl::BYTES, STAGE = 2 * BYTES + 2 * N * 4;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
     const int tiles = (a.longest_keys + OWN - 1) / OWN;
     const Place at = place_of(a.kv_heads, a.sequences, tiles, false);
@@ -622,7 +731,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     const int first = at.tile * OWN, kv = at.head, group = a.heads / a.kv_heads;
     if (first >= s.nk) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int pieces = a.head_dim / Tl::V;
+    const int pieces = a.head_dim / 8;
     const int wave_first = TEAM == 1 ? first : first + 32 * wave, key = wave_first + (lane & 31);
     const bool there = key < s.nk;
     RowsOf<T> k[Tl::KC], v[Tl::KC];
@@ -645,7 +754,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
 #pragma unroll
             for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.0f;
         // turn i: head i / turns of the group, rows from begin + N (i % turns) on
-        auto stage = [&](int buf, int i) {
+        typename Tl::template Stager<TEAM, A> queries, gradients;
+        auto begin_tile = [&](int buf, int i) {
             const int head = kv * group + i / turns, t = begin + i % turns * N;
             char* const to = tiles_at + buf * STAGE;
             if (TEAM == 1 || wave < 2 * N / 64) {  // references, then deltas
@@ -653,27 +763,25 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 const float* const from = a.delta + (i < N ? 0 : (long long)a.heads * a.query_rows) + (long long)head * a.query_rows + s.q0 + r;
                 issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), r < s.nq ? (const void*)from : (const void*)zero_piece);
             }
-            Tl::template stage<N, TEAM, A>(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
-            Tl::template stage<N, TEAM, A>(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
-                                     (long long)a.heads * a.head_dim, t, s.nq, pieces);
+            queries.begin(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
+            gradients.begin(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
+                            (long long)a.heads * a.head_dim, t, s.nq, pieces);
         };
-        if (STAGES == 2 && mine < all) stage(0, mine);
-        for (int i = mine, buf = 0; i < all; i += STEP, buf ^= STAGES - 1) {
-            if (STAGES == 1) {
-                wait_for_tile(false);
-                stage(0, i);
-            }
-            wait_for_tile(TEAM == 4);
-            if (STAGES == 2 && i + STEP < all) stage(buf ^ 1, i + STEP);
+        auto finish = [&](int buf) {
+            char* const to = tiles_at + buf * STAGE;
+            queries.template finish<decltype(careful)::value>(to);
+            gradients.template finish<decltype(careful)::value>(to + BYTES);
+        };
+        auto use = [&](int buf, int i) {
             const int t = begin + i % turns * N;
-            if (t + N <= least || wave_first >= s.nk) continue;
+            if (t + N <= least || wave_first >= s.nk) return;
             const char* const qt = tiles_at + buf * STAGE;
             const char* const ot = qt + BYTES;
             const float* const references = reinterpret_cast<const float*>(ot + BYTES);
             const bool masked = t < most || t + N > s.nq;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                floatx16 p = product<T, D>(qt, 32 * b, k), dp = product<T, D>(ot, 32 * b, v);
+                floatx16 p = Tl::product(qt, 32 * b, k), dp = Tl::product(ot, 32 * b, v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 32 * b + block_row(4 * e);
@@ -692,14 +800,15 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                         if (!sees(block_row(e))) p[e] = dp[e] = 0.0f;
                 }
                 if (decltype(careful)::value && masked) {
-                    add_seen<T, D>(dv, ot, 32 * b, p, sees);
-                    add_seen<T, D>(dk, qt, 32 * b, dp, sees);
+                    add_seen<T, D, N>(dv, ot, 32 * b, p, sees);
+                    add_seen<T, D, N>(dk, qt, 32 * b, dp, sees);
                 } else {
-                    Mma<T>::template add<D>(dv, ot, 32 * b, Mma<T>::cols(p));
-                    Mma<T>::template add<D>(dk, qt, 32 * b, Mma<T>::cols(dp));
+                    Tl::add(dv, ot, 32 * b, Mma<T>::template cols<decltype(careful)::value>(p));
+                    Tl::add(dk, qt, 32 * b, Mma<T>::template cols<decltype(careful)::value>(dp));
                 }
             }
-        }
+        };
+        over_tiles<STAGES, 1, TEAM>(mine, all, STEP, begin_tile, finish, use);
     };
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(dk) || any_not_finite(dv))) pass(std::true_type{});
@@ -714,14 +823,18 @@ bool whole_pieces(const void* p, long long stride, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
 }
 
-// f(element type, padded head width, waves a team, rows start on 16-byte boundaries)
+// f(element type, padded head width, waves a team, rows on 16-byte boundaries, where that matters)
 template <typename F>
 hipError_t with_kernel(bool bf16, int head_dim, bool few, bool aligned, F f) {
     auto rows = [&](auto type, auto width, auto team) -> hipError_t {
-        return aligned ? f(type, width, team, std::true_type{}) : f(type, width, team, std::false_type{});
+        if constexpr (sizeof(type) == 2)
+            if (aligned) return f(type, width, team, std::true_type{});
+        return f(type, width, team, std::false_type{});
     };
     auto team = [&](auto type, auto width) -> hipError_t {
-        return few ? rows(type, width, std::integral_constant<int, 1>{}) : rows(type, width, std::integral_constant<int, 4>{});
+        if constexpr (sizeof(type) * decltype(width)::value > 256)  // (four teams' tiles of three parts are more than the LDS)
+            return rows(type, width, std::integral_constant<int, 4>{});
+        else return few ? rows(type, width, std::integral_constant<int, 1>{}) : rows(type, width, std::integral_constant<int, 4>{});
     };
     auto width = [&](auto type) -> hipError_t {
         return head_dim <= 64 ? team(type, std::integral_constant<int, 64>{}) : team(type, std::integral_constant<int, 128>{});
