@@ -331,6 +331,11 @@ __device__ __forceinline__ void load_own(const T* __restrict__ row, bool there, 
             own[kc] = __builtin_bit_cast(bf16x8, x);
         }
     }
+    // In use here and now: the wait for these loads would otherwise stand in front of their first use in the loop over tiles, where every turn
+    // would wait for the next tile's loads with it.
+    if constexpr (sizeof(T) == 2)
+#pragma unroll
+        for (int kc = 0; kc < D / 16; ++kc) asm volatile("" : "+v"(own[kc]));
 }
 __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
     *reinterpret_cast<Any16*>(p) = Any16{__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)};
@@ -626,7 +631,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
         for (int i = 0; i < 8; ++i) delta = __builtin_fmaf(x[i], y[i], delta);
     }
     delta = other_half_sum(delta);
-    const float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
+    float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
+    asm volatile("" : "+v"(reference));  // (as in load_own)
 
     auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
