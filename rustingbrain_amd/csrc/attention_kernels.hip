@@ -254,8 +254,10 @@ struct Tile {
         }
         return c;
     }
-    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]
-    static __device__ __forceinline__ void add(floatx16 (&acc)[DB], const char* tile, int row0, const typename Mma<T>::Cols& p) {
+    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]; of M's parts (bf16_t: the first ones alone)
+    template <typename M = T>
+    static __device__ __forceinline__ void add(floatx16 (&acc)[DB], const char* tile, int row0, const typename Mma<M>::Cols& p) {
+        constexpr int P = Mma<M>::P;
         const int lane = threadIdx.x & 63, h = lane >> 5, j = (lane >> 2) & 3;
         const int c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), in = (lane & 1) * 8;
 #pragma unroll
@@ -277,7 +279,7 @@ struct Tile {
 #pragma unroll
                 for (int s = P - 1; s >= 0; --s)
 #pragma unroll
-                    for (int i = 0; i <= s; ++i) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols[i], Mma<T>::part(p, k, s - i), acc[b], 0, 0, 0);
+                    for (int i = 0; i <= s; ++i) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols[i], Mma<M>::part(p, k, s - i), acc[b], 0, 0, 0);
             }
     }
 };
@@ -434,14 +436,15 @@ template <typename T, int TEAM>
 constexpr int tile_rows() {
     return sizeof(T) == 2 && TEAM == 4 ? 64 : 32;
 }
-// Stages of tiles.  TEAM 4: two, one is filled while the other is used.  TEAM 1: one, the workgroups beside this one on its compute unit are busy meanwhile.
-template <int TEAM>
+// Stages of tiles.  TEAM 4: two, one is filled while the other is used.  TEAM 1: one, where workgroups beside this one on its compute unit are busy
+// meanwhile, or the next tile waits in registers; two for kernels whose registers leave room for one workgroup (ALONE).
+template <typename T, int D, int TEAM, bool ALONE>
 constexpr int tile_stages() {
-    return TEAM == 1 ? 1 : 2;
+    return TEAM == 4 || (ALONE && sizeof(T) == 2 && D == 128) ? 2 : 1;
 }
-template <typename T, int D, int TEAM>
+template <typename T, int D, int TEAM, bool ALONE>
 constexpr int tiles_lds(int extra) {  // of two tiles and `extra` bytes a stage
-    return (kWaves / TEAM) * tile_stages<TEAM>() * (2 * Tile<T, D, tile_rows<T, TEAM>()>::BYTES + extra);
+    return (kWaves / TEAM) * tile_stages<T, D, TEAM, ALONE>() * (2 * Tile<T, D, tile_rows<T, TEAM>()>::BYTES + extra);
 }
 __device__ __forceinline__ void wait_for_tile(bool common) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's part of the tile has landed, its reads of the other stage are done
@@ -478,8 +481,8 @@ __device__ __forceinline__ void over_tiles(int start, int end, int step, B begin
 // ---- forward ----------------------------------------------------------------------------------------
 
 template <typename T, int D, int TEAM, bool A>
-__global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attention_forward_kernel(AttentionCall a) {
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<TEAM>();
+__global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 && TEAM == 1) ? 1 : 2) void attention_forward_kernel(AttentionCall a) {
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, false>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of keys and values
@@ -599,8 +602,8 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 ? 1 : 2) void attenti
 
 // ---- backward: gradients of the queries ------------------------------------------------------------------
 template <typename T, int D, int TEAM, bool A>
-__global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_kernel(AttentionCall a) {
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<TEAM>();
+__global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_q_kernel(AttentionCall a) {
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, true>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
@@ -641,18 +644,18 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
     const int start = TEAM == 1 ? wave * N : 0;
     char* const tiles_at = attention_lds + (TEAM == 1 ? wave * STAGES * 2 * BYTES : 0);
     const float c = a.scale * Mma<T>::unit;
-    // For bf16 rows delta comes from rounded rows of `out`, and ds is rounded.  Both errors make a row's ds add up to something
-    // else than its true sum of zero, and where keys share a direction that goes along it.  So the sum of the rounded ds is taken
-    // off again in proportion to p (grad_q -= sum * mean key), and delta handed on as what makes the sum of the unrounded ones zero.
-    constexpr bool mend = sizeof(T) == 2;
-    floatx16 acc[Tl::DB], mean[mend ? Tl::DB : 1];
+    // delta comes from `out` as it was stored, and ds is rounded for bf16 rows.  Both errors make a row's ds add up to something
+    // else than its true sum of zero, and where keys share a direction that goes along it.  So the sum of the ds is taken
+    // off again in proportion to p (grad_q -= sum * mean key; the sum is small, bf16 does for the mean), and delta handed on as what makes the
+    // sum of the unrounded ones zero.
+    floatx16 acc[Tl::DB], mean[Tl::DB];
     float sum, rounded_sum;
 
     auto pass = [&](auto careful) {
 #pragma unroll
         for (int b = 0; b < Tl::DB; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[b][i] = mean[mend ? b : 0][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) acc[b][i] = mean[b][i] = 0.0f;
         sum = rounded_sum = 0.0f;
         typename Tl::template Stager<TEAM, A> keys, values;
         auto begin = [&](int buf, int t) {
@@ -683,18 +686,16 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
                         if (t + 32 * b + block_row(i) >= own_limit) p[i] = dp[i] = 0.0f;
                 }
                 const auto ds = Mma<T>::template cols<decltype(careful)::value>(dp);
-                if constexpr (mend) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum += dp[i];
-                    rounded_sum = Mma<T>::total(ds, rounded_sum);
-                }
+                for (int i = 0; i < 16; ++i) sum += dp[i];
+                if constexpr (sizeof(T) == 2) rounded_sum = Mma<T>::total(ds, rounded_sum);
                 if (decltype(careful)::value && t + N > least) {
                     auto sees = [&](int r) { return t + 32 * b + r < own_limit; };
                     add_seen<T, D, N>(acc, kt, 32 * b, dp, sees);
-                    if constexpr (mend) add_seen<T, D, N>(mean, kt, 32 * b, p, sees);
+                    add_seen<T, D, N>(mean, kt, 32 * b, p, sees);
                 } else {
                     Tl::add(acc, kt, 32 * b, ds);
-                    if constexpr (mend) Tl::add(mean, kt, 32 * b, Mma<T>::template cols<false>(p));
+                    Tl::template add<bf16_t>(mean, kt, 32 * b, Mma<bf16_t>::cols<false>(p));
                 }
             }
         };
@@ -703,31 +704,31 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void attention_grad_q_k
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(acc))) pass(std::true_type{});
     if constexpr (TEAM == 1) __syncthreads();
-    if constexpr (mend) {
-        rounded_sum = other_half_sum(rounded_sum);
-        sum = other_half_sum(sum);
-        if constexpr (TEAM == 1) {
-            rounded_sum = over_waves<false>(rounded_sum, attention_lds);
-            sum = over_waves<false>(sum, attention_lds);
-        }
-        delta += sum;
-#pragma unroll
-        for (int b = 0; b < Tl::DB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_fmaf(-rounded_sum, mean[b][i], acc[b][i]);
+    if constexpr (sizeof(T) == 4) rounded_sum = sum;
+    rounded_sum = other_half_sum(rounded_sum);
+    sum = other_half_sum(sum);
+    if constexpr (TEAM == 1) {
+        rounded_sum = over_waves<false>(rounded_sum, attention_lds);
+        sum = over_waves<false>(sum, attention_lds);
     }
+    delta += sum;
+#pragma unroll
+    for (int b = 0; b < Tl::DB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_fmaf(-rounded_sum, mean[b][i], acc[b][i]);
     if (there && h == 0 && (TEAM == 4 || wave == 0)) {
         a.delta[in_lse] = reference;
         a.delta[(long long)a.heads * a.query_rows + in_lse] = delta;
     }
-    store_own<T, D, TEAM>(acc, static_cast<T*>(a.grad_q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, a.scale,
-                          a.head_dim, attention_lds);
+    // (a row that sees one key has p = 1 and ds = 0, whatever the roundings made of it)
+    store_own<T, D, TEAM>(acc, static_cast<T*>(a.grad_q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there,
+                          own_limit == 1 ? 0.0f : a.scale, a.head_dim, attention_lds);
 }
 
 // ---- backward: gradients of keys and values -------------------------------------------------------------
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_kv_kernel(AttentionCall a) {
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<TEAM>();
+    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, true>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES, STAGE = 2 * BYTES + 2 * N * 4;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
@@ -746,6 +747,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
 
     // the rows that see a key are those from its start on
     auto start = [&](int j) { return a.causal ? max(j - (s.nk - s.nq), 0) : 0; };
+    const int lone = a.causal ? s.nq - s.nk : -1;  // the row that sees one key: p = 1 and ds = 0
     const int own_start = start(key), least = start(wave_first), most = start(wave_first + 31);
     const int begin = start(first) / N * N, turns = begin < s.nq ? (s.nq - begin + N - 1) / N : 0, all = turns * group;
     constexpr int STEP = TEAM == 1 ? kWaves : 1;
@@ -761,13 +763,15 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
             for (int i = 0; i < 16; ++i) dk[b][i] = dv[b][i] = 0.0f;
         // turn i: head i / turns of the group, rows from begin + N (i % turns) on
         typename Tl::template Stager<TEAM, A> queries, gradients;
+        float statistic = 0.0f;
         auto begin_tile = [&](int buf, int i) {
             const int head = kv * group + i / turns, t = begin + i % turns * N;
             char* const to = tiles_at + buf * STAGE;
             if (TEAM == 1 || wave < 2 * N / 64) {  // references, then deltas
-                const int i = TEAM == 1 ? lane : threadIdx.x, r = t + i % N;
-                const float* const from = a.delta + (i < N ? 0 : (long long)a.heads * a.query_rows) + (long long)head * a.query_rows + s.q0 + r;
-                issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), r < s.nq ? (const void*)from : (const void*)zero_piece);
+                const int at = TEAM == 1 ? lane : threadIdx.x, r = t + at % N;
+                const float* const from = a.delta + (at < N ? 0 : (long long)a.heads * a.query_rows) + (long long)head * a.query_rows + s.q0 + r;
+                if constexpr (Tl::P == 3) statistic = r < s.nq ? *from : 0.0f;
+                else issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), r < s.nq ? (const void*)from : (const void*)zero_piece);
             }
             queries.begin(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
             gradients.begin(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
@@ -775,6 +779,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
         };
         auto finish = [&](int buf) {
             char* const to = tiles_at + buf * STAGE;
+            if constexpr (Tl::P == 3)
+                if (TEAM == 1 || wave < 2 * N / 64) *reinterpret_cast<float*>(to + 2 * BYTES + (TEAM == 1 ? lane : threadIdx.x) * 4) = statistic;
             queries.template finish<decltype(careful)::value>(to);
             gradients.template finish<decltype(careful)::value>(to + BYTES);
         };
@@ -802,8 +808,10 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 auto sees = [&](int r) { return t + 32 * b + r >= own_start && t + 32 * b + r < s.nq; };
                 if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
+                    for (int e = 0; e < 16; ++e) {
                         if (!sees(block_row(e))) p[e] = dp[e] = 0.0f;
+                        if (t + 32 * b + block_row(e) == lone) dp[e] = 0.0f;
+                    }
                 }
                 if (decltype(careful)::value && masked) {
                     add_seen<T, D, N>(dv, ot, 32 * b, p, sees);
@@ -814,13 +822,13 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 }
             }
         };
-        over_tiles<STAGES, 1, TEAM>(mine, all, STEP, begin_tile, finish, use);
+        over_tiles<STAGES, Tl::P, TEAM>(mine, all, STEP, begin_tile, finish, use);
     };
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(dk) || any_not_finite(dv))) pass(std::true_type{});
     if constexpr (TEAM == 1) __syncthreads();
-    store_own<T, D, TEAM>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there, a.scale, a.head_dim,
-                          attention_lds);
+    store_own<T, D, TEAM>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there,
+                          s.nk == 1 ? 0.0f : a.scale, a.head_dim, attention_lds);
     store_own<T, D, TEAM>(dv, static_cast<T*>(a.grad_v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, 1.0f, a.head_dim,
                           attention_lds);
 }
@@ -875,7 +883,7 @@ hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
         return launch(attention_forward_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
-                      tiles_lds<T, D, TEAM>(0), s);
+                      tiles_lds<T, D, TEAM, false>(0), s);
     });
 }
 
@@ -889,7 +897,7 @@ hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStrea
             constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
             static std::atomic<unsigned long long> once{0};
             return launch(attention_grad_q_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
-                          tiles_lds<T, D, TEAM>(0), s);
+                          tiles_lds<T, D, TEAM, true>(0), s);
         });
     }
     if (e != hipSuccess || a.longest_keys == 0) return e;
@@ -899,7 +907,7 @@ hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStrea
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
         return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_keys + OWN - 1) / OWN, a.kv_heads,
-                      tiles_lds<T, D, TEAM>(8 * tile_rows<T, TEAM>()), s);
+                      tiles_lds<T, D, TEAM, true>(8 * tile_rows<T, TEAM>()), s);
     });
 }
 
