@@ -413,7 +413,8 @@ int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* h
  * sized by (a longer sequence counts as that long, and what lies outside the arrays is cut off).  With causal != 0 query r of a sequence sees its keys up to
  * r + key_count - query_count: the queries are the last of the keys, whose first may come from a cache.
  *   s_ij = scale q_i . k_j,   lse_i = log sum_j exp s_ij,   out_i = sum_j exp(s_ij - lse_i) v_j    over the keys that row i sees
- * A row that sees no key is zeros, its lse -inf.  What is not seen has no effect, whatever it holds.  scale is positive.  Two sequences may share keys
+ * A row that sees no key is zeros, its lse -inf.  What is not seen has no effect, whatever it holds; an infinity that is seen may come out as
+ * NaN (f32 rows are multiplied in parts).  scale is positive.  Two sequences may share keys
  * (forward only), not queries.
  *   out  [query_rows, heads, head_dim] without gaps      lse [heads, query_rows] f32 or NULL
  * Sums and statistics are f32 (f32 rows: their products too); bf16 rows round exp(s_ij - m) to bf16 for the product with v. */
@@ -455,7 +456,8 @@ int rbmoe_kv_cache_read(rbmoe_kv_cache* cache, int32_t rows, void* k, int32_t k_
  * tables[i][0 .. table_pages).  The new row's own key is written before, and counts.  Lengths go up to `longest` (longer ones are cut), by which a
  * launch is sized: a captured graph takes the longest that its replays will see.  A table entry that is no page of the cache has no rows; a
  * sequence without any gives zeros.  The handle holds the workspace for up to max_sequences sequences, joins parts of long sequences in
- * it, and serves any number of caches, one call after the other. */
+ * it, and serves any number of caches, one call after the other.  Where the parts end depends on all lengths of a call, and the last bits of its f32
+ * sums with it. */
 typedef struct rbmoe_decode rbmoe_decode;
 int rbmoe_decode_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t max_sequences,
                         rbmoe_decode** out);

@@ -63,11 +63,10 @@ __device__ __forceinline__ float other_half_sum(float v) {
 // ---- operands ------------------------------------------------------------------------------------
 // f32 rows as matrix operands: three bf16 parts of 8 bits each, cut off one behind the other, which add up to the value exactly.
 // Of the nine products of two values' parts the six largest are taken; the others are below 2^-22 of the product.
-// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  `guard`: an infinity has no rest, where inf - inf would make it NaN.
+// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  An infinity's rest is NaN, and so is what it goes into.
 struct Parts8 {
     bf16x8 part[3];
 };
-template <bool GUARD>
 __device__ __forceinline__ Parts8 cut8(const float (&x)[8]) {
     Parts8 r;
     float rest[8];
@@ -82,11 +81,7 @@ __device__ __forceinline__ Parts8 cut8(const float (&x)[8]) {
         r.part[n] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
         if (n == 2) break;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool stop = GUARD && n == 0 && fabsf(rest[i]) == __builtin_inff();
-            rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
-            if (stop) rest[i] = 0.0f;
-        }
+        for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
     }
     return r;
 }
@@ -102,7 +97,6 @@ struct Mma<bf16_t> {
     };
     static __device__ __forceinline__ bf16x8 part(const Rows& r, int) { return r; }
     static __device__ __forceinline__ bf16x8 part(const Cols& p, int k, int) { return p.c[k]; }
-    template <bool GUARD>
     static __device__ __forceinline__ Cols cols(const floatx16& p) {
         Cols r;
 #pragma unroll
@@ -140,13 +134,12 @@ struct Mma<float> {
     };
     static __device__ __forceinline__ bf16x8 part(const Rows& r, int i) { return r.part[i]; }
     static __device__ __forceinline__ bf16x8 part(const Cols& p, int k, int i) { return p.c[k].part[i]; }
-    template <bool GUARD>
     static __device__ __forceinline__ Cols cols(const floatx16& p) {
         Cols r;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const float x[8] = {p[8 * k], p[8 * k + 1], p[8 * k + 2], p[8 * k + 3], p[8 * k + 4], p[8 * k + 5], p[8 * k + 6], p[8 * k + 7]};
-            r.c[k] = cut8<GUARD>(x);
+            r.c[k] = cut8(x);
         }
         return r;
     }
@@ -218,14 +211,13 @@ struct Tile {
                 }
             }
         }
-        template <bool GUARD>
         __device__ __forceinline__ void finish(char* tile) {
             if constexpr (P == 3 || !A) {
 #pragma unroll
                 for (int i = 0; i < UNITS; ++i) {
                     char* const to = tile + (i * TEAM * 64 + (int)(threadIdx.x & (64 * TEAM - 1))) * 16;
                     if constexpr (P == 3) {
-                        const Parts8 parts = cut8<GUARD>(x[i]);
+                        const Parts8 parts = cut8(x[i]);
 #pragma unroll
                         for (int k = 0; k < 3; ++k) *reinterpret_cast<bf16x8*>(to + k * PART) = parts.part[k];
                     } else {
@@ -326,7 +318,7 @@ __device__ __forceinline__ void load_own(const T* __restrict__ row, bool there, 
         if constexpr (sizeof(T) == 4) {
             float x[8] = {};
             if (in) load8(row + (2 * kc + h) * 8, x);
-            own[kc] = cut8<true>(x);
+            own[kc] = cut8(x);
         } else {
             Any16 x = {0, 0, 0, 0};
             if (in) x = *reinterpret_cast<const Any16*>(row + (2 * kc + h) * 8);
@@ -526,8 +518,8 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
         };
         auto finish = [&](int buf) {
             char* const to = tiles_at + buf * 2 * BYTES;
-            keys.template finish<decltype(careful)::value>(to);
-            values.template finish<decltype(careful)::value>(to + BYTES);
+            keys.finish(to);
+            values.finish(to + BYTES);
         };
         auto use = [&](int buf, int t) {
             if (t >= most || wave_first >= s.nq) return;
@@ -574,7 +566,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
                 if (decltype(careful)::value && t + N > least)
                     add_seen<T, D, N>(acc, vt, 32 * b, p[b], [&](int r) { return t + 32 * b + r < own_limit; });
                 else
-                    Tl::add(acc, vt, 32 * b, Mma<T>::template cols<decltype(careful)::value>(p[b]));
+                    Tl::add(acc, vt, 32 * b, Mma<T>::cols(p[b]));
             }
         };
         over_tiles<STAGES, Tl::P, TEAM>(start, end, STEP, begin, finish, use);
@@ -665,8 +657,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
         };
         auto finish = [&](int buf) {
             char* const to = tiles_at + buf * 2 * BYTES;
-            keys.template finish<decltype(careful)::value>(to);
-            values.template finish<decltype(careful)::value>(to + BYTES);
+            keys.finish(to);
+            values.finish(to + BYTES);
         };
         auto use = [&](int buf, int t) {
             if (t >= most || wave_first >= s.nq) return;
@@ -685,7 +677,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                     for (int i = 0; i < 16; ++i)
                         if (t + 32 * b + block_row(i) >= own_limit) p[i] = dp[i] = 0.0f;
                 }
-                const auto ds = Mma<T>::template cols<decltype(careful)::value>(dp);
+                const auto ds = Mma<T>::cols(dp);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += dp[i];
                 if constexpr (sizeof(T) == 2) rounded_sum = Mma<T>::total(ds, rounded_sum);
@@ -695,7 +687,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                     add_seen<T, D, N>(mean, kt, 32 * b, p, sees);
                 } else {
                     Tl::add(acc, kt, 32 * b, ds);
-                    Tl::template add<bf16_t>(mean, kt, 32 * b, Mma<bf16_t>::cols<false>(p));
+                    Tl::template add<bf16_t>(mean, kt, 32 * b, Mma<bf16_t>::cols(p));
                 }
             }
         };
@@ -781,8 +773,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
             char* const to = tiles_at + buf * STAGE;
             if constexpr (Tl::P == 3)
                 if (TEAM == 1 || wave < 2 * N / 64) *reinterpret_cast<float*>(to + 2 * BYTES + (TEAM == 1 ? lane : threadIdx.x) * 4) = statistic;
-            queries.template finish<decltype(careful)::value>(to);
-            gradients.template finish<decltype(careful)::value>(to + BYTES);
+            queries.finish(to);
+            gradients.finish(to + BYTES);
         };
         auto use = [&](int buf, int i) {
             const int t = begin + i % turns * N;
@@ -817,8 +809,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                     add_seen<T, D, N>(dv, ot, 32 * b, p, sees);
                     add_seen<T, D, N>(dk, qt, 32 * b, dp, sees);
                 } else {
-                    Tl::add(dv, ot, 32 * b, Mma<T>::template cols<decltype(careful)::value>(p));
-                    Tl::add(dk, qt, 32 * b, Mma<T>::template cols<decltype(careful)::value>(dp));
+                    Tl::add(dv, ot, 32 * b, Mma<T>::cols(p));
+                    Tl::add(dk, qt, 32 * b, Mma<T>::cols(dp));
                 }
             }
         };
