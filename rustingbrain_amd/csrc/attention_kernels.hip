@@ -119,11 +119,9 @@ struct Mma<bf16_t> {
         return sum;
     }
     static __device__ __forceinline__ float rounded(float v) { return bf16_bits_to_f32(f32_to_bf16_bits(v)); }
-    // exp of a score by its factor `c`, less the reference: both times log2 e, for the base-2 exponential
+    // exp of x / `unit`: scores and references are kept times log2 e, for the base-2 exponential
     static constexpr float unit = kLog2e, natural = kLn2;
-    static __device__ __forceinline__ float exponential(float s, float c, float reference) {
-        return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -reference));
-    }
+    static __device__ __forceinline__ float exponential(float x) { return __builtin_amdgcn_exp2f(x); }
 };
 template <>
 struct Mma<float> {
@@ -146,9 +144,7 @@ struct Mma<float> {
     static __device__ __forceinline__ float rounded(float v) { return v; }
     // (the factor is the caller's scale as it is, and only the difference is rounded with log2 e)
     static constexpr float unit = 1.0f, natural = 1.0f;
-    static __device__ __forceinline__ float exponential(float s, float c, float reference) {
-        return __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -reference) * kLog2e);
-    }
+    static __device__ __forceinline__ float exponential(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 };
 template <typename T>
 using RowsOf = typename Mma<T>::Rows;
@@ -473,7 +469,7 @@ __device__ __forceinline__ void over_tiles(int start, int end, int step, B begin
 // ---- forward ----------------------------------------------------------------------------------------
 
 template <typename T, int D, int TEAM, bool A>
-__global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 && TEAM == 1) ? 1 : 2) void attention_forward_kernel(AttentionCall a) {
+__global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 && TEAM == 1) ? 1 : D * sizeof(T) == 128 ? 3 : 2) void attention_forward_kernel(AttentionCall a) {
     constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, false>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
@@ -535,29 +531,37 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
                     for (int i = 0; i < 16; ++i)
                         if (t + 32 * b + block_row(i) >= own_limit) p[b][i] = -__builtin_inff();
             }
-            float top = p[0][0];
+            // The exponents' arguments by the reference that there is: it moves only when a score passes it by 2^8.  The results are
+            // the same, sums and accumulators have room for it, and after a few tiles nothing has to be scaled.
+            const float reference = m == -__builtin_inff() ? 0.0f : m;
+            float top = -__builtin_inff();
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, p[b][i]);
-            top = other_half_max(top) * c;
-            // The reference of the exponents moves only when a score passes it by 2^8: the results are the same, sums and accumulators
-            // have room for it, and after a few tiles nothing has to be scaled.
-            if (__any(top > m + 8.0f)) {
-                const float next = fmaxf(m, top), down = next == m ? 1.0f : Mma<T>::exponential(1.0f, m, next);
+                for (int i = 0; i < 16; ++i) {
+                    p[b][i] = __builtin_fmaf(p[b][i], c, -reference);
+                    top = fmaxf(top, p[b][i]);
+                }
+            if (__any(top > (m == -__builtin_inff() ? m : 8.0f))) {
+                top = other_half_max(top);
+                const float next = top > (m == -__builtin_inff() ? m : 0.0f) ? reference + top : m;
+                const float down = next == m ? 1.0f : Mma<T>::exponential(m - next), shift = next == m ? 0.0f : next - reference;
                 m = next;
                 l *= down;
 #pragma unroll
                 for (int b = 0; b < Tl::DB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[b][i] *= down;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[b][i] -= shift;
             }
-            const float reference = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[b][i] = Mma<T>::exponential(p[b][i], c, reference);
+                    p[b][i] = Mma<T>::exponential(p[b][i]);
                     l += p[b][i];
                 }
             }
@@ -577,7 +581,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
     l = other_half_sum(l);
     if constexpr (TEAM == 1) {  // to one reference
         __syncthreads();
-        const float all = over_waves<true>(m, attention_lds), down = m == all ? 1.0f : Mma<T>::exponential(1.0f, m, all);
+        const float all = over_waves<true>(m, attention_lds), down = m == all ? 1.0f : Mma<T>::exponential(m - all);
         m = all;
         l = over_waves<false>(l * down, attention_lds);
 #pragma unroll
@@ -669,7 +673,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 floatx16 p = Tl::product(kt, 32 * b, q), dp = Tl::product(vt, 32 * b, dout);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[i] = Mma<T>::exponential(p[i], c, reference);
+                    p[i] = Mma<T>::exponential(__builtin_fmaf(p[i], c, -reference));
                     dp[i] = p[i] * (dp[i] - delta);
                 }
                 if (t + N > least) {
@@ -793,7 +797,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                     const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        p[4 * e + j] = Mma<T>::exponential(p[4 * e + j], c, xs[j]);
+                        p[4 * e + j] = Mma<T>::exponential(__builtin_fmaf(p[4 * e + j], c, -xs[j]));
                         dp[4 * e + j] = p[4 * e + j] * (dp[4 * e + j] - ys[j]);
                     }
                 }
