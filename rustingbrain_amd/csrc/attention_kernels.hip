@@ -420,9 +420,11 @@ __device__ __forceinline__ Place place_of(int heads, int sequences, int tiles, b
 
 // How a workgroup's four waves share the work.  TEAM 4: each owns 32 rows, the tiles are common.  TEAM 1: all own the same 32 rows, each takes every
 // fourth tile, stages it for itself, and their sums are added at the end: four times the workgroups, for calls that have few.
-template <typename T, int TEAM>
+// A tile has 64 rows where the rest leaves registers for two blocks' operands on their way, 32 otherwise (grad_q, 8 sequences up to 2048 rows, 8 heads of
+// 64: 60 us by 32, 77 by 64; 8192 rows, 16 heads of 128: 700 and 650).
+template <typename T, int D, int TEAM, bool GRAD_Q = false>
 constexpr int tile_rows() {
-    return sizeof(T) == 2 && TEAM == 4 ? 64 : 32;
+    return sizeof(T) == 2 && TEAM == 4 && !(GRAD_Q && D == 64) ? 64 : 32;
 }
 // Stages of tiles.  TEAM 4: two, one is filled while the other is used.  TEAM 1: one, where workgroups beside this one on its compute unit are busy
 // meanwhile, or the next tile waits in registers; two for kernels whose registers leave room for one workgroup (ALONE).
@@ -430,9 +432,9 @@ template <typename T, int D, int TEAM, bool ALONE>
 constexpr int tile_stages() {
     return TEAM == 4 || (ALONE && sizeof(T) == 2 && D == 128) ? 2 : 1;
 }
-template <typename T, int D, int TEAM, bool ALONE>
-constexpr int tiles_lds(int extra) {  // of two tiles and `extra` bytes a stage
-    return (kWaves / TEAM) * tile_stages<T, D, TEAM, ALONE>() * (2 * Tile<T, D, tile_rows<T, TEAM>()>::BYTES + extra);
+template <typename T, int D, int TEAM, int N, bool ALONE>
+constexpr int tiles_lds(int extra) {  // of two tiles of N rows and `extra` bytes a stage
+    return (kWaves / TEAM) * tile_stages<T, D, TEAM, ALONE>() * (2 * Tile<T, D, N>::BYTES + extra);
 }
 __device__ __forceinline__ void wait_for_tile(bool common) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's part of the tile has landed, its reads of the other stage are done
@@ -470,7 +472,7 @@ __device__ __forceinline__ void over_tiles(int start, int end, int step, B begin
 
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 && TEAM == 1) ? 1 : D * sizeof(T) == 128 ? 3 : 2) void attention_forward_kernel(AttentionCall a) {
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, false>();
+    constexpr int N = tile_rows<T, D, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, false>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of keys and values
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
 // ---- backward: gradients of the queries ------------------------------------------------------------------
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_q_kernel(AttentionCall a) {
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, true>();
+    constexpr int N = tile_rows<T, D, TEAM, true>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, true>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
@@ -724,7 +726,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
 // ---- backward: gradients of keys and values -------------------------------------------------------------
 template <typename T, int D, int TEAM, bool A>
 __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void attention_grad_kv_kernel(AttentionCall a) {
-    constexpr int N = tile_rows<T, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, true>();
+    constexpr int N = tile_rows<T, D, TEAM>(), NB = N / 32, OWN = 32 * TEAM, STAGES = tile_stages<T, D, TEAM, true>();
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES, STAGE = 2 * BYTES + 2 * N * 4;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
@@ -879,7 +881,7 @@ hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
         return launch(attention_forward_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
-                      tiles_lds<T, D, TEAM, false>(0), s);
+                      tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM>(), false>(0), s);
     });
 }
 
@@ -893,7 +895,7 @@ hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStrea
             constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
             static std::atomic<unsigned long long> once{0};
             return launch(attention_grad_q_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
-                          tiles_lds<T, D, TEAM, true>(0), s);
+                          tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM, true>(), true>(0), s);
         });
     }
     if (e != hipSuccess || a.longest_keys == 0) return e;
@@ -903,7 +905,7 @@ hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStrea
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
         return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_keys + OWN - 1) / OWN, a.kv_heads,
-                      tiles_lds<T, D, TEAM, true>(8 * tile_rows<T, TEAM>()), s);
+                      tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM>(), true>(8 * tile_rows<T, D, TEAM>()), s);
     });
 }
 

@@ -46,41 +46,34 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 __device__ __forceinline__ void store8(bf16_t* p, const float (&v)[8]) {
     *reinterpret_cast<Any16*>(p) = Any16{pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7])};
 }
-__device__ __forceinline__ void store8(int8_t* p, const float (&v)[8]) {
-    uint32_t w[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        w[i] = ((uint32_t)(int)v[4 * i] & 255) | ((uint32_t)(int)v[4 * i + 1] & 255) << 8 | ((uint32_t)(int)v[4 * i + 2] & 255) << 16 |
-               (uint32_t)(int)v[4 * i + 3] << 24;
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-}
-
-template <typename C>
-__device__ __forceinline__ C stored_as(float v) {
-    if constexpr (sizeof(C) == 1) return (int8_t)(int)v;
-    else return from_f32<C>(v);
-}
-
-// The 8 values of each of a row's TR threads, rounded to whole numbers of the returned scale.
+// The 8 values of each of a row's TR threads as bytes, and the scale.  The quotient 127 x / a is rounded as a division would: its approximation by the
+// reciprocal is mended by the remainder (Markstein's method: with the correctly rounded reciprocal one step gives the correctly rounded
+// quotient), 4 operations where a division takes ten; adding 1.5 * 2^23 rounds to a whole number, ties to even, and leaves it in the low bits.
 template <int TR>
-__device__ __forceinline__ float quantize(float (&v)[8]) {
-    float most = 0.0f;
-    bool bad = false;
+__device__ __forceinline__ float quantize(const float (&v)[8], uint2& bytes) {
+    uint32_t top = 0;  // of the magnitudes' bits: NaN come out above infinities
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        most = fmaxf(most, fabsf(v[i]));
-        bad |= !(fabsf(v[i]) < __builtin_inff());
+        const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
+        top = u > top ? u : top;
     }
-    // (a mark that the maximum hands on: infinities come out of it anyway)
-    most = group_fmax(bad ? __builtin_inff() : most, TR);
-    if (!(most < __builtin_inff())) {
+    top = group_umax(top, TR);
+    bytes = make_uint2(0, 0);
+    if (top >= 0x7f800000u) return __builtin_nanf("");
+    const float most = __uint_as_float(top);
+    if (top == 0) return 0.0f;
+    const float factor = most > 0x1p100f ? 0x1p-20f : most < 0x1p-100f ? 0x1p60f : 1.0f;  // 127 x and 1 / a stay in range
+    const float a = most * factor, r = __fdiv_rn(1.0f, a), n = 127.0f * factor;
+    uint32_t q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        return __builtin_nanf("");
+    for (int i = 0; i < 8; ++i) {
+        const float x = n * v[i], y = x * r;
+        q[i] = __float_as_uint(__builtin_fmaf(__builtin_fmaf(-y, a, x), r, y) + 12582912.0f);
     }
-    const float small = most > 0x1p100f ? 0x1p-20f : 1.0f;  // 127 x stays in range
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = most > 0.0f ? rintf(__fdiv_rn(__fmul_rn(127.0f, v[i] * small), most * small)) : 0.0f;
+    auto join = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400), __builtin_amdgcn_perm(b, a, 0x0c0c0400), 0x05040100);
+    };
+    bytes = make_uint2(join(q[0], q[1], q[2], q[3]), join(q[4], q[5], q[6], q[7]));
     return __fdiv_rn(most, 127.0f);
 }
 
@@ -100,7 +93,7 @@ __device__ __forceinline__ int run_from(uint64_t next, int r) {
 template <typename T, typename C, int W>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
     constexpr int R = cache_rows<W>(), TR = W / 8, G = 16 / sizeof(C);
-    __shared__ C values[R][W + 16 / sizeof(C)];
+    __shared__ __attribute__((aligned(16))) C values[R][W + 16 / sizeof(C)];
     __shared__ long long places[R];
     __shared__ uint64_t neighbours;
     const CachePool& p = a.pool;
@@ -130,21 +123,42 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
         }
         unsigned char* const block = cache_block(p, at >= 0 ? at >> p.page_shift : 0, head);
         const int row = (int)(at & page_mask);
+        union Stored {  // the 8 values as the cache holds them
+            uint2 bytes;
+            uint4 words[sizeof(C) == 4 ? 2 : 1];
+            C c[8];
+        } ks, vs;
         if constexpr (sizeof(C) == 1) {
-            const float k_scale = quantize<TR>(k), v_scale = quantize<TR>(v);
+            const float k_scale = quantize<TR>(k, ks.bytes), v_scale = quantize<TR>(v, vs.bytes);
             if (at >= 0 && tid % TR == 0) {
                 float* const scales = reinterpret_cast<float*>(block + 2 * p.half_bytes());
                 scales[row] = k_scale;
                 scales[(1 << p.page_shift) + row] = v_scale;
             }
         }
-        if (at >= 0) store8(reinterpret_cast<C*>(block) + (size_t)row * W + c, k);
+        if constexpr (sizeof(C) == 2) {
+            ks.words[0] = make_uint4(pack2(k[0], k[1]), pack2(k[2], k[3]), pack2(k[4], k[5]), pack2(k[6], k[7]));
+            vs.words[0] = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+        } else if constexpr (sizeof(C) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ks.c[j] = k[j];
+                vs.c[j] = v[j];
+            }
+        }
+        auto put = [](C* to, const Stored& x) {  // (16-byte boundaries, or 8 for bytes)
+            if constexpr (sizeof(C) == 1) *reinterpret_cast<uint2*>(to) = x.bytes;
+            else
+#pragma unroll
+                for (size_t j = 0; j < sizeof(C) / 2; ++j) reinterpret_cast<uint4*>(to)[j] = x.words[j];
+        };
+        if (at >= 0) put(reinterpret_cast<C*>(block) + (size_t)row * W + c, ks);
         if (!scattered) {
-            store8(&values[r][c], v);
+            put(&values[r][c], vs);
         } else if (at >= 0) {
             C* const to = reinterpret_cast<C*>(block + p.half_bytes()) + value_at<W, G>(row, c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) to[j * G] = stored_as<C>(v[j]);
+            for (int j = 0; j < 8; ++j) to[j * G] = vs.c[j];
         }
     }
     if (scattered) return;
@@ -200,7 +214,7 @@ __device__ __forceinline__ void widen8(const int8_t* p, float (&v)[8]) {
 template <typename T, typename C, int W>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheRows a) {
     constexpr int R = cache_rows<W>(), TR = W / 8, G = 16 / sizeof(C);
-    __shared__ C values[R][W + 16 / sizeof(C)];
+    __shared__ __attribute__((aligned(16))) C values[R][W + 16 / sizeof(C)];
     __shared__ long long places[R];
     __shared__ uint64_t neighbours;
     const CachePool& p = a.pool;
