@@ -419,7 +419,8 @@ int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* h
  *   out  [query_rows, heads, head_dim] without gaps      lse [heads, query_rows] f32 or NULL
  * Sums and statistics are f32 (f32 rows: their products too); bf16 rows round exp(s_ij - m) to bf16 for the product with v. */
 typedef struct rbmoe_attention rbmoe_attention;
-/* backward_rows: the most query rows of a backward pass (0: forward only), 8 bytes a row and head, counted against the budget. */
+/* backward_rows: the most query rows of a backward pass (0: forward only): 8 bytes a row and head, and for the first 16384 / kv_heads rows of
+ * heads in groups 8 * head_dim bytes a row and head more, counted against the budget. */
 int rbmoe_attention_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t backward_rows,
                            rbmoe_attention** out);
 void rbmoe_attention_destroy(rbmoe_attention* attention);

@@ -14,8 +14,9 @@ using namespace rbmoe;
 struct rbmoe_attention {
     rbmoe_ctx* ctx = nullptr;
     int heads = 0, kv_heads = 0, head_dim = 0, dtype = 0, backward_rows = 0;
-    void* delta = nullptr;
-    size_t delta_bytes = 0;
+    void* workspace = nullptr;  // references and deltas of rows, then sums of shares
+    size_t bytes = 0, parts_at = 0;
+    int part_rows = 0;
 };
 
 struct rbmoe_kv_cache {
@@ -116,9 +117,11 @@ int rbmoe_attention_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int3
     a->head_dim = head_dim;
     a->dtype = dtype;
     a->backward_rows = backward_rows;
-    a->delta_bytes = (size_t)backward_rows * heads * 8;
-    if (a->delta_bytes)
-        if (const int rc = ctx_alloc(ctx, a->delta_bytes, "the backward pass's row sums", &a->delta)) {
+    a->part_rows = attention_part_rows(backward_rows, kv_heads, heads / kv_heads);
+    a->parts_at = ((size_t)backward_rows * heads * 8 + 15) / 16 * 16;
+    a->bytes = a->parts_at + (size_t)a->part_rows * (heads / kv_heads) * 2 * head_dim * 4;
+    if (a->bytes)
+        if (const int rc = ctx_alloc(ctx, a->bytes, "the backward pass's sums", &a->workspace)) {
             delete a;
             return rc;
         }
@@ -130,7 +133,7 @@ int rbmoe_attention_create(rbmoe_ctx* ctx, int32_t heads, int32_t kv_heads, int3
 void rbmoe_attention_destroy(rbmoe_attention* a) {
     if (!a) return;
     (void)hipStreamSynchronize(a->ctx->stream);
-    ctx_free(a->ctx, a->delta, a->delta_bytes);
+    ctx_free(a->ctx, a->workspace, a->bytes);
     ctx_release(a->ctx);
     delete a;
 }
@@ -196,7 +199,9 @@ int rbmoe_attention_backward(rbmoe_attention* at, int32_t sequences, int32_t lon
     a.grad_q = grad_q;
     a.grad_k = grad_k;
     a.grad_v = grad_v;
-    a.delta = static_cast<float*>(at->delta);
+    a.delta = static_cast<float*>(at->workspace);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(at->workspace) + at->parts_at);
+    a.part_rows = at->part_rows;
     HIP_TRY(ctx, launch_attention_backward(a, at->dtype == RBMOE_BF16, ctx->stream));
     return RBMOE_OK;
 }

@@ -35,7 +35,12 @@ struct AttentionCall {
     void* grad_k;
     void* grad_v;
     float* delta;  // [2][heads, query_rows], references of the exponents and deltas: written by the queries' gradients, read by the keys'
+    float* parts;  // [shares][key_rows, kv_heads][2][head_dim]: sums of dk and dv over a share of a group's heads
+    int part_rows; // room for so many rows of a share
+    int shares;    // set by the launch
 };
+// rows of f32 sums [2][head_dim], for every head of a group, that the backward pass of up to so many rows may share out
+int attention_part_rows(int backward_rows, int kv_heads, int group);
 hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream_t s);
 hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStream_t s);
 

@@ -731,9 +731,10 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     constexpr int BYTES = Tl::BYTES, STAGE = 2 * BYTES + 2 * N * 4;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
     const int tiles = (a.longest_keys + OWN - 1) / OWN;
-    const Place at = place_of(a.kv_heads, a.sequences, tiles, false);
+    const Place at = place_of(a.kv_heads * a.shares, a.sequences, tiles, false);
     const Sequence s = sequence_of(a, at.sequence);
-    const int first = at.tile * OWN, kv = at.head, group = a.heads / a.kv_heads;
+    const int first = at.tile * OWN, kv = at.head / a.shares, share = at.head % a.shares;
+    const int group = a.heads / a.kv_heads / a.shares, head0 = at.head * group;  // the heads of this share of the group
     if (first >= s.nk) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int pieces = a.head_dim / 8;
@@ -763,7 +764,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
         typename Tl::template Stager<TEAM, A> queries, gradients;
         float statistic = 0.0f;
         auto begin_tile = [&](int buf, int i) {
-            const int head = kv * group + i / turns, t = begin + i % turns * N;
+            const int head = head0 + i / turns, t = begin + i % turns * N;
             char* const to = tiles_at + buf * STAGE;
             if (TEAM == 1 || wave < 2 * N / 64) {  // references, then deltas
                 const int at = TEAM == 1 ? lane : threadIdx.x, r = t + at % N;
@@ -825,10 +826,36 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     pass(std::false_type{});
     if (__syncthreads_or(any_not_finite(dk) || any_not_finite(dv))) pass(std::true_type{});
     if constexpr (TEAM == 1) __syncthreads();
-    store_own<T, D, TEAM>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there,
-                          s.nk == 1 ? 0.0f : a.scale, a.head_dim, attention_lds);
-    store_own<T, D, TEAM>(dv, static_cast<T*>(a.grad_v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, 1.0f, a.head_dim,
-                          attention_lds);
+    const float factor = s.nk == 1 ? 0.0f : 1.0f;
+    if (a.shares == 1) {
+        store_own<T, D, TEAM>(dk, static_cast<T*>(a.grad_k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there, factor * a.scale,
+                              a.head_dim, attention_lds);
+        store_own<T, D, TEAM>(dv, static_cast<T*>(a.grad_v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, 1.0f, a.head_dim,
+                              attention_lds);
+    } else {
+        float* const part = a.parts + (((long long)share * a.key_rows + s.k0 + key) * a.kv_heads + kv) * 2 * a.head_dim;
+        store_own<float, D, TEAM>(dk, part, there, factor, a.head_dim, attention_lds);
+        store_own<float, D, TEAM>(dv, part + a.head_dim, there, 1.0f, a.head_dim, attention_lds);
+    }
+}
+
+// The shares' sums, in their order; four elements a thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attention_add_shares_kernel(AttentionCall a) {
+    const Sequence s = sequence_of(a, blockIdx.y);
+    const int quads = a.head_dim / 4, i = blockIdx.x * kThreads + threadIdx.x;
+    const int d = i % quads * 4, kv = i / quads % a.kv_heads, row = i / quads / a.kv_heads;
+    if (row >= s.nk) return;
+    const float* part = a.parts + ((long long)(s.k0 + row) * a.kv_heads + kv) * 2 * a.head_dim + d;
+    float k[4] = {}, v[4] = {};
+    for (int n = 0; n < a.shares; ++n, part += (long long)a.key_rows * a.kv_heads * 2 * a.head_dim)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            k[j] += part[j];
+            v[j] += part[a.head_dim + j];
+        }
+    store4(static_cast<T*>(a.grad_k) + (long long)(s.k0 + row) * a.k_stride + (long long)kv * a.head_dim + d, k[0] * a.scale, k[1] * a.scale, k[2] * a.scale, k[3] * a.scale);
+    store4(static_cast<T*>(a.grad_v) + (long long)(s.k0 + row) * a.v_stride + (long long)kv * a.head_dim + d, v[0], v[1], v[2], v[3]);
 }
 
 bool whole_pieces(const void* p, long long stride, int size) {
@@ -854,10 +881,13 @@ hipError_t with_kernel(bool bf16, int head_dim, bool few, bool aligned, F f) {
     return bf16 ? width(bf16_t{}) : width(float{});
 }
 
-#ifndef RBMOE_ATTENTION_FEW
-#define RBMOE_ATTENTION_FEW 512
-#endif
-constexpr int kFew = RBMOE_ATTENTION_FEW;
+// Workgroups of 128 rows below which 32 rows make one.  Two of them fill a compute unit, so 512 fill the device.  us with teams of 1 / 4: 5 bf16 prompts
+// behind 4000 keys, 32 heads of 128 (800 workgroups) 188 / 147; keys' gradients of 8 sequences up to 2048 rows, 2 kv heads of 64 (256) 92 / 190.
+constexpr int kFew = 512;
+// Workgroups of 32 keys below which a group's heads get their own.  us with / without: 2 x 2048 rows, 8 heads of 64, bf16 (256 workgroups) 74 / 100, 4 x 1024
+// f32 175 / 200, 8 x 512 bf16 (256, short ones) 44 / 41; 512 rows, 32 heads of 128 (128) 56 / 55, 1024 (256) 124 / 112: heads of 128 leave room
+// for one workgroup a unit.
+constexpr int kShared = 512;
 // Whether a launch over `longest` rows of `heads` heads a sequence would have few workgroups of 128 rows.
 bool few_workgroups(const AttentionCall& a, int longest, int heads) { return (long long)((longest + 127) / 128) * heads * a.sequences < kFew; }
 
@@ -899,14 +929,29 @@ hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStrea
         });
     }
     if (e != hipSuccess || a.longest_keys == 0) return e;
+    // A kv head's workgroups go through all heads of its group.  Where they are few, each head gets workgroups of its own, and their sums are added.
+    AttentionCall b = a;
+    const int group = a.heads / a.kv_heads;
+    const long long blocks = (long long)((a.longest_keys + 31) / 32) * a.kv_heads * a.sequences;
+    const bool few = few_workgroups(a, a.longest_keys, a.kv_heads);
+    b.shares = few && group > 1 && blocks < (a.head_dim <= 64 ? kShared : kShared / 2) && (long long)a.key_rows * a.kv_heads <= a.part_rows ? group : 1;
     const bool aligned = whole_pieces(a.q, a.q_stride, size) && whole_pieces(a.grad_out, a.head_dim, size);
-    return with_kernel(bf16, a.head_dim, few_workgroups(a, a.longest_keys, a.kv_heads), aligned, [&](auto type, auto width, auto team, auto whole) {
+    e = with_kernel(bf16, a.head_dim, few, aligned, [&](auto type, auto width, auto team, auto whole) {
         typedef decltype(type) T;
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
-        return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_keys + OWN - 1) / OWN, a.kv_heads,
+        return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, b, (a.longest_keys + OWN - 1) / OWN, a.kv_heads * b.shares,
                       tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM>(), true>(8 * tile_rows<T, D, TEAM>()), s);
     });
+    if (e != hipSuccess || b.shares == 1) return e;
+    const dim3 grid((unsigned)(((long long)a.longest_keys * a.kv_heads * a.head_dim / 4 + kThreads - 1) / kThreads), a.sequences);
+    if (bf16) hipLaunchKernelGGL(attention_add_shares_kernel<bf16_t>, grid, dim3(kThreads), 0, s, b);
+    else hipLaunchKernelGGL(attention_add_shares_kernel<float>, grid, dim3(kThreads), 0, s, b);
+    return hipGetLastError();
+}
+
+int attention_part_rows(int backward_rows, int kv_heads, int group) {
+    return group == 1 ? 0 : (int)std::min<long long>((long long)backward_rows * kv_heads, kShared * 32);
 }
 
 }  // namespace rbmoe
