@@ -4,9 +4,10 @@
  * Drop-in boundary for RustingBrain's `MoeLayer`: the forward pass with the two
  * auxiliary losses (reference src/moe.rs:203-341), the backward pass
  * (src/moe.rs:348-489) and the block's RMSNorm and residual add either side of
- * the layer (src/transformer_block.rs:216-222, 257-263); and, on their own, two
- * operators of a training step around it: a sub-layer joined to the residual
- * stream, and orthogonalised weight updates.  The reference
+ * the layer (src/transformer_block.rs:216-222, 257-263); and, on their own,
+ * operators of a training or serving step around it: a sub-layer joined to the
+ * residual stream, orthogonalised weight updates, and the attention half of a
+ * block with a paged cache of keys and values.  The reference
  * has no FFI seam for this layer; each entry point below names the reference
  * interface it stands in for, so that a Rust `extern "C"` block can bind them
  * one to one.  Plain pointers and sizes only.  Every function returns an

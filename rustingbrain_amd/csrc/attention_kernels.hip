@@ -5,18 +5,29 @@
 //   backward, delta_i = dout_i . out_i:   dp_ij = dout_i . v_j,  ds_ij = p_ij (dp_ij - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij dout_i   (sums over the heads of a group too)
 //
-// All five products run on the matrix cores in blocks of 32 x 32 with f32 accumulators: bf16 rows 16 reduction elements an
-// instruction, f32 rows 2 (exact f32 products and sums).  A wave owns 32 rows (forward, dq) or 32 keys (dk, dv) and keeps
-// them as the instruction's B operand; the other side goes through LDS in tiles that a workgroup's four waves share.  A product of two
-// row arrays comes out with the lane's own row in its column and the tile's rows in its registers, in the order in which the next
-// product takes them as its B operand: scores never leave registers, and no lane hands a value to another except the row statistics.
-// The second product needs the tile with rows and columns exchanged, which the transposing LDS read gives (bf16), or a read
-// along the row (f32).  p and ds are rounded to bf16 for bf16 rows (the matrix cores take bf16 operands): 2^-9 a term at random, no more
-// than the rounding of the result itself; their sums, the running maximum and sum of the softmax and all accumulators are f32.
+// All products run on the matrix cores in blocks of 32 x 32 x 16 with f32 accumulators: bf16 rows as they are, f32 rows as three bf16 parts.
+// A wave owns 32 rows (forward, dq) or 32 keys (dk, dv) and keeps them as the instruction's B operand; the other side goes through LDS in
+// tiles, loaded ahead.  A product of two row arrays comes out with the lane's own row in its column and the tile's rows in its registers,
+// in the order in which the next product takes them as its B operand: scores never leave registers, and no lane hands a value to another
+// except the row statistics.  The second product needs the tile with rows and columns exchanged, which the transposing LDS read gives.  For
+// bf16 rows p and ds are rounded to bf16 (the matrix cores take bf16 operands): half a step a term at random, no more than the rounding of the result
+// itself; their sums, the running maximum and sum of the softmax and all accumulators are f32.
+//
+// The backward pass takes ds = p (dp - delta) twice, from the queries' side and from the keys', instead of adding one side's sums in
+// memory: eight products where five would do, but the same bits from the same call, and no f32 gradients that pass through memory.
 //
 // Masked places: a masked score is replaced behind the product, whatever it was.  A masked p of zero times an infinity or NaN
 // in the tile would still be NaN, so a workgroup that ends with such a value goes over its tiles again and adds the blocks
 // on the diagonal row by row; nothing else is read twice.
+//
+// What bounds them (a large bf16 product by the library reaches 1370 TFLOP/s, an f32 one 153):
+//   forward, 16384 rows, 16 heads of 128, bf16, causal: 1.14 ms, 965 TFLOP/s.  A wave reads every tile from LDS whole, which takes as many cycles
+//     of the LDS as the products take of the matrix cores; both are busy seven cycles of ten.
+//   heads of 64 (8 x 2048 rows, 8 heads): 52 us, 660 TFLOP/s: a block has half the products and as many exponentials, which take
+//     as long as they do; three workgroups a unit instead of two give 8 %.
+//   backward, 8192 rows, 16 heads of 128, bf16: 0.65 ms (dq, with its fourth product) and 0.77 (dk, dv), 840 and 710 TFLOP/s of the products taken:
+//     registers leave one wave a SIMD, which waits for its exponentials.
+//   short or ragged calls: the longest rows' workgroups; f32 rows: 6 products for one, and cutting p and ds in parts.
 #include "attention_kernels.h"
 
 #include <algorithm>

@@ -3,6 +3,10 @@
 // int8 rows have a scale each (per token and head): a = max |x|, scale = a / 127, stored round(127 x / a), ties to even, read back as
 // stored * scale.  (127 x is exact for bf16 rows, so one division decides the rounding, and ties are ties.)  A row with an
 // infinity or NaN reads back as NaN whole.
+//
+// All of it is bound by memory (a large copy moves 4.9 TB/s): 23165 bf16 rows of 8 x 128 to 8 bits and back 57 us, 5.0 TB/s; new rows over 4 x 131072 cached
+// ones, bf16, 8 kv heads of 128, 198 us, 5.4 TB/s; over 64 sequences up to 8192 rows in 8 bits 122 us, 4.0 TB/s (widening bytes to
+// bf16 keeps the vector units busy a third of the time, pages of 16 rows come in pieces of 2 KB).  Small calls: launches of 3 to 6 us.
 #include "kv_cache_kernels.h"
 
 #include <algorithm>
@@ -324,13 +328,13 @@ hipError_t launch_cache_read(const CacheRows& a, bool bf16_rows, hipStream_t s) 
 
 // ---- decode -------------------------------------------------------------------------------------------
 //
-// A workgroup takes the heads of one group (up to 16) of one sequence over a part of its keys; its four waves take tiles of
-// keys in turn and load them straight into registers in operand order, a tile ahead.  Both products run on the matrix cores: a block
-// of 16 keys times the heads' rows (unused columns are zeros: there is nothing else for them to do, the loads decide), then the values' columns times
-// the scores.  A tile has four groups of g = 16 / element bytes neighbouring keys, one a row of 16 lanes: key g (m / 4) + 4 b + m % 4 of the
+// A workgroup takes the heads of one group (up to 16) of one sequence over a part of its keys; its waves take tiles of
+// keys in turn and load them straight into registers in operand order.  Both products run on the matrix cores: a block
+// of 16 keys times the heads' rows (unused columns are zeros: the matrix cores have nothing else to do, the loads decide), then the values' columns
+// times the scores.  A tile has four groups of g = 16 / element bytes neighbouring keys, one a row of 16 lanes: key g (m / 4) + 4 b + m % 4 of the
 // tile is row m of its block b, so that a lane's scores belong to the g keys whose values it loads as one piece.
 // Products of bf16 operands: bf16 and int8 values are such exactly; f32 rows over int8 are cut into three bf16 parts, p (times the
-// value's scale) into two for bf16 rows and three for f32 rows.  An f32 cache takes the f32 instruction.
+// value's scale) into two for bf16 rows and three for f32 rows: they cost nothing here.  An f32 cache takes the f32 instruction.
 template <int N>
 __device__ __forceinline__ void cut(const float (&x)[8], bf16x8 (&part)[N]) {
     float rest[8];
@@ -374,9 +378,6 @@ __device__ __forceinline__ float over_rows_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-#ifndef RBMOE_DECODE_OCC
-#define RBMOE_DECODE_OCC 2
-#endif
 // Waves of a workgroup: 4, or as many as registers allow where a call is so small that one workgroup a group of heads takes all of its keys (no
 // parts, no second launch).
 template <typename C, int W>
@@ -401,7 +402,7 @@ __device__ __forceinline__ int sequence_tiles(const DecodeCall& a, int i, int ke
 __device__ __forceinline__ long long range_start(long long tiles, int i, int n) { return tiles * i / n; }
 
 template <typename T, typename C, int W, int NW, bool STREAM>
-__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : RBMOE_DECODE_OCC) void decode_attention_kernel(DecodeCall a) {
+__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void decode_attention_kernel(DecodeCall a) {
     typedef Decode<T, C, W> X;
     constexpr int G = X::G, KT = X::KT, NB = X::NB, KP = X::KP, VP = X::VP;
     __shared__ float joined[NW][16][W + 4];
@@ -414,248 +415,248 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : RBMOE_DECODE_OCC) void deco
 
     // the tiles `from` to `to` of a sequence; `part`: where they go if they are not all of it, or -1
     auto work = [&](const int sequence, const int from, const int to, const long long part) {
-    const int length = sequence_length(a, sequence);
-    const int32_t* const table = a.tables + (long long)sequence * a.table_pages;
+        const int length = sequence_length(a, sequence);
+        const int32_t* const table = a.tables + (long long)sequence * a.table_pages;
 
-    // the heads' rows as B operand: lane l holds head l % 16
-    float q[W / 4];
-    bf16x8 qb[sizeof(C) == 4 ? 1 : W / 32][X::QP];
-    {
-        const T* const row = static_cast<const T*>(a.q) + (long long)sequence * a.q_stride + (long long)(head0 + m16) * p.head_dim;
-        const bool there = m16 < heads;
-        if constexpr (sizeof(C) == 4) {
+        // the heads' rows as B operand: lane l holds head l % 16
+        float q[W / 4];
+        bf16x8 qb[sizeof(C) == 4 ? 1 : W / 32][X::QP];
+        {
+            const T* const row = static_cast<const T*>(a.q) + (long long)sequence * a.q_stride + (long long)(head0 + m16) * p.head_dim;
+            const bool there = m16 < heads;
+            if constexpr (sizeof(C) == 4) {
 #pragma unroll
-            for (int c = 0; c < W / 16; ++c) {
-                const int d = 16 * c + 4 * g;
-                Any16 x = {0, 0, 0, 0};
-                if (there && d < p.head_dim) x = *reinterpret_cast<const Any16*>(row + d);
+                for (int c = 0; c < W / 16; ++c) {
+                    const int d = 16 * c + 4 * g;
+                    Any16 x = {0, 0, 0, 0};
+                    if (there && d < p.head_dim) x = *reinterpret_cast<const Any16*>(row + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q[4 * c + i] = __uint_as_float(x[i]);
+                    for (int i = 0; i < 4; ++i) q[4 * c + i] = __uint_as_float(x[i]);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < W / 32; ++c) {
+                    // bf16 keys: piece 4 c + g of 8; int8: half c % 2 of piece 4 (c / 2) + g of 16
+                    const int d = sizeof(C) == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
+                    float x[8] = {};
+                    if (there && d < p.head_dim) load8(row + d, x);
+                    cut<X::QP>(x, qb[c]);
+                }
             }
-        } else {
+        }
+
+        auto entry = [&](int t, int quarter) {  // the page of a tile's quarter; -1: none
+            const int key = t * KT + quarter * G;
+            if (key >= length) return -1;
+            const int e = table[key >> p.page_shift];
+            return e >= 0 && e < p.pages ? e : -1;
+        };
+        // (a lane loads keys of quarter m16 / 4 and values of quarter g)
+        auto load_keys = [&](typename X::Keys& x, int t, int page, int scale_page) {
+            const unsigned char* const block = cache_block(p, max(page, 0), kv);
+            const int row = ((t * KT + (m16 >> 2) * G) & page_mask) + (m16 & 3);
 #pragma unroll
-            for (int c = 0; c < W / 32; ++c) {
-                // bf16 keys: piece 4 c + g of 8; int8: half c % 2 of piece 4 (c / 2) + g of 16
-                const int d = sizeof(C) == 2 ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2);
-                float x[8] = {};
-                if (there && d < p.head_dim) load8(row + d, x);
-                cut<X::QP>(x, qb[c]);
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int c = 0; c < KP; ++c)
+                    x.k[b][c] = *reinterpret_cast<const uint4*>(block + ((size_t)(row + 4 * b) * W + (4 * c + g) * G) * sizeof(C));
+            if constexpr (sizeof(C) == 1) {
+                const float* const scales = reinterpret_cast<const float*>(cache_block(p, max(scale_page, 0), kv) + 2 * p.half_bytes()) + ((t * KT + g * G) & page_mask);
+#pragma unroll
+                for (int i = 0; i < G / 4; ++i) x.scale[i] = *reinterpret_cast<const float4*>(scales + 4 * i);
             }
-        }
-    }
+        };
+        auto load_values = [&](typename X::Values& x, int t, int page) {
+            const unsigned char* const block = cache_block(p, max(page, 0), kv);
+            const int row = (t * KT + g * G) & page_mask;
+            const unsigned char* const values = block + p.half_bytes() + ((size_t)row * W + m16 * G) * sizeof(C);
+#pragma unroll
+            for (int c = 0; c < VP; ++c) x.v[c] = *reinterpret_cast<const uint4*>(values + c * 256);
+            if constexpr (sizeof(C) == 1) {
+                const float* const scales = reinterpret_cast<const float*>(block + 2 * p.half_bytes()) + page_mask + 1 + row;
+#pragma unroll
+                for (int i = 0; i < G / 4; ++i) x.scale[i] = *reinterpret_cast<const float4*>(scales + 4 * i);
+            }
+        };
 
-    auto entry = [&](int t, int quarter) {  // the page of a tile's quarter; -1: none
-        const int key = t * KT + quarter * G;
-        if (key >= length) return -1;
-        const int e = table[key >> p.page_shift];
-        return e >= 0 && e < p.pages ? e : -1;
-    };
-    // (a lane loads keys of quarter m16 / 4 and values of quarter g)
-    auto load_keys = [&](typename X::Keys& x, int t, int page, int scale_page) {
-        const unsigned char* const block = cache_block(p, max(page, 0), kv);
-        const int row = ((t * KT + (m16 >> 2) * G) & page_mask) + (m16 & 3);
+        const float c = a.scale * 1.44269504088896340736f;
+        floatx4 acc[VP];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int c = 0; c < KP; ++c)
-                x.k[b][c] = *reinterpret_cast<const uint4*>(block + ((size_t)(row + 4 * b) * W + (4 * c + g) * G) * sizeof(C));
-        if constexpr (sizeof(C) == 1) {
-            const float* const scales = reinterpret_cast<const float*>(cache_block(p, max(scale_page, 0), kv) + 2 * p.half_bytes()) + ((t * KT + g * G) & page_mask);
-#pragma unroll
-            for (int i = 0; i < G / 4; ++i) x.scale[i] = *reinterpret_cast<const float4*>(scales + 4 * i);
-        }
-    };
-    auto load_values = [&](typename X::Values& x, int t, int page) {
-        const unsigned char* const block = cache_block(p, max(page, 0), kv);
-        const int row = (t * KT + g * G) & page_mask;
-        const unsigned char* const values = block + p.half_bytes() + ((size_t)row * W + m16 * G) * sizeof(C);
-#pragma unroll
-        for (int c = 0; c < VP; ++c) x.v[c] = *reinterpret_cast<const uint4*>(values + c * 256);
-        if constexpr (sizeof(C) == 1) {
-            const float* const scales = reinterpret_cast<const float*>(block + 2 * p.half_bytes()) + page_mask + 1 + row;
-#pragma unroll
-            for (int i = 0; i < G / 4; ++i) x.scale[i] = *reinterpret_cast<const float4*>(scales + 4 * i);
-        }
-    };
+        for (int i = 0; i < VP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -__builtin_inff(), l = 0.0f;
 
-    const float c = a.scale * 1.44269504088896340736f;
-    floatx4 acc[VP];
+        auto score = [&](const typename X::Keys& x, float (&s)[G]) {
 #pragma unroll
-    for (int i = 0; i < VP; ++i) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -__builtin_inff(), l = 0.0f;
-
-    auto score = [&](const typename X::Keys& x, float (&s)[G]) {
+            for (int b = 0; b < NB; ++b) {
+                floatx4 r = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            floatx4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int k = 0; k < KP; ++k) {
+                    if constexpr (sizeof(C) == 4) {
+                        const float y[4] = {__uint_as_float(x.k[b][k].x), __uint_as_float(x.k[b][k].y), __uint_as_float(x.k[b][k].z), __uint_as_float(x.k[b][k].w)};
 #pragma unroll
-            for (int k = 0; k < KP; ++k) {
-                if constexpr (sizeof(C) == 4) {
-                    const float y[4] = {__uint_as_float(x.k[b][k].x), __uint_as_float(x.k[b][k].y), __uint_as_float(x.k[b][k].z), __uint_as_float(x.k[b][k].w)};
+                        for (int i = 0; i < 4; ++i) r = __builtin_amdgcn_mfma_f32_16x16x4f32(y[i], q[4 * k + i], r, 0, 0, 0);
+                    } else if constexpr (sizeof(C) == 2) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) r = __builtin_amdgcn_mfma_f32_16x16x4f32(y[i], q[4 * k + i], r, 0, 0, 0);
-                } else if constexpr (sizeof(C) == 2) {
+                        for (int n = X::QP - 1; n >= 0; --n)
+                            r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[b][k]), qb[k][n], r, 0, 0, 0);
+                    } else {
+                        const bf16x8 lo = widen_i8(make_uint2(x.k[b][k].x, x.k[b][k].y)), hi = widen_i8(make_uint2(x.k[b][k].z, x.k[b][k].w));
 #pragma unroll
-                    for (int n = X::QP - 1; n >= 0; --n)
-                        r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[b][k]), qb[k][n], r, 0, 0, 0);
-                } else {
-                    const bf16x8 lo = widen_i8(make_uint2(x.k[b][k].x, x.k[b][k].y)), hi = widen_i8(make_uint2(x.k[b][k].z, x.k[b][k].w));
+                        for (int n = X::QP - 1; n >= 0; --n) {
+                            r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qb[2 * k][n], r, 0, 0, 0);
+                            r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qb[2 * k + 1][n], r, 0, 0, 0);
+                        }
+                    }
+                }
 #pragma unroll
-                    for (int n = X::QP - 1; n >= 0; --n) {
-                        r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, qb[2 * k][n], r, 0, 0, 0);
-                        r = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, qb[2 * k + 1][n], r, 0, 0, 0);
+                for (int i = 0; i < 4; ++i) s[4 * b + i] = r[i] * c;
+            }
+            if constexpr (sizeof(C) == 1) {
+#pragma unroll
+                for (int i = 0; i < G / 4; ++i) {
+                    s[4 * i] *= x.scale[i].x; s[4 * i + 1] *= x.scale[i].y; s[4 * i + 2] *= x.scale[i].z; s[4 * i + 3] *= x.scale[i].w;
+                }
+            }
+        };
+        auto add = [&](float (&s)[G], typename X::Values& x, int t, int v_page) {
+            // keys behind the end and keys without a page: no score, and nothing of what their values' places hold
+            const int left = v_page < 0 ? 0 : length - (t * KT + g * G);
+            const bool ragged = __any(left < G);
+            if (ragged) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) s[i] = i < left ? s[i] : -__builtin_inff();
+                if constexpr (sizeof(C) != 1) {
+                    uint4 keep;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = sizeof(C) == 4 ? (i < left ? ~0u : 0u) : (2 * i < left ? 0xffffu : 0u) | (2 * i + 1 < left ? 0xffff0000u : 0u);
+                    keep = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int i = 0; i < VP; ++i) {
+                        x.v[i].x &= keep.x; x.v[i].y &= keep.y; x.v[i].z &= keep.z; x.v[i].w &= keep.w;
                     }
                 }
             }
+            float top = s[0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * b + i] = r[i] * c;
-        }
-        if constexpr (sizeof(C) == 1) {
+            for (int i = 1; i < G; ++i) top = fmaxf(top, s[i]);
+            if (__any(top > m + 8.0f)) {  // (as in the kernels over whole sequences)
+                const float next = fmaxf(m, over_rows_max(top)), down = next == m ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+                m = next;
+                l *= down;
 #pragma unroll
-            for (int i = 0; i < G / 4; ++i) {
-                s[4 * i] *= x.scale[i].x; s[4 * i + 1] *= x.scale[i].y; s[4 * i + 2] *= x.scale[i].z; s[4 * i + 3] *= x.scale[i].w;
+                for (int i = 0; i < VP; ++i) acc[i] *= down;
             }
-        }
-    };
-    auto add = [&](float (&s)[G], typename X::Values& x, int t, int v_page) {
-        // keys behind the end and keys without a page: no score, and nothing of what their values' places hold
-        const int left = v_page < 0 ? 0 : length - (t * KT + g * G);
-        const bool ragged = __any(left < G);
-        if (ragged) {
+            const float reference = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-            for (int i = 0; i < G; ++i) s[i] = i < left ? s[i] : -__builtin_inff();
-            if constexpr (sizeof(C) != 1) {
-                uint4 keep;
-                uint32_t w[4];
+            for (int i = 0; i < G; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(s[i] - reference);
+                l += s[i];
+            }
+            if constexpr (sizeof(C) == 4) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[i] = sizeof(C) == 4 ? (i < left ? ~0u : 0u) : (2 * i < left ? 0xffffu : 0u) | (2 * i + 1 < left ? 0xffff0000u : 0u);
-                keep = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int k = 0; k < VP; ++k) {
+                    const float y[4] = {__uint_as_float(x.v[k].x), __uint_as_float(x.v[k].y), __uint_as_float(x.v[k].z), __uint_as_float(x.v[k].w)};
 #pragma unroll
-                for (int i = 0; i < VP; ++i) {
-                    x.v[i].x &= keep.x; x.v[i].y &= keep.y; x.v[i].z &= keep.z; x.v[i].w &= keep.w;
+                    for (int i = 0; i < 4; ++i) acc[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[i], s[i], acc[k], 0, 0, 0);
                 }
-            }
-        }
-        float top = s[0];
+            } else {
+                bf16x8 part[G / 8][X::PP];
 #pragma unroll
-        for (int i = 1; i < G; ++i) top = fmaxf(top, s[i]);
-        if (__any(top > m + 8.0f)) {  // (as in the kernels over whole sequences)
-            const float next = fmaxf(m, over_rows_max(top)), down = next == m ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-            m = next;
-            l *= down;
+                for (int h = 0; h < G / 8; ++h) {
+                    float y[8];
 #pragma unroll
-            for (int i = 0; i < VP; ++i) acc[i] *= down;
-        }
-        const float reference = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - reference);
-            l += s[i];
-        }
-        if constexpr (sizeof(C) == 4) {
-#pragma unroll
-            for (int k = 0; k < VP; ++k) {
-                const float y[4] = {__uint_as_float(x.v[k].x), __uint_as_float(x.v[k].y), __uint_as_float(x.v[k].z), __uint_as_float(x.v[k].w)};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[i], s[i], acc[k], 0, 0, 0);
-            }
-        } else {
-            bf16x8 part[G / 8][X::PP];
-#pragma unroll
-            for (int h = 0; h < G / 8; ++h) {
-                float y[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[i] = s[8 * h + i];
-                    if constexpr (sizeof(C) == 1) {
-                        const float4 f = x.scale[2 * h + i / 4];
-                        y[i] = !ragged || 8 * h + i < left ? y[i] * (i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w) : 0.0f;
+                    for (int i = 0; i < 8; ++i) {
+                        y[i] = s[8 * h + i];
+                        if constexpr (sizeof(C) == 1) {
+                            const float4 f = x.scale[2 * h + i / 4];
+                            y[i] = !ragged || 8 * h + i < left ? y[i] * (i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w) : 0.0f;
+                        }
                     }
+                    cut<X::PP>(y, part[h]);
                 }
-                cut<X::PP>(y, part[h]);
-            }
 #pragma unroll
-            for (int k = 0; k < VP; ++k) {
-                if constexpr (sizeof(C) == 2) {
+                for (int k = 0; k < VP; ++k) {
+                    if constexpr (sizeof(C) == 2) {
 #pragma unroll
-                    for (int n = X::PP - 1; n >= 0; --n)
-                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.v[k]), part[0][n], acc[k], 0, 0, 0);
-                } else {
-                    const bf16x8 lo = widen_i8(make_uint2(x.v[k].x, x.v[k].y)), hi = widen_i8(make_uint2(x.v[k].z, x.v[k].w));
+                        for (int n = X::PP - 1; n >= 0; --n)
+                            acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.v[k]), part[0][n], acc[k], 0, 0, 0);
+                    } else {
+                        const bf16x8 lo = widen_i8(make_uint2(x.v[k].x, x.v[k].y)), hi = widen_i8(make_uint2(x.v[k].z, x.v[k].w));
 #pragma unroll
-                    for (int n = X::PP - 1; n >= 0; --n) {
-                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, part[0][n], acc[k], 0, 0, 0);
-                        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, part[1][n], acc[k], 0, 0, 0);
+                        for (int n = X::PP - 1; n >= 0; --n) {
+                            acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, part[0][n], acc[k], 0, 0, 0);
+                            acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, part[1][n], acc[k], 0, 0, 0);
+                        }
                     }
                 }
             }
-        }
-    };
+        };
 
-    // A tile's values are under way while its scores are made, the next tile's keys while its values are added; page numbers come a tile
-    // earlier.  (Behind the last tile that one is loaded again: no load depends on a branch, so that each is waited for alone.)
-    int t = from + wave;
-    if (t < to) {
-        typename X::Keys keys;
-        typename X::Values values;
-        int v_page = entry(t, g);
-        load_keys(keys, t, entry(t, m16 >> 2), v_page);
-        int next = min(t + NW, to - 1);
-        int k_next = entry(next, m16 >> 2), v_next = entry(next, g);
-        for (; t < to; t += NW) {
-            load_values(values, t, v_page);
-            const int after = min(t + 2 * NW, to - 1);
-            const int k_after = entry(after, m16 >> 2), v_after = entry(after, g);
-            __builtin_amdgcn_sched_barrier(0);
-            float s[G];
-            score(keys, s);
-            __builtin_amdgcn_sched_barrier(0);
-            load_keys(keys, next, k_next, v_next);
-            __builtin_amdgcn_sched_barrier(0);
-            add(s, values, t, v_page);
-            v_page = v_next;
-            k_next = k_after;
-            v_next = v_after;
-            next = after;
-        }
-    }
-    l = over_rows_sum(l);
-
-    // the waves' parts
-    if (g == 0) {
-        wave_m[wave][m16] = m;
-        wave_l[wave][m16] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < VP; ++i)
-        *reinterpret_cast<floatx4*>(&joined[wave][m16][16 * i + 4 * g]) = acc[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * W; i += 64 * NW) {
-        const int h = i / W, d = i % W;
-        if (d >= p.head_dim) continue;
-        float top = wave_m[0][h];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, wave_m[w][h]);
-        float o = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = wave_m[w][h] == top ? 1.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
-            o = __builtin_fmaf(f, joined[w][h][d], o);
-            sum = __builtin_fmaf(f, wave_l[w][h], sum);
-        }
-        if (part < 0) {
-            static_cast<T*>(a.out)[((long long)sequence * a.heads + head0 + h) * p.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
-        } else {
-            const long long row = part * a.heads + head0 + h;
-            a.partial[row * W + d] = o;
-            if (d == 0) {
-                a.statistics[row * 2] = top;
-                a.statistics[row * 2 + 1] = sum;
+        // A tile's values are under way while its scores are made, the next tile's keys while its values are added; page numbers come a tile
+        // earlier.  (Behind the last tile that one is loaded again: no load depends on a branch, so that each is waited for alone.)
+        int t = from + wave;
+        if (t < to) {
+            typename X::Keys keys;
+            typename X::Values values;
+            int v_page = entry(t, g);
+            load_keys(keys, t, entry(t, m16 >> 2), v_page);
+            int next = min(t + NW, to - 1);
+            int k_next = entry(next, m16 >> 2), v_next = entry(next, g);
+            for (; t < to; t += NW) {
+                load_values(values, t, v_page);
+                const int after = min(t + 2 * NW, to - 1);
+                const int k_after = entry(after, m16 >> 2), v_after = entry(after, g);
+                __builtin_amdgcn_sched_barrier(0);
+                float s[G];
+                score(keys, s);
+                __builtin_amdgcn_sched_barrier(0);
+                load_keys(keys, next, k_next, v_next);
+                __builtin_amdgcn_sched_barrier(0);
+                add(s, values, t, v_page);
+                v_page = v_next;
+                k_next = k_after;
+                v_next = v_after;
+                next = after;
             }
         }
-    }
-    };  // work
+        l = over_rows_sum(l);
+
+        // the waves' parts
+        if (g == 0) {
+            wave_m[wave][m16] = m;
+            wave_l[wave][m16] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < VP; ++i)
+            *reinterpret_cast<floatx4*>(&joined[wave][m16][16 * i + 4 * g]) = acc[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < heads * W; i += 64 * NW) {
+            const int h = i / W, d = i % W;
+            if (d >= p.head_dim) continue;
+            float top = wave_m[0][h];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, wave_m[w][h]);
+            float o = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = wave_m[w][h] == top ? 1.0f : __builtin_amdgcn_exp2f(wave_m[w][h] - top);
+                o = __builtin_fmaf(f, joined[w][h][d], o);
+                sum = __builtin_fmaf(f, wave_l[w][h], sum);
+            }
+            if (part < 0) {
+                static_cast<T*>(a.out)[((long long)sequence * a.heads + head0 + h) * p.head_dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
+            } else {
+                const long long row = part * a.heads + head0 + h;
+                a.partial[row * W + d] = o;
+                if (d == 0) {
+                    a.statistics[row * 2] = top;
+                    a.statistics[row * 2 + 1] = sum;
+                }
+            }
+        }
+    };
 
     if constexpr (!STREAM) {
         work(blockIdx.y, 0, (sequence_length(a, blockIdx.y) + KT - 1) / KT, -1);
@@ -702,16 +703,9 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : RBMOE_DECODE_OCC) void deco
 
 // One workgroup a row whose sequence passes the ends of ranges: its parts.  256 / W threads share a column, each takes every so many parts; their
 // sums are added in order.
-#ifndef RBMOE_DECODE_WG
-#define RBMOE_DECODE_WG 512
-#endif
-#ifndef RBMOE_DECODE_PART
-#define RBMOE_DECODE_PART 512
-#endif
-#ifndef RBMOE_DECODE_ONE
-#define RBMOE_DECODE_ONE 1024
-#endif
-constexpr int kDecodeWorkgroups = RBMOE_DECODE_WG, kLeastPart = RBMOE_DECODE_PART, kOnePart = RBMOE_DECODE_ONE;
+// Two workgroups a compute unit (1024: 134 us for the 64 sequences above, 512: 124; in fixed parts of each sequence 156); a sequence of 777 rows by
+// one workgroup 10.7 us with its write, in parts 13.0.
+constexpr int kDecodeWorkgroups = 512, kLeastPart = 512, kOnePart = 1024;
 
 template <typename T, typename C, int W>
 __global__ __launch_bounds__(256) void decode_join_kernel(DecodeCall a) {
