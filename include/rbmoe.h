@@ -447,7 +447,7 @@ typedef struct rbmoe_kv_cache rbmoe_kv_cache;
 int rbmoe_kv_cache_create(rbmoe_ctx* ctx, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t cache_dtype, int32_t page_rows,
                           int32_t pages, rbmoe_kv_cache** out);
 void rbmoe_kv_cache_destroy(rbmoe_kv_cache* cache);
-/* Rows k and v [rows, kv_heads, head_dim] to their slots.  A row whose slot is negative or behind the last page is left out (padding).  The
+/* Rows k and v [rows, kv_heads, head_dim] (up to 2^28 a call) to their slots.  A row whose slot is negative or behind the last page is left out (padding).  The
  * rows of one call go to different slots: two rows for one slot leave a mixture of both there. */
 int rbmoe_kv_cache_write(rbmoe_kv_cache* cache, int32_t rows, const void* k, int32_t k_stride, const void* v, int32_t v_stride,
                          const int64_t* slots);

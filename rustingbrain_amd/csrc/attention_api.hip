@@ -35,7 +35,7 @@ struct rbmoe_decode {
 
 namespace {
 
-constexpr int kMostHeads = 1024, kMostSequences = 65535, kMostRows = 1 << 30;
+constexpr int kMostHeads = 1024, kMostSequences = 65535, kMostRows = 1 << 30, kMostCacheRows = 1 << 28;
 
 bool off_element(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == RBMOE_BF16 ? 2 : 4) != 0; }
 
@@ -254,7 +254,7 @@ static int cache_rows_call(rbmoe_kv_cache* c, int32_t rows, const void* k, int32
     if (!c) return fail(nullptr, RBMOE_NULL_POINTER, "cache is NULL");
     rbmoe_ctx* ctx = c->ctx;
     if (rows < 0) return fail(ctx, RBMOE_INVALID_INPUT, "the row count must not be negative");
-    if (rows > kMostRows) return fail(ctx, RBMOE_UNSUPPORTED, "more than 2^30 rows");
+    if (rows > kMostCacheRows) return fail(ctx, RBMOE_UNSUPPORTED, "more than 2^28 rows");  // (a launch's 2^32 threads)
     CacheRows a{};
     if (const int rc = stride_problem(ctx, k_stride, c->pool.kv_heads * c->pool.head_dim, a.k_stride)) return rc;
     if (const int rc = stride_problem(ctx, v_stride, c->pool.kv_heads * c->pool.head_dim, a.v_stride)) return rc;

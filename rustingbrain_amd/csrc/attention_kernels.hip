@@ -502,7 +502,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
     load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
 
     // the keys that a row sees are those below its limit
-    auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
+    auto limit = [&](int r) { return a.causal ? min(max(r - s.nq + s.nk + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
     const int end = limit(min(first + OWN, s.nq) - 1);
     constexpr int STEP = TEAM == 1 ? kWaves * N : N;
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
                     for (int i = 0; i < 16; ++i)
                         if (t + 32 * b + block_row(i) >= own_limit) p[b][i] = -__builtin_inff();
             }
-            // The exponents' arguments by the reference that there is: it moves only when a score passes it by 2^8.  The results are
+            // The exponents' arguments by the reference that there is: it moves only when a score passes it by 2^8 (f32 rows: e^8).  The results are
             // the same, sums and accumulators have room for it, and after a few tiles nothing has to be scaled.
             const float reference = m == -__builtin_inff() ? 0.0f : m;
             float top = -__builtin_inff();
@@ -646,7 +646,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
     asm volatile("" : "+v"(reference));  // (as in load_own)
 
-    auto limit = [&](int r) { return a.causal ? min(max(r + s.nk - s.nq + 1, 0), s.nk) : s.nk; };
+    auto limit = [&](int r) { return a.causal ? min(max(r - s.nq + s.nk + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
     const int end = limit(min(first + OWN, s.nq) - 1);
     constexpr int STEP = TEAM == 1 ? kWaves * N : N;

@@ -418,6 +418,14 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void decode_attention_ke
         const int length = sequence_length(a, sequence);
         const int32_t* const table = a.tables + (long long)sequence * a.table_pages;
 
+        auto entry_at = [&](int t, int quarter) {
+            const int i = (t * KT + quarter * G) >> p.page_shift;
+            return i < a.table_pages ? table[i] : -1;
+        };
+        // (under way beside the length and the heads' rows)
+        int t = from + wave;
+        const int first_k = entry_at(t, m16 >> 2), first_v = entry_at(t, g);
+
         // the heads' rows as B operand: lane l holds head l % 16
         float q[W / 4];
         bf16x8 qb[sizeof(C) == 4 ? 1 : W / 32][X::QP];
@@ -445,12 +453,9 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void decode_attention_ke
             }
         }
 
-        auto entry = [&](int t, int quarter) {  // the page of a tile's quarter; -1: none
-            const int key = t * KT + quarter * G;
-            if (key >= length) return -1;
-            const int e = table[key >> p.page_shift];
-            return e >= 0 && e < p.pages ? e : -1;
-        };
+        // the page of a tile's quarter, or -1: what the table holds there, and whether the quarter has keys
+        auto page_of = [&](int entry, int t, int quarter) { return t * KT + quarter * G < length && entry >= 0 && entry < p.pages ? entry : -1; };
+        auto entry = [&](int t, int quarter) { return page_of(entry_at(t, quarter), t, quarter); };
         // (a lane loads keys of quarter m16 / 4 and values of quarter g)
         auto load_keys = [&](typename X::Keys& x, int t, int page, int scale_page) {
             const unsigned char* const block = cache_block(p, max(page, 0), kv);
@@ -596,12 +601,11 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void decode_attention_ke
 
         // A tile's values are under way while its scores are made, the next tile's keys while its values are added; page numbers come a tile
         // earlier.  (Behind the last tile that one is loaded again: no load depends on a branch, so that each is waited for alone.)
-        int t = from + wave;
         if (t < to) {
             typename X::Keys keys;
             typename X::Values values;
-            int v_page = entry(t, g);
-            load_keys(keys, t, entry(t, m16 >> 2), v_page);
+            int v_page = page_of(first_v, t, g);
+            load_keys(keys, t, page_of(first_k, t, m16 >> 2), v_page);
             int next = min(t + NW, to - 1);
             int k_next = entry(next, m16 >> 2), v_next = entry(next, g);
             for (; t < to; t += NW) {

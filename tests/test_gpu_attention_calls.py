@@ -464,6 +464,8 @@ def test_refused_calls(device):
                 call(*args)
         with pytest.raises(rb.InvalidInput):
             call(4, k, v, slots.ptr, k_stride=100)
+        with pytest.raises(rb.Unsupported):
+            call((1 << 28) + 1, k, v, slots.ptr)
         call(0, 0, 0, 0)
     with pytest.raises(rb.InvalidInput):
         c.read_device(4, grads[1].ptr, grads[1].ptr, slots.ptr)
