@@ -5,8 +5,8 @@
 // infinity or NaN reads back as NaN whole.
 //
 // All of it is bound by memory (a large copy moves 4.9 TB/s): 23165 bf16 rows of 8 x 128 to 8 bits and back 57 us, 5.0 TB/s; new rows over 4 x 131072 cached
-// ones, bf16, 8 kv heads of 128, 198 us, 5.4 TB/s; over 64 sequences up to 8192 rows in 8 bits 122 us, 4.0 TB/s (widening bytes to
-// bf16 keeps the vector units busy a third of the time, pages of 16 rows come in pieces of 2 KB).  Small calls: launches of 3 to 6 us.
+// ones, bf16, 8 kv heads of 128, 192 us, 5.6 TB/s; over 64 sequences up to 8192 rows in 8 bits 114 us, 4.3 TB/s (4.8 without the new rows' write and the
+// join).  Small calls: launches of 2 to 8 us.
 #include "kv_cache_kernels.h"
 
 #include <algorithm>
@@ -94,6 +94,10 @@ __device__ __forceinline__ int run_from(uint64_t next, int r) {
     return stops ? (int)__builtin_ctzll(stops) + 1 : 64;
 }
 
+// Calls of less than a workgroup a compute unit are bound by the way of a load and a store, not by their number: each element by itself (628 rows of
+// 2 x 64 written and read: 8.4 us; by pieces through LDS 10.7).
+__device__ __forceinline__ bool few_rows() { return gridDim.x * gridDim.y < 256; }
+
 template <typename T, typename C, int W>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
     constexpr int R = cache_rows<W>(), TR = W / 8, G = 16 / sizeof(C);
@@ -114,7 +118,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheRows a) {
     }
     __syncthreads();
     const int page_mask = (1 << p.page_shift) - 1, c = tid % TR * 8;
-    const bool scattered = neighbours == 0;  // (new rows of many sequences: the way through LDS would gain nothing)
+    const bool scattered = few_rows() || neighbours == 0;  // (new rows of many sequences: pieces would have one element)
 #pragma unroll
     for (int i = 0; i < R * TR / 256; ++i) {
         const int r = i * (256 / TR) + tid / TR;
@@ -235,9 +239,10 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheRows a) {
     }
     __syncthreads();
     const int page_mask = (1 << p.page_shift) - 1;
+    const bool direct = few_rows();
     const int d = tid % W, end = tid / W * 16 + 16;
     const uint64_t next = neighbours;
-    for (int r = end - 16; r < end;) {
+    for (int r = direct ? end : end - 16; r < end;) {
         const long long at = places[r];
         if (at < 0) {
             ++r;
@@ -281,7 +286,15 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheRows a) {
             const unsigned char* const block = cache_block(p, at >> p.page_shift, head);
             const int row = (int)(at & page_mask);
             widen8(reinterpret_cast<const C*>(block) + (size_t)row * W + c, k);
-            widen8(&values[r][c], v);
+            if (direct) {
+                __attribute__((aligned(16))) C own[8];
+                const C* const from = reinterpret_cast<const C*>(block + p.half_bytes()) + value_at<W, G>(row, c);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) own[j] = from[j * G];
+                widen8(own, v);
+            } else {
+                widen8(&values[r][c], v);
+            }
             if constexpr (sizeof(C) == 1) {
                 const float* const scales = reinterpret_cast<const float*>(block + 2 * p.half_bytes());
                 const float k_scale = scales[row], v_scale = scales[(1 << p.page_shift) + row];
@@ -707,8 +720,8 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void decode_attention_ke
 
 // One workgroup a row whose sequence passes the ends of ranges: its parts.  256 / W threads share a column, each takes every so many parts; their
 // sums are added in order.
-// Two workgroups a compute unit (1024: 134 us for the 64 sequences above, 512: 124; in fixed parts of each sequence 156); a sequence of 777 rows by
-// one workgroup 10.7 us with its write, in parts 13.0.
+// Two workgroups a compute unit (1024: 134 us for the 64 sequences above, 512: 124, before loads of the table were moved; in fixed parts of each sequence
+// 156); a sequence of 777 rows by one workgroup 10.7 us with its write, in parts 13.0.
 constexpr int kDecodeWorkgroups = 512, kLeastPart = 512, kOnePart = 1024;
 
 template <typename T, typename C, int W>

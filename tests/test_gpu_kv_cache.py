@@ -98,6 +98,22 @@ def test_rows_come_back(device, dtype, cache, kv, d, page):
     c.op.close()
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 32), (40, 128)])
+def test_many_rows_come_back(device, dtype, cache, d, page):
+    """Calls of more workgroups than compute units, whose values go through LDS in pieces."""
+    rng, kv, size = np.random.default_rng(d), 16, 1280
+    c = Cache(device, kv, d, size // page, page, dtype, cache)
+    gaps = np.arange(1200)  # runs of every length, off every alignment, with rows of no place between
+    gaps[rng.integers(0, 1200, 150)] = -1
+    swapped = np.arange(1280).reshape(-1, 5)[:, ::-1].reshape(-1)
+    for i, slots in enumerate((np.arange(7, 7 + 1270), gaps + np.where(gaps < 0, 0, 3), rng.permutation(size)[:1100], swapped)):
+        c.write(rows_of(rng, len(slots), kv, d, dtype), rows_of(rng, len(slots), kv, d, dtype), slots, i % 2)
+        for order in (np.arange(-1, size + 1), rng.permutation(size), slots):
+            assert same(np.stack(c.read(order, i % 2)), c.expected(order)), i
+    c.op.close()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_eight_bits_of_odd_rows(device, dtype):
     """Zeros, ties, one large value, values near the ends of the range, infinities and NaN; a row's scale is its own."""
