@@ -411,8 +411,9 @@ int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* h
 /* Attention of whole sequences.  Sequence i has the queries query_begin[i] .. + query_count[i] and the keys key_begin[i] .. +
  * key_count[i] (key arrays NULL: the queries'), of arrays of query_rows and key_rows rows: packed one behind the other, or padded,
  * with rows between them that are left as they are.  Counts go up to longest_queries and longest_keys, which a launch is
- * sized by (a longer sequence counts as that long, and what lies outside the arrays is cut off).  With causal != 0 query r of a sequence sees its keys up to
- * r + key_count - query_count: the queries are the last of the keys, whose first may come from a cache.
+ * sized by (a longer sequence counts as that long).  With causal != 0 query r of a sequence sees its keys up to
+ * r + key_count - query_count: the queries are the last of the keys, whose first may come from a cache.  Rows and keys of a sequence that lie outside the
+ * arrays are left out, and the others see what they would see beside them.
  *   s_ij = scale q_i . k_j,   lse_i = log sum_j exp s_ij,   out_i = sum_j exp(s_ij - lse_i) v_j    over the keys that row i sees
  * A row that sees no key is zeros, its lse -inf.  What is not seen has no effect, whatever it holds; an infinity that is seen may come out as
  * NaN (f32 rows are multiplied in parts).  scale is positive.  Two sequences may share keys

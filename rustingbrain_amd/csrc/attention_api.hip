@@ -86,13 +86,15 @@ int sequences_problem(rbmoe_attention* at, int32_t sequences, int32_t longest_qu
     a.sequences = sequences;
     a.query_rows = query_rows;
     a.key_rows = key_rows;
-    a.longest_queries = longest_queries < query_rows ? longest_queries : query_rows;
-    a.longest_keys = longest_keys < key_rows ? longest_keys : key_rows;
+    a.longest_queries = longest_queries;
+    a.longest_keys = longest_keys;
+    a.most_queries = longest_queries < query_rows ? longest_queries : query_rows;
+    a.most_keys = longest_keys < key_rows ? longest_keys : key_rows;
     a.heads = at->heads;
     a.kv_heads = at->kv_heads;
     a.head_dim = at->head_dim;
     a.scale = scale;
-    const long long tiles = ((long long)a.longest_queries + 127) / 128, key_tiles = ((long long)a.longest_keys + 127) / 128;
+    const long long tiles = ((long long)a.most_queries + 127) / 128, key_tiles = ((long long)a.most_keys + 127) / 128;
     if (tiles * at->heads * sequences > (1 << 23) || key_tiles * at->kv_heads * sequences > (1 << 23))
         return fail(ctx, RBMOE_UNSUPPORTED, "sequences * heads * longest is more than a launch has workgroups for");
     return RBMOE_OK;
@@ -148,8 +150,8 @@ int rbmoe_attention_forward(rbmoe_attention* at, int32_t sequences, int32_t long
     if (const int rc = sequences_problem(at, sequences, longest_queries, longest_keys, query_begin, query_count, key_begin, key_count, query_rows,
                                          key_rows, q_stride, k_stride, v_stride, scale, a))
         return rc;
-    if (sequences == 0 || a.longest_queries == 0) return RBMOE_OK;
-    if (!q || !out || (a.longest_keys > 0 && (!k || !v))) return fail(ctx, RBMOE_NULL_POINTER, "q, k, v or out is NULL");
+    if (sequences == 0 || a.most_queries == 0) return RBMOE_OK;
+    if (!q || !out || (a.most_keys > 0 && (!k || !v))) return fail(ctx, RBMOE_NULL_POINTER, "q, k, v or out is NULL");
     for (const void* p : {q, k, v, (const void*)out})
         if (off_element(p, at->dtype)) return fail(ctx, RBMOE_INVALID_INPUT, "rows must start at an element");
     if (off_element(lse, RBMOE_F32)) return fail(ctx, RBMOE_INVALID_INPUT, "lse must start at an element");
@@ -178,11 +180,11 @@ int rbmoe_attention_backward(rbmoe_attention* at, int32_t sequences, int32_t lon
     if (query_rows > at->backward_rows)
         return fail(ctx, RBMOE_INVALID_INPUT, "this attention was created for the backward pass of " + std::to_string(at->backward_rows) + " rows, got " +
                                                   std::to_string(query_rows));
-    if (sequences == 0 || (a.longest_queries == 0 && a.longest_keys == 0)) return RBMOE_OK;
-    if (a.longest_queries > 0) {
+    if (sequences == 0 || (a.most_queries == 0 && a.most_keys == 0)) return RBMOE_OK;
+    if (a.most_queries > 0) {
         if (!q || !out || !lse || !grad_out || !grad_q) return fail(ctx, RBMOE_NULL_POINTER, "q, out, lse, grad_out or grad_q is NULL");
     }
-    if (a.longest_keys > 0 && (!k || !v || !grad_k || !grad_v)) return fail(ctx, RBMOE_NULL_POINTER, "k, v, grad_k or grad_v is NULL");
+    if (a.most_keys > 0 && (!k || !v || !grad_k || !grad_v)) return fail(ctx, RBMOE_NULL_POINTER, "k, v, grad_k or grad_v is NULL");
     if (grad_q && (grad_q == grad_k || grad_q == grad_v)) return fail(ctx, RBMOE_INVALID_INPUT, "gradients must be three arrays");
     if (grad_k && grad_k == grad_v) return fail(ctx, RBMOE_INVALID_INPUT, "gradients must be three arrays");
     for (const void* p : {q, k, v, out, grad_out, (const void*)grad_q, (const void*)grad_k, (const void*)grad_v})
@@ -354,6 +356,17 @@ int rbmoe_decode_attention(rbmoe_decode* d, rbmoe_kv_cache* c, int32_t sequences
     a.statistics = a.partial + d->partials * (d->head_dim <= 64 ? 64 : 128);
     HIP_TRY(ctx, launch_decode_attention(a, d->dtype == RBMOE_BF16, ctx->stream));
     return RBMOE_OK;
+}
+
+// Which rows of a sequence a call finds: q0, nq, k0, nk, ahead; for tests (no GPU needed).
+void rbmoe_internal_attention_sequence(int32_t query_begin, int32_t query_count, int32_t key_begin, int32_t key_count, int32_t query_rows,
+                                       int32_t key_rows, int32_t longest_queries, int32_t longest_keys, int32_t* out) {
+    const Sequence s = cut_sequence(query_begin, query_count, key_begin, key_count, query_rows, key_rows, longest_queries, longest_keys);
+    out[0] = s.q0;
+    out[1] = s.nq;
+    out[2] = s.k0;
+    out[3] = s.nk;
+    out[4] = s.ahead;
 }
 
 // Into how many ranges a call cuts its sequences: for tests (no GPU needed).

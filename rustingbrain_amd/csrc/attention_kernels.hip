@@ -393,17 +393,8 @@ __device__ __forceinline__ float over_waves(float v, char* room) {
 }
 
 // ---- sequences -------------------------------------------------------------------------------------
-struct Sequence {
-    int q0, nq, k0, nk;
-};
-// (whatever the arrays hold, a sequence lies inside the rows that the call names)
 __device__ __forceinline__ Sequence sequence_of(const AttentionCall& a, int i) {
-    Sequence s;
-    s.q0 = min(max(a.query_begin[i], 0), a.query_rows);
-    s.nq = min(max(a.query_count[i], 0), min(a.longest_queries, a.query_rows - s.q0));
-    s.k0 = min(max(a.key_begin[i], 0), a.key_rows);
-    s.nk = min(max(a.key_count[i], 0), min(a.longest_keys, a.key_rows - s.k0));
-    return s;
+    return cut_sequence(a.query_begin[i], a.query_count[i], a.key_begin[i], a.key_count[i], a.query_rows, a.key_rows, a.longest_queries, a.longest_keys);
 }
 // Which tile, head and sequence a workgroup takes.  Workgroup i runs on XCD i % 8: where the heads divide among them, every XCD has
 // its own heads (neighbours, so that a group's heads share their keys in one L2), otherwise all take turns.  Tiles in descending order: the last are the
@@ -487,7 +478,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of keys and values
-    const int tiles = (a.longest_queries + OWN - 1) / OWN;
+    const int tiles = (a.most_queries + OWN - 1) / OWN;
     const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
     const Sequence s = sequence_of(a, at.sequence);
     const int first = at.tile * OWN;
@@ -502,7 +493,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
     load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
 
     // the keys that a row sees are those below its limit
-    auto limit = [&](int r) { return a.causal ? min(max(r - s.nq + s.nk + 1, 0), s.nk) : s.nk; };
+    auto limit = [&](int r) { return a.causal ? min(max(r + s.ahead + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
     const int end = limit(min(first + OWN, s.nq) - 1);
     constexpr int STEP = TEAM == 1 ? kWaves * N : N;
@@ -616,7 +607,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];
-    const int tiles = (a.longest_queries + OWN - 1) / OWN;
+    const int tiles = (a.most_queries + OWN - 1) / OWN;
     const Place at = place_of(a.heads, a.sequences, tiles, a.causal);
     const Sequence s = sequence_of(a, at.sequence);
     const int first = at.tile * OWN;
@@ -646,7 +637,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
     asm volatile("" : "+v"(reference));  // (as in load_own)
 
-    auto limit = [&](int r) { return a.causal ? min(max(r - s.nq + s.nk + 1, 0), s.nk) : s.nk; };
+    auto limit = [&](int r) { return a.causal ? min(max(r + s.ahead + 1, 0), s.nk) : s.nk; };
     const int own_limit = limit(row), least = limit(wave_first), most = limit(min(wave_first + 31, s.nq - 1));
     const int end = limit(min(first + OWN, s.nq) - 1);
     constexpr int STEP = TEAM == 1 ? kWaves * N : N;
@@ -741,7 +732,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     typedef Tile<T, D, N> Tl;
     constexpr int BYTES = Tl::BYTES, STAGE = 2 * BYTES + 2 * N * 4;
     extern __shared__ __attribute__((aligned(16))) char attention_lds[];  // two stages of queries, gradients, lse and delta
-    const int tiles = (a.longest_keys + OWN - 1) / OWN;
+    const int tiles = (a.most_keys + OWN - 1) / OWN;
     const Place at = place_of(a.kv_heads * a.shares, a.sequences, tiles, false);
     const Sequence s = sequence_of(a, at.sequence);
     const int first = at.tile * OWN, kv = at.head / a.shares, share = at.head % a.shares;
@@ -756,8 +747,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     load_own<T, D>(static_cast<const T*>(a.v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, pieces, v);
 
     // the rows that see a key are those from its start on
-    auto start = [&](int j) { return a.causal ? max(j - (s.nk - s.nq), 0) : 0; };
-    const int lone = a.causal ? s.nq - s.nk : -1;  // the row that sees one key: p = 1 and ds = 0
+    auto start = [&](int j) { return a.causal ? max(j - s.ahead, 0) : 0; };
+    const int lone = a.causal ? -s.ahead : -1;  // the row that sees one key: p = 1 and ds = 0
     const int own_start = start(key), least = start(wave_first), most = start(wave_first + 31);
     const int begin = start(first) / N * N, turns = begin < s.nq ? (s.nq - begin + N - 1) / N : 0, all = turns * group;
     constexpr int STEP = TEAM == 1 ? kWaves : 1;
@@ -917,11 +908,11 @@ hipError_t launch(K kernel, std::atomic<unsigned long long>& once, const Attenti
 hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream_t s) {
     const int size = bf16 ? 2 : 4;
     const bool aligned = whole_pieces(a.k, a.k_stride, size) && whole_pieces(a.v, a.v_stride, size);
-    return with_kernel(bf16, a.head_dim, few_workgroups(a, a.longest_queries, a.heads), aligned, [&](auto type, auto width, auto team, auto whole) {
+    return with_kernel(bf16, a.head_dim, few_workgroups(a, a.most_queries, a.heads), aligned, [&](auto type, auto width, auto team, auto whole) {
         typedef decltype(type) T;
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
-        return launch(attention_forward_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
+        return launch(attention_forward_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.most_queries + OWN - 1) / OWN, a.heads,
                       tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM>(), false>(0), s);
     });
 }
@@ -929,33 +920,33 @@ hipError_t launch_attention_forward(const AttentionCall& a, bool bf16, hipStream
 hipError_t launch_attention_backward(const AttentionCall& a, bool bf16, hipStream_t s) {
     const int size = bf16 ? 2 : 4;
     hipError_t e = hipSuccess;
-    if (a.longest_queries > 0) {
+    if (a.most_queries > 0) {
         const bool aligned = whole_pieces(a.k, a.k_stride, size) && whole_pieces(a.v, a.v_stride, size);
-        e = with_kernel(bf16, a.head_dim, few_workgroups(a, a.longest_queries, a.heads), aligned, [&](auto type, auto width, auto team, auto whole) {
+        e = with_kernel(bf16, a.head_dim, few_workgroups(a, a.most_queries, a.heads), aligned, [&](auto type, auto width, auto team, auto whole) {
             typedef decltype(type) T;
             constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
             static std::atomic<unsigned long long> once{0};
-            return launch(attention_grad_q_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.longest_queries + OWN - 1) / OWN, a.heads,
+            return launch(attention_grad_q_kernel<T, D, TEAM, decltype(whole)::value>, once, a, (a.most_queries + OWN - 1) / OWN, a.heads,
                           tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM, true>(), true>(0), s);
         });
     }
-    if (e != hipSuccess || a.longest_keys == 0) return e;
+    if (e != hipSuccess || a.most_keys == 0) return e;
     // A kv head's workgroups go through all heads of its group.  Where they are few, each head gets workgroups of its own, and their sums are added.
     AttentionCall b = a;
     const int group = a.heads / a.kv_heads;
-    const long long blocks = (long long)((a.longest_keys + 31) / 32) * a.kv_heads * a.sequences;
-    const bool few = few_workgroups(a, a.longest_keys, a.kv_heads);
+    const long long blocks = (long long)((a.most_keys + 31) / 32) * a.kv_heads * a.sequences;
+    const bool few = few_workgroups(a, a.most_keys, a.kv_heads);
     b.shares = few && group > 1 && blocks < (a.head_dim <= 64 ? kShared : kShared / 2) && (long long)a.key_rows * a.kv_heads <= a.part_rows ? group : 1;
     const bool aligned = whole_pieces(a.q, a.q_stride, size) && whole_pieces(a.grad_out, a.head_dim, size);
     e = with_kernel(bf16, a.head_dim, few, aligned, [&](auto type, auto width, auto team, auto whole) {
         typedef decltype(type) T;
         constexpr int D = decltype(width)::value, TEAM = decltype(team)::value, OWN = 32 * TEAM;
         static std::atomic<unsigned long long> once{0};
-        return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, b, (a.longest_keys + OWN - 1) / OWN, a.kv_heads * b.shares,
+        return launch(attention_grad_kv_kernel<T, D, TEAM, decltype(whole)::value>, once, b, (a.most_keys + OWN - 1) / OWN, a.kv_heads * b.shares,
                       tiles_lds<T, D, TEAM, tile_rows<T, D, TEAM>(), true>(8 * tile_rows<T, D, TEAM>()), s);
     });
     if (e != hipSuccess || b.shares == 1) return e;
-    const dim3 grid((unsigned)(((long long)a.longest_keys * a.kv_heads * a.head_dim / 4 + kThreads - 1) / kThreads), a.sequences);
+    const dim3 grid((unsigned)(((long long)a.most_keys * a.kv_heads * a.head_dim / 4 + kThreads - 1) / kThreads), a.sequences);
     if (bf16) hipLaunchKernelGGL(attention_add_shares_kernel<bf16_t>, grid, dim3(kThreads), 0, s, b);
     else hipLaunchKernelGGL(attention_add_shares_kernel<float>, grid, dim3(kThreads), 0, s, b);
     return hipGetLastError();
