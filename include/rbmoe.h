@@ -415,8 +415,8 @@ int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* h
  * r + key_count - query_count: the queries are the last of the keys, whose first may come from a cache.  Rows and keys of a sequence that lie outside the
  * arrays are left out, and the others see what they would see beside them.
  *   s_ij = scale q_i . k_j,   lse_i = log sum_j exp s_ij,   out_i = sum_j exp(s_ij - lse_i) v_j    over the keys that row i sees
- * A row that sees no key is zeros, its lse -inf.  What is not seen has no effect, whatever it holds; an infinity that is seen may come out as
- * NaN (f32 rows are multiplied in parts).  scale is positive.  Two sequences may share keys
+ * A row that sees no key is zeros, its lse -inf; a key whose score is -inf counts as not seen.  What is not seen has no effect, whatever it
+ * holds; infinities and NaN that are seen have the effect that f32 arithmetic gives them.  scale is positive.  Two sequences may share keys
  * (forward only), not queries.
  *   out  [query_rows, heads, head_dim] without gaps      lse [heads, query_rows] f32 or NULL
  * Sums and statistics are f32 (f32 rows: their products too); bf16 rows round exp(s_ij - m) to bf16 for the product with v. */

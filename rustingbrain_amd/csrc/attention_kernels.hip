@@ -17,8 +17,9 @@
 // memory: eight products where five would do, but the same bits from the same call, and no f32 gradients that pass through memory.
 //
 // Masked places: a masked score is replaced behind the product, whatever it was.  A masked p of zero times an infinity or NaN
-// in the tile would still be NaN, so a workgroup that ends with such a value goes over its tiles again and adds the blocks
-// on the diagonal row by row; nothing else is read twice.
+// in the tile would still be NaN, so a workgroup that ends with such a value goes over its tiles again: bf16 rows add the blocks
+// on the diagonal row by row, f32 rows, whose parts make NaN of an infinity, leave the parts alone (product_f32).  6 x 2048 rows of 8 heads of 64 with
+// a NaN in the first value of each: 1.5 ms where clean ones take 0.12; 8192 bf16 rows of 16 heads of 128, backward: 4.9 for 1.5.
 //
 // What bounds them (a large bf16 product by the library reaches 1370 TFLOP/s, an f32 one 153):
 //   forward, 16384 rows, 16 heads of 128, bf16, causal: 1.14 ms, 965 TFLOP/s.  A wave reads every tile from LDS whole, which takes as many cycles
@@ -74,7 +75,7 @@ __device__ __forceinline__ float other_half_sum(float v) {
 // ---- operands ------------------------------------------------------------------------------------
 // f32 rows as matrix operands: three bf16 parts of 8 bits each, cut off one behind the other, which add up to the value exactly.
 // Of the nine products of two values' parts the six largest are taken; the others are below 2^-22 of the product.
-// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  An infinity's rest is NaN, and so is what it goes into.
+// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  An infinity's rest is NaN, and so is what it goes into, which the workgroup notices.
 struct Parts8 {
     bf16x8 part[3];
 };
@@ -185,11 +186,10 @@ struct Tile {
         return (r & 3) << 2 | ((r >> 2) & 3);
     }
     static __device__ __forceinline__ const char* piece(const char* tile, int r, int c) { return tile + r * ROW + ((c ^ swizzle(r)) << 4); }
-    static __device__ __forceinline__ float element(const char* tile, int r, int d) {
-        float x = 0.0f;
-#pragma unroll
-        for (int i = P - 1; i >= 0; --i) x += to_f32(*reinterpret_cast<const bf16_t*>(piece(tile + i * PART, r, d / 8) + d % 8 * 2));
-        return x;
+    static __device__ __forceinline__ void quad(const char* tile, int r, int d, float (&y)[4]) {  // (of bf16 rows)
+        const uint2 x = *reinterpret_cast<const uint2*>(piece(tile, r, d / 8) + d % 8 * 2);
+        y[0] = __uint_as_float(x.x << 16); y[1] = __uint_as_float(x.x & 0xffff0000u);
+        y[2] = __uint_as_float(x.y << 16); y[3] = __uint_as_float(x.y & 0xffff0000u);
     }
 
     // The rows from `first` on of a sequence's n, by TEAM waves; columns from head_dim on and rows from n on are zeros.  begin() has the loads
@@ -284,9 +284,10 @@ struct Tile {
 };
 __device__ __forceinline__ int block_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (i & 3); }
 
-// Tile::add for a block of which some places are masked, whatever the tile holds there: row by row, the places that `sees`(row) allows.
-template <typename T, int D, int N, typename F>
-__device__ __forceinline__ void add_seen(floatx16 (&acc)[D / 32], const char* tile, int row0, const floatx16& p, F sees) {
+// Tile::add one element after the other: for a block of which some places are masked, whatever the tile holds there.  Row by row, the places that
+// `sees`(row) allows; `quad`(row, d, y) gives four elements of a row.
+template <typename T, int D, typename Q, typename F>
+__device__ __forceinline__ void add_seen(floatx16 (&acc)[D / 32], const floatx16& p, Q quad, F sees) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma clang loop unroll(disable)
     for (int r = 0; r < 32; ++r) {
@@ -298,11 +299,43 @@ __device__ __forceinline__ void add_seen(floatx16 (&acc)[D / 32], const char* ti
 #pragma unroll
         for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float y = Tile<T, D, N>::element(tile, row0 + r, 32 * b + 8 * (e >> 2) + 4 * h + (e & 3));
-                acc[b][e] = seen ? __builtin_fmaf(x, y, acc[b][e]) : acc[b][e];
+            for (int e = 0; e < 4; ++e) {
+                float y[4] = {};
+                quad(r, 32 * b + 8 * e + 4 * h, y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[b][4 * e + j] = seen ? __builtin_fmaf(x, y[j], acc[b][4 * e + j]) : acc[b][4 * e + j];
             }
     }
+}
+// Parts of an infinity do not multiply as it does (0 times infinity, infinity minus infinity), so a pass over f32 rows that hold one takes
+// them as they are, from memory: the scores by the f32 instruction, in the same order and layout as Tile::product, sums by add_seen.
+template <int D, typename T>
+__device__ __forceinline__ floatx16 product_f32(const T* __restrict__ rows, long long stride, int n, const T* __restrict__ own, bool there, int pieces) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    floatx16 c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+#pragma clang loop unroll(disable)
+    for (int kc = 0; kc < D / 16; ++kc) {
+        float x[8] = {}, y[8] = {};
+        if (2 * kc + h < pieces) {
+            if ((lane & 31) < n) load8(rows + (long long)(lane & 31) * stride + (2 * kc + h) * 8, x);
+            if (there) load8(own + (2 * kc + h) * 8, y);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+    }
+    return c;
+}
+// `quad` of add_seen over n rows in memory
+template <typename T>
+__device__ __forceinline__ auto quads_of(const T* __restrict__ rows, long long stride, int n, int head_dim) {
+    return [=](int r, int d, float (&y)[4]) {
+        if (r >= n || d >= head_dim) return;
+        const Any16 x = *reinterpret_cast<const Any16*>(rows + (long long)r * stride + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = __uint_as_float(x[j]);
+    };
 }
 template <int N>
 __device__ __forceinline__ bool any_not_finite(const floatx16 (&acc)[N]) {
@@ -489,8 +522,9 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
     const T* const v = static_cast<const T*>(a.v) + (long long)s.k0 * a.v_stride + (long long)kv * a.head_dim;
     const int wave_first = TEAM == 1 ? first : first + 32 * wave, row = wave_first + (lane & 31);
     const bool there = row < s.nq;
+    const T* const q_row = static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim;
     RowsOf<T> q[Tl::KC];
-    load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
+    load_own<T, D>(q_row, there, pieces, q);
 
     // the keys that a row sees are those below its limit
     auto limit = [&](int r) { return a.causal ? min(max(r + s.ahead + 1, 0), s.nk) : s.nk; };
@@ -504,6 +538,7 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
     float m, l;
 
     auto pass = [&](auto careful) {
+        constexpr bool F32 = decltype(careful)::value && sizeof(T) == 4;
 #pragma unroll
         for (int b = 0; b < Tl::DB; ++b)
 #pragma unroll
@@ -527,7 +562,11 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
             const char* const vt = kt + BYTES;
             floatx16 p[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) p[b] = Tl::product(kt, 32 * b, q);
+            for (int b = 0; b < NB; ++b) {
+                const int r0 = t + 32 * b;
+                if constexpr (F32) p[b] = product_f32<D>(k + (long long)r0 * a.k_stride, a.k_stride, s.nk - r0, q_row, there, pieces);
+                else p[b] = Tl::product(kt, 32 * b, q);
+            }
             if (t + N > least) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -571,10 +610,15 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (decltype(careful)::value && t + N > least)
-                    add_seen<T, D, N>(acc, vt, 32 * b, p[b], [&](int r) { return t + 32 * b + r < own_limit; });
-                else
+                const int r0 = t + 32 * b;
+                auto sees = [&](int r) { return r0 + r < own_limit; };
+                if constexpr (F32) {
+                    add_seen<T, D>(acc, p[b], quads_of(v + (long long)r0 * a.v_stride, a.v_stride, s.nk - r0, a.head_dim), sees);
+                } else if (decltype(careful)::value && t + N > least) {
+                    add_seen<T, D>(acc, p[b], [&](int r, int d, float (&y)[4]) { Tl::quad(vt, 32 * b + r, d, y); }, sees);
+                } else {
                     Tl::add(acc, vt, 32 * b, Mma<T>::cols(p[b]));
+                }
             }
         };
         over_tiles<STAGES, Tl::P, TEAM>(start, end, STEP, begin, finish, use);
@@ -619,9 +663,11 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     const int wave_first = TEAM == 1 ? first : first + 32 * wave, row = wave_first + (lane & 31);
     const bool there = row < s.nq;
     const long long in_out = ((long long)(s.q0 + row) * a.heads + at.head) * a.head_dim, in_lse = (long long)at.head * a.query_rows + s.q0 + row;
+    const T* const q_row = static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim;
+    const T* const dout_row = static_cast<const T*>(a.grad_out) + in_out;
     RowsOf<T> q[Tl::KC], dout[Tl::KC];
-    load_own<T, D>(static_cast<const T*>(a.q) + (long long)(s.q0 + row) * a.q_stride + (long long)at.head * a.head_dim, there, pieces, q);
-    load_own<T, D>(static_cast<const T*>(a.grad_out) + in_out, there, pieces, dout);
+    load_own<T, D>(q_row, there, pieces, q);
+    load_own<T, D>(dout_row, there, pieces, dout);
 
     float delta = 0.0f;
 #pragma unroll
@@ -652,6 +698,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     float sum, rounded_sum;
 
     auto pass = [&](auto careful) {
+        constexpr bool F32 = decltype(careful)::value && sizeof(T) == 4;
 #pragma unroll
         for (int b = 0; b < Tl::DB; ++b)
 #pragma unroll
@@ -674,7 +721,15 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
             const char* const vt = kt + BYTES;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                floatx16 p = Tl::product(kt, 32 * b, q), dp = Tl::product(vt, 32 * b, dout);
+                const int r0 = t + 32 * b;
+                floatx16 p, dp;
+                if constexpr (F32) {
+                    p = product_f32<D>(k + (long long)r0 * a.k_stride, a.k_stride, s.nk - r0, q_row, there, pieces);
+                    dp = product_f32<D>(v + (long long)r0 * a.v_stride, a.v_stride, s.nk - r0, dout_row, there, pieces);
+                } else {
+                    p = Tl::product(kt, 32 * b, q);
+                    dp = Tl::product(vt, 32 * b, dout);
+                }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     p[i] = Mma<T>::exponential(__builtin_fmaf(p[i], c, -reference));
@@ -683,16 +738,21 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 if (t + N > least) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (t + 32 * b + block_row(i) >= own_limit) p[i] = dp[i] = 0.0f;
+                        if (r0 + block_row(i) >= own_limit) p[i] = dp[i] = 0.0f;
                 }
                 const auto ds = Mma<T>::cols(dp);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += dp[i];
                 if constexpr (sizeof(T) == 2) rounded_sum = Mma<T>::total(ds, rounded_sum);
-                if (decltype(careful)::value && t + N > least) {
-                    auto sees = [&](int r) { return t + 32 * b + r < own_limit; };
-                    add_seen<T, D, N>(acc, kt, 32 * b, dp, sees);
-                    add_seen<T, D, N>(mean, kt, 32 * b, p, sees);
+                auto sees = [&](int r) { return r0 + r < own_limit; };
+                if constexpr (F32) {
+                    auto quad = quads_of(k + (long long)r0 * a.k_stride, a.k_stride, s.nk - r0, a.head_dim);
+                    add_seen<T, D>(acc, dp, quad, sees);
+                    add_seen<T, D>(mean, p, quad, sees);
+                } else if (decltype(careful)::value && t + N > least) {
+                    auto quad = [&](int r, int d, float (&y)[4]) { Tl::quad(kt, 32 * b + r, d, y); };
+                    add_seen<T, D>(acc, dp, quad, sees);
+                    add_seen<T, D>(mean, p, quad, sees);
                 } else {
                     Tl::add(acc, kt, 32 * b, ds);
                     Tl::template add<bf16_t>(mean, kt, 32 * b, Mma<bf16_t>::cols(p));
@@ -743,8 +803,10 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     const int wave_first = TEAM == 1 ? first : first + 32 * wave, key = wave_first + (lane & 31);
     const bool there = key < s.nk;
     RowsOf<T> k[Tl::KC], v[Tl::KC];
-    load_own<T, D>(static_cast<const T*>(a.k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim, there, pieces, k);
-    load_own<T, D>(static_cast<const T*>(a.v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim, there, pieces, v);
+    const T* const k_row = static_cast<const T*>(a.k) + (long long)(s.k0 + key) * a.k_stride + (long long)kv * a.head_dim;
+    const T* const v_row = static_cast<const T*>(a.v) + (long long)(s.k0 + key) * a.v_stride + (long long)kv * a.head_dim;
+    load_own<T, D>(k_row, there, pieces, k);
+    load_own<T, D>(v_row, there, pieces, v);
 
     // the rows that see a key are those from its start on
     auto start = [&](int j) { return a.causal ? max(j - s.ahead, 0) : 0; };
@@ -755,9 +817,13 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     const int mine = TEAM == 1 ? wave : 0;
     char* const tiles_at = attention_lds + (TEAM == 1 ? wave * STAGES * STAGE : 0);
     const float c = a.scale * Mma<T>::unit;
+    const long long dout_stride = (long long)a.heads * a.head_dim;
+    auto q_of = [&](int head) { return static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim; };
+    auto dout_of = [&](int head) { return static_cast<const T*>(a.grad_out) + s.q0 * dout_stride + (long long)head * a.head_dim; };
     floatx16 dk[Tl::DB], dv[Tl::DB];
 
     auto pass = [&](auto careful) {
+        constexpr bool F32 = decltype(careful)::value && sizeof(T) == 4;
 #pragma unroll
         for (int b = 0; b < Tl::DB; ++b)
 #pragma unroll
@@ -774,9 +840,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 if constexpr (Tl::P == 3) statistic = r < s.nq ? *from : 0.0f;
                 else issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), r < s.nq ? (const void*)from : (const void*)zero_piece);
             }
-            queries.begin(to, static_cast<const T*>(a.q) + (long long)s.q0 * a.q_stride + (long long)head * a.head_dim, a.q_stride, t, s.nq, pieces);
-            gradients.begin(to + BYTES, static_cast<const T*>(a.grad_out) + ((long long)s.q0 * a.heads + head) * a.head_dim,
-                            (long long)a.heads * a.head_dim, t, s.nq, pieces);
+            queries.begin(to, q_of(head), a.q_stride, t, s.nq, pieces);
+            gradients.begin(to + BYTES, dout_of(head), dout_stride, t, s.nq, pieces);
         };
         auto finish = [&](int buf) {
             char* const to = tiles_at + buf * STAGE;
@@ -786,7 +851,7 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
             gradients.finish(to + BYTES);
         };
         auto use = [&](int buf, int i) {
-            const int t = begin + i % turns * N;
+            const int head = head0 + i / turns, t = begin + i % turns * N;
             if (t + N <= least || wave_first >= s.nk) return;
             const char* const qt = tiles_at + buf * STAGE;
             const char* const ot = qt + BYTES;
@@ -794,7 +859,15 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
             const bool masked = t < most || t + N > s.nq;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                floatx16 p = Tl::product(qt, 32 * b, k), dp = Tl::product(ot, 32 * b, v);
+                const int r0 = t + 32 * b;
+                floatx16 p, dp;
+                if constexpr (F32) {
+                    p = product_f32<D>(q_of(head) + r0 * a.q_stride, a.q_stride, s.nq - r0, k_row, there, pieces);
+                    dp = product_f32<D>(dout_of(head) + r0 * dout_stride, dout_stride, s.nq - r0, v_row, there, pieces);
+                } else {
+                    p = Tl::product(qt, 32 * b, k);
+                    dp = Tl::product(ot, 32 * b, v);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 32 * b + block_row(4 * e);
@@ -806,17 +879,20 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                         dp[4 * e + j] = p[4 * e + j] * (dp[4 * e + j] - ys[j]);
                     }
                 }
-                auto sees = [&](int r) { return t + 32 * b + r >= own_start && t + 32 * b + r < s.nq; };
+                auto sees = [&](int r) { return r0 + r >= own_start && r0 + r < s.nq; };
                 if (masked) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         if (!sees(block_row(e))) p[e] = dp[e] = 0.0f;
-                        if (t + 32 * b + block_row(e) == lone) dp[e] = 0.0f;
+                        if (r0 + block_row(e) == lone) dp[e] = 0.0f;
                     }
                 }
-                if (decltype(careful)::value && masked) {
-                    add_seen<T, D, N>(dv, ot, 32 * b, p, sees);
-                    add_seen<T, D, N>(dk, qt, 32 * b, dp, sees);
+                if constexpr (F32) {
+                    add_seen<T, D>(dv, p, quads_of(dout_of(head) + r0 * dout_stride, dout_stride, s.nq - r0, a.head_dim), sees);
+                    add_seen<T, D>(dk, dp, quads_of(q_of(head) + r0 * a.q_stride, a.q_stride, s.nq - r0, a.head_dim), sees);
+                } else if (decltype(careful)::value && masked) {
+                    add_seen<T, D>(dv, p, [&](int r, int d, float (&y)[4]) { Tl::quad(ot, 32 * b + r, d, y); }, sees);
+                    add_seen<T, D>(dk, dp, [&](int r, int d, float (&y)[4]) { Tl::quad(qt, 32 * b + r, d, y); }, sees);
                 } else {
                     Tl::add(dv, ot, 32 * b, Mma<T>::cols(p));
                     Tl::add(dk, qt, 32 * b, Mma<T>::cols(dp));
