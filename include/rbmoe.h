@@ -458,7 +458,7 @@ int rbmoe_kv_cache_read(rbmoe_kv_cache* cache, int32_t rows, void* k, int32_t k_
 /* One query row a sequence over the cache: out[i] = attention of q[i] over the first lengths[i] rows of sequence i, whose pages are
  * tables[i][0 .. table_pages).  The new row's own key is written before, and counts.  Lengths go up to `longest` (longer ones are cut), by which a
  * launch is sized: a captured graph takes the longest that its replays will see.  A table entry that is no page of the cache has no rows; a
- * sequence without any gives zeros.  The handle holds the workspace for up to max_sequences sequences, joins parts of long sequences in
+ * sequence without any gives zeros.  Infinities and NaN have the effect that f32 arithmetic gives them.  The handle holds the workspace for up to max_sequences sequences, joins parts of long sequences in
  * it, and serves any number of caches, one call after the other.  Where the parts end depends on all lengths of a call, and the last bits of its f32
  * sums with it. */
 typedef struct rbmoe_decode rbmoe_decode;

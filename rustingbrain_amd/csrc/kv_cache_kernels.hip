@@ -364,6 +364,20 @@ __device__ __forceinline__ void cut(const float (&x)[8], bf16x8 (&part)[N]) {
     }
 }
 
+// p in two parts for values that may hold infinities: both parts are positive where p is, as every part of it times infinity is infinity then.  The first is
+// cut off, so that the rest is not negative, and a rest of nothing becomes 2^-24 p, which is below what two parts keep (16 bits).
+__device__ __forceinline__ void cut_positive(const float (&x)[8], bf16x8 (&part)[2]) {
+    float rest[8];
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = fmaxf(x[i] - __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u), x[i] * 0x1p-24f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // the upper halves of two
+        w[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302);
+    part[0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+    part[1] = __builtin_bit_cast(bf16x8, make_uint4(pack2(rest[0], rest[1]), pack2(rest[2], rest[3]), pack2(rest[4], rest[5]), pack2(rest[6], rest[7])));
+}
+
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
 
 template <typename T, typename C, int W>
@@ -592,7 +606,8 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void decode_attention_ke
                             y[i] = !ragged || 8 * h + i < left ? y[i] * (i % 4 == 0 ? f.x : i % 4 == 1 ? f.y : i % 4 == 2 ? f.z : f.w) : 0.0f;
                         }
                     }
-                    cut<X::PP>(y, part[h]);
+                    if constexpr (sizeof(C) == 2) cut_positive(y, part[h]);
+                    else cut<X::PP>(y, part[h]);
                 }
 #pragma unroll
                 for (int k = 0; k < VP; ++k) {
