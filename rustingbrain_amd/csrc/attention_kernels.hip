@@ -28,7 +28,9 @@
 //     as long as they do; three workgroups a unit instead of two give 8 %.
 //   backward, 8192 rows, 16 heads of 128, bf16: 0.65 ms (dq, with its fourth product) and 0.77 (dk, dv), 840 and 710 TFLOP/s of the products taken:
 //     registers leave one wave a SIMD, which waits for its exponentials.
-//   short or ragged calls: the longest rows' workgroups; f32 rows: 6 products for one, and cutting p and ds in parts.
+//   short or ragged calls: the longest rows' workgroups; f32 rows: 6 products for one, and cutting p and ds in parts.  (Parts rounded to nearest, small
+//     products and blocks summed apart: errors of 1.1 to 1.5e-7 of the result forward, 3.3 to 5e-7 of the gradients, where f32 products by the library have
+//     2 to 6e-7 and 5e-7 to 1.5e-6; 2 % of the time forward and 10 backward, 6 x 2048 and 3 x 700 rows of 8 heads of 64.)
 #include "attention_kernels.h"
 
 #include <algorithm>
@@ -73,9 +75,10 @@ __device__ __forceinline__ float other_half_sum(float v) {
 }
 
 // ---- operands ------------------------------------------------------------------------------------
-// f32 rows as matrix operands: three bf16 parts of 8 bits each, cut off one behind the other, which add up to the value exactly.
-// Of the nine products of two values' parts the six largest are taken; the others are below 2^-22 of the product.
-// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  An infinity's rest is NaN, and so is what it goes into, which the workgroup notices.
+// f32 rows as matrix operands: three bf16 parts of 8 bits each, each the rest of those in front rounded to nearest, which add up to the value exactly.
+// Of the nine products of two values' parts the six largest are taken; the others are below 2^-25 of the product and of any sign.
+// (32 x 32 x 16 of them take 192 cycles, the f32 instruction 512.)  An infinity's rest is NaN, and so is what it goes into, which the workgroup
+// notices, as it does values that round to one (above 3.39e38).
 struct Parts8 {
     bf16x8 part[3];
 };
@@ -86,14 +89,13 @@ __device__ __forceinline__ Parts8 cut8(const float (&x)[8]) {
     for (int i = 0; i < 8; ++i) rest[i] = x[i];
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)  // the upper halves of two
-            w[i] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * i + 1]), __float_as_uint(rest[2 * i]), 0x07060302);
-        r.part[n] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+        const uint4 w = make_uint4(pack2(rest[0], rest[1]), pack2(rest[2], rest[3]), pack2(rest[4], rest[5]), pack2(rest[6], rest[7]));
+        r.part[n] = __builtin_bit_cast(bf16x8, w);
         if (n == 2) break;
+        float back[8];
+        Vec16<bf16_t>::widen(w, back);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xffff0000u);
+        for (int i = 0; i < 8; ++i) rest[i] -= back[i];
     }
     return r;
 }
@@ -238,48 +240,68 @@ struct Tile {
     // The product of 32 of the tile's rows with the wave's own: register i of lane l holds tile row 8 (i / 4) + 4 (l / 32) + i % 4, own row l % 32.
     static __device__ __forceinline__ floatx16 product(const char* tile, int row0, const RowsOf<T> (&own)[KC]) {
         const int lane = threadIdx.x & 63;
-        floatx16 c;
+        floatx16 c, small;  // (sums of their own: the large one is rounded once a step, not six times)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+        for (int i = 0; i < 16; ++i) c[i] = small[i] = 0.0f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
             bf16x8 rows[P];
 #pragma unroll
             for (int i = 0; i < P; ++i) rows[i] = *reinterpret_cast<const bf16x8*>(piece(tile + i * PART, row0 + (lane & 31), 2 * kc + (lane >> 5)));
 #pragma unroll
-            for (int s = P - 1; s >= 0; --s)  // small ones first
+            for (int s = P - 1; s > 0; --s)
 #pragma unroll
-                for (int i = 0; i <= s; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows[i], Mma<T>::part(own[kc], s - i), c, 0, 0, 0);
+                for (int i = 0; i <= s; ++i) small = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows[i], Mma<T>::part(own[kc], s - i), small, 0, 0, 0);
+            c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rows[0], Mma<T>::part(own[kc], 0), c, 0, 0, 0);
         }
+        if constexpr (P > 1)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c[i] += small[i];
         return c;
     }
-    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]; of M's parts (bf16_t: the first ones alone)
+    // acc[d][own] += sum over the block's 32 rows r of tile[r][d] p[r][own]; of M's parts (bf16_t: the first ones alone).  Several products a term are
+    // summed up over the block first, so that the sum over all blocks is rounded once a block.
     template <typename M = T>
     static __device__ __forceinline__ void add(floatx16 (&acc)[DB], const char* tile, int row0, const typename Mma<M>::Cols& p) {
         constexpr int P = Mma<M>::P;
         const int lane = threadIdx.x & 63, h = lane >> 5, j = (lane >> 2) & 3;
         const int c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), in = (lane & 1) * 8;
+        auto columns = [&](int k, int b, int part) {
+            const int r = row0 + 16 * k + 4 * h + j;
+            union {
+                v4i16 x[2];
+                bf16x8 v;
+            } u;
+            u.x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(piece(tile + part * PART, r, 4 * b + c0) + in));
+            u.x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(piece(tile + part * PART, r + 8, 4 * b + c0) + in));
+            return u.v;
+        };
+        if constexpr (P == 1) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int b = 0; b < DB; ++b)
+                    acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(columns(k, b, 0), Mma<M>::part(p, k, 0), acc[b], 0, 0, 0);
+        } else {
 #pragma unroll
             for (int b = 0; b < DB; ++b) {
-                const int r = row0 + 16 * k + 4 * h + j;
-                bf16x8 cols[P];
+                floatx16 c;
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    union {
-                        v4i16 x[2];
-                        bf16x8 v;
-                    } u;
-                    u.x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(piece(tile + i * PART, r, 4 * b + c0) + in));
-                    u.x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(piece(tile + i * PART, r + 8, 4 * b + c0) + in));
-                    cols[i] = u.v;
+                for (int i = 0; i < 16; ++i) c[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    bf16x8 cols[P];
+#pragma unroll
+                    for (int i = 0; i < P; ++i) cols[i] = columns(k, b, i);
+#pragma unroll
+                    for (int s = P - 1; s >= 0; --s)  // small ones first
+#pragma unroll
+                        for (int i = 0; i <= s; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols[i], Mma<M>::part(p, k, s - i), c, 0, 0, 0);
                 }
 #pragma unroll
-                for (int s = P - 1; s >= 0; --s)
-#pragma unroll
-                    for (int i = 0; i <= s; ++i) acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cols[i], Mma<M>::part(p, k, s - i), acc[b], 0, 0, 0);
+                for (int i = 0; i < 16; ++i) acc[b][i] += c[i];
             }
+        }
     }
 };
 __device__ __forceinline__ int block_row(int i) { return 8 * (i >> 2) + 4 * ((threadIdx.x >> 5) & 1) + (i & 3); }
@@ -602,11 +624,13 @@ __global__ __launch_bounds__(kThreads, D * sizeof(T) > 256 || (sizeof(T) == 4 &&
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                float sum = 0.0f;  // of the block: the sum over all is rounded once a block
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     p[b][i] = Mma<T>::exponential(p[b][i]);
-                    l += p[b][i];
+                    sum += p[b][i];
                 }
+                l += sum;
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
