@@ -46,7 +46,13 @@ namespace {
 constexpr int kThreads = 256, kWaves = 4;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-__device__ uint32_t zero_piece[4];  // what is staged for rows and columns that are not there
+// What is loaded for rows and columns that are not there.  (A branch around the load would do too, but not in kernels that fill their registers: at the
+// end of a region that only some lanes run, the compiler may save a register before the others are back, and theirs is lost.)
+__device__ __attribute__((aligned(16))) uint32_t zero_piece[8];
+template <typename T>
+__device__ __forceinline__ const T* or_zeros(const T* p, bool there) {
+    return there ? p : reinterpret_cast<const T*>(zero_piece);
+}
 
 typedef uint32_t Any16 __attribute__((ext_vector_type(4), aligned(2), may_alias));
 typedef uint32_t Any8 __attribute__((ext_vector_type(2), aligned(2), may_alias));
@@ -209,14 +215,11 @@ struct Tile {
                 const bool there = first + r < n && c < pieces;
                 const T* const src = base + (long long)(first + r) * stride + c * 8;
                 if constexpr (P == 3) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-                    if (there) load8(src, x[i]);
+                    load8(or_zeros(src, there), x[i]);
                 } else if constexpr (A) {
-                    issue_dma(lds_address(tile) + at * 16, there ? (const void*)src : (const void*)zero_piece);
+                    issue_dma(lds_address(tile) + at * 16, or_zeros(src, there));
                 } else {
-                    raw[i] = Any16{0, 0, 0, 0};
-                    if (there) raw[i] = *reinterpret_cast<const Any16*>(src);
+                    raw[i] = *reinterpret_cast<const Any16*>(or_zeros(src, there));
                 }
             }
         }
@@ -339,11 +342,9 @@ __device__ __forceinline__ floatx16 product_f32(const T* __restrict__ rows, long
     for (int i = 0; i < 16; ++i) c[i] = 0.0f;
 #pragma clang loop unroll(disable)
     for (int kc = 0; kc < D / 16; ++kc) {
-        float x[8] = {}, y[8] = {};
-        if (2 * kc + h < pieces) {
-            if ((lane & 31) < n) load8(rows + (long long)(lane & 31) * stride + (2 * kc + h) * 8, x);
-            if (there) load8(own + (2 * kc + h) * 8, y);
-        }
+        float x[8], y[8];
+        load8(or_zeros(rows + (long long)(lane & 31) * stride + (2 * kc + h) * 8, (lane & 31) < n && 2 * kc + h < pieces), x);
+        load8(or_zeros(own + (2 * kc + h) * 8, there && 2 * kc + h < pieces), y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
     }
@@ -353,8 +354,7 @@ __device__ __forceinline__ floatx16 product_f32(const T* __restrict__ rows, long
 template <typename T>
 __device__ __forceinline__ auto quads_of(const T* __restrict__ rows, long long stride, int n, int head_dim) {
     return [=](int r, int d, float (&y)[4]) {
-        if (r >= n || d >= head_dim) return;
-        const Any16 x = *reinterpret_cast<const Any16*>(rows + (long long)r * stride + d);
+        const Any16 x = *reinterpret_cast<const Any16*>(or_zeros(rows + (long long)r * stride + d, r < n && d < head_dim));
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = __uint_as_float(x[j]);
     };
@@ -378,12 +378,11 @@ __device__ __forceinline__ void load_own(const T* __restrict__ row, bool there, 
     for (int kc = 0; kc < D / 16; ++kc) {
         const bool in = there && 2 * kc + h < pieces;
         if constexpr (sizeof(T) == 4) {
-            float x[8] = {};
-            if (in) load8(row + (2 * kc + h) * 8, x);
+            float x[8];
+            load8(or_zeros(row + (2 * kc + h) * 8, in), x);
             own[kc] = cut8(x);
         } else {
-            Any16 x = {0, 0, 0, 0};
-            if (in) x = *reinterpret_cast<const Any16*>(row + (2 * kc + h) * 8);
+            const Any16 x = *reinterpret_cast<const Any16*>(or_zeros(row + (2 * kc + h) * 8, in));
             own[kc] = __builtin_bit_cast(bf16x8, x);
         }
     }
@@ -696,15 +695,15 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
     float delta = 0.0f;
 #pragma unroll
     for (int kc = 0; kc < Tl::KC; ++kc) {
-        if (!there || 2 * kc + h >= pieces) continue;
+        const bool in = there && 2 * kc + h < pieces;
         float x[8], y[8];
-        load8(static_cast<const T*>(a.out) + in_out + (2 * kc + h) * 8, x);
-        load8(static_cast<const T*>(a.grad_out) + in_out + (2 * kc + h) * 8, y);
+        load8(or_zeros(static_cast<const T*>(a.out) + in_out + (2 * kc + h) * 8, in), x);
+        load8(or_zeros(dout_row + (2 * kc + h) * 8, in), y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) delta = __builtin_fmaf(x[i], y[i], delta);
     }
     delta = other_half_sum(delta);
-    float reference = there ? a.lse[in_lse] * Mma<T>::unit : 0.0f;
+    float reference = *or_zeros(a.lse + in_lse, there) * Mma<T>::unit;
     asm volatile("" : "+v"(reference));  // (as in load_own)
 
     auto limit = [&](int r) { return a.causal ? min(max(r + s.ahead + 1, 0), s.nk) : s.nk; };
@@ -861,8 +860,8 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
             if (TEAM == 1 || wave < 2 * N / 64) {  // references, then deltas
                 const int at = TEAM == 1 ? lane : threadIdx.x, r = t + at % N;
                 const float* const from = a.delta + (at < N ? 0 : (long long)a.heads * a.query_rows) + (long long)head * a.query_rows + s.q0 + r;
-                if constexpr (Tl::P == 3) statistic = r < s.nq ? *from : 0.0f;
-                else issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), r < s.nq ? (const void*)from : (const void*)zero_piece);
+                if constexpr (Tl::P == 3) statistic = *or_zeros(from, r < s.nq);
+                else issue_dma_word(lds_address(to) + 2 * BYTES + (TEAM == 1 ? 0 : wave * 256), or_zeros(from, r < s.nq));
             }
             queries.begin(to, q_of(head), a.q_stride, t, s.nq, pieces);
             gradients.begin(to + BYTES, dout_of(head), dout_stride, t, s.nq, pieces);
