@@ -1,5 +1,5 @@
 """The accuracy that the kernels are held to (attention_precision) tells arithmetics apart: three parts of operands and six products pass, two parts and
-three products, or fewer, do not.  No GPU."""
+three products, or fewer, do not; bf16 rows whose ds are not mended do not.  No GPU."""
 import numpy as np
 import pytest
 
@@ -30,3 +30,18 @@ def test_parts_of_operands(nq, nk, d):
     for parts, dropped in ((2, 2), (2, 3), (1, 1)):
         bad = ap.as_exact_as_f32(ap.formulas(*wide, mask, float(scale), ap.in_parts(parts, dropped)), f32, want)
         assert set(bad) == set(ap.NAMES), (parts, bad)
+
+
+@pytest.mark.parametrize("nq,nk,d", [(300, 300, 64), (600, 600, 128), (130, 700, 40)])
+def test_ds_that_do_not_add_up_to_nothing(nq, nk, d):
+    q, k, v, go = (ap.rounded(a) for a in ap.rows(np.random.default_rng(nq + d), nq, nk, d))
+    mask, scale = ao.seen(nq, nk, True), d ** -0.5
+    want = ap.formulas(q, k, v, go, mask, scale)
+    model, plain = (ap.bf16_rounded(q, k, v, go, mask, scale, mended) for mended in (True, False))
+    got = {n: ap.rounded(a) for n, a in model.items()}
+    assert not ap.as_exact_as_bf16(got, model, want)
+    for name in ("out", "grad_q", "grad_k", "grad_v"):
+        err, norm = ap.error(got[name], want[name])
+        assert err <= 0.0027 * norm, (name, err / norm)  # (sqrt(2) roundings of the result, and what a few keys a row add)
+    bad = ap.as_exact_as_bf16({n: ap.rounded(a) for n, a in plain.items()}, model, want)
+    assert "grad_q" in bad, bad  # (keys share a direction, queries do not: grad_k hardly shows it)

@@ -1,4 +1,5 @@
-"""How exact attention of f32 rows is: beside the same formulas in f32 (attention_precision has the tolerance)."""
+"""How exact attention is: f32 rows beside the same formulas in f32, bf16 rows beside what rounding p, ds and the results costs (attention_precision has
+the tolerances)."""
 import numpy as np
 import pytest
 
@@ -9,18 +10,18 @@ from test_gpu_attention import Problem
 pytestmark = pytest.mark.gpu
 
 
-def per_head(p):
-    """(f32's results, those of 64 bits), laid out like the kernels'; the gradients of a kv head are summed over its group in that arithmetic."""
+def per_head(p, *arithmetics):
+    """What each of [(type, formulas)] gives, laid out like the kernels'; the gradients of a kv head are summed over its group in that type."""
     group, scale = p.h // p.kv, np.float32(p.scale)
     got = []
-    for kind in (np.float32, np.float64):
+    for kind, formulas in arithmetics:
         r = {"out": np.zeros(p.q.shape, kind), "lse": np.zeros((p.h, p.rows), kind), "grad_q": np.zeros(p.q.shape, kind),
              "grad_k": np.zeros(p.k.shape, kind), "grad_v": np.zeros(p.v.shape, kind)}
         for b, n, kb, m in zip(p.begin, p.counts, p.key_begin, p.key_counts):
             mask = ao.seen(n, m, p.causal)
             for h in range(p.h):
-                f = ap.formulas(*(a.astype(kind) for a in (p.q[b:b + n, h], p.k[kb:kb + m, h // group], p.v[kb:kb + m, h // group], p.go[b:b + n, h])), mask,
-                                kind(scale))
+                f = formulas(*(a.astype(kind) for a in (p.q[b:b + n, h], p.k[kb:kb + m, h // group], p.v[kb:kb + m, h // group], p.go[b:b + n, h])), mask,
+                             kind(scale))
                 r["out"][b:b + n, h], r["lse"][h, b:b + n], r["grad_q"][b:b + n, h] = f["out"], f["lse"], f["grad_q"]
                 r["grad_k"][kb:kb + m, h // group] += f["grad_k"]
                 r["grad_v"][kb:kb + m, h // group] += f["grad_v"]
@@ -28,13 +29,25 @@ def per_head(p):
     return got
 
 
-@pytest.mark.parametrize("counts,earlier,heads,causal", [
+CASES = [
     ([300], 0, (2, 1, 64), True), ([1500], 0, (1, 1, 64), True), ([77, 200, 1], 0, (8, 2, 64), True), ([1100], 0, (2, 1, 128), True),
     ([33], 2000, (2, 2, 128), True), ([20, 40], [900, 1500], (4, 2, 64), True), ([300, 65], 0, (3, 3, 40), False), ([260], 0, (2, 2, 80), True),
-    ([130] * 40, 0, (16, 8, 64), True), ([150] * 30, 0, (16, 16, 104), True)])
+    ([130] * 40, 0, (16, 8, 64), True), ([150] * 30, 0, (16, 16, 104), True)]
+
+
+@pytest.mark.parametrize("counts,earlier,heads,causal", CASES)
 def test_f32_rows_are_as_exact_as_f32(device, counts, earlier, heads, causal):
     p = Problem(device, counts, earlier, heads, "f32", causal)
-    f32, want = per_head(p)
+    f32, want = per_head(p, (np.float32, ap.formulas), (np.float64, ap.formulas))
     got = {**p.forward(), **p.backward()}
     assert not ap.as_exact_as_f32(got, f32, want)
+    p.op.close()
+
+
+@pytest.mark.parametrize("counts,earlier,heads,causal", CASES)
+def test_bf16_rows_lose_what_rounding_costs(device, counts, earlier, heads, causal):
+    p = Problem(device, counts, earlier, heads, "bf16", causal)
+    model, want = per_head(p, (np.float64, ap.bf16_rounded), (np.float64, ap.formulas))
+    got = {**p.forward(), **p.backward()}
+    assert not ap.as_exact_as_bf16(got, model, want)
     p.op.close()
