@@ -373,5 +373,9 @@ void rbmoe_internal_attention_sequence(int32_t query_begin, int32_t query_count,
 int rbmoe_internal_decode_ranges(int32_t sequences, int32_t kv_heads, int32_t group, int32_t longest) {
     return decode_plan(sequences, kv_heads, group, longest).ranges;
 }
+// And for how many parts of heads the workspace of a handle for so many sequences has room.
+int64_t rbmoe_internal_decode_parts(int32_t max_sequences, int32_t kv_heads, int32_t group) {
+    return (int64_t)decode_partials(max_sequences, kv_heads, group);
+}
 
 }  // extern "C"
