@@ -90,3 +90,35 @@ def test_infinite_gradients(device, dtype, heads, copies):
           {name: (np.where(c, want[name][0], 0), want[name][1]) for name, c in clean.items()}, dtype)
     assert group >= 1
     p.op.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,copies", [((4, 2, 64), 1), ((8, 8, 104), 40)])
+def test_rows_side_by_side_off_their_boundaries(device, dtype, heads, copies):
+    """q, k and v in one array that starts three elements off, rows of nothing between the sequences."""
+    n = 140
+    p = Problem(device, [n] * copies, 0, heads, dtype, gap=2, shift=3, fused=True)
+    want = p.wanted()
+    first, group = p.begin[-1], heads[0] // heads[1]
+    at = (p.h + p.kv) * p.d + 5  # column 5 of kv head 0's values
+    both = np.concatenate([a.reshape(p.rows, -1) for a in (p.q, p.k, p.v)] + [np.full((p.rows, 8), np.nan, np.float32)], axis=1)
+    clean = p.all
+    both[first + 90, at], both[first + 91, at + 1] = -INF, INF
+    p.all = Array(device, both.shape, dtype, both, 3)
+    got = p.forward()
+    bad = ~np.isfinite(got["out"]) & ~np.isnan(want["out"][0])
+    assert (got["out"][first + 90:first + n, :group, 5] == -INF).all() and (got["out"][first + 91:first + n, :group, 6] == INF).all()
+    assert bad.sum() == group * (50 + 49)
+    check({"out": np.where(bad, 0, got["out"]), "lse": got["lse"]}, {"out": (np.where(bad, 0, want["out"][0]), want["out"][1]), "lse": want["lse"]}, dtype)
+    p.all = clean
+    p.forward()
+    go = p.go.copy()
+    go[first + 90, 0, 2] = INF
+    p.dgo = Array(device, go.shape, dtype, go, 3)
+    got = p.backward()
+    assert (got["grad_v"][first:first + 91, 0, 2] == INF).all()
+    spoilt = {name: np.zeros(a.shape, bool) for name, a in got.items()}
+    spoilt["grad_q"][first + 90, 0] = spoilt["grad_k"][first:first + 91, 0] = spoilt["grad_v"][first:first + 91, 0, 2] = True
+    check({name: np.where(s, 0, got[name]) for name, s in spoilt.items()},
+          {name: (np.where(s, 0, want[name][0]), want[name][1]) for name, s in spoilt.items()}, dtype)
+    p.op.close()
