@@ -11,7 +11,9 @@
 // in the order in which the next product takes them as its B operand: scores never leave registers, and no lane hands a value to another
 // except the row statistics.  The second product needs the tile with rows and columns exchanged, which the transposing LDS read gives.  For
 // bf16 rows p and ds are rounded to bf16 (the matrix cores take bf16 operands): half a step a term at random, no more than the rounding of the result
-// itself; their sums, the running maximum and sum of the softmax and all accumulators are f32.
+// itself, 0.235 % of a gradient in all for 0.166 %; their sums, the running maximum and sum of the softmax and all accumulators are f32.  (The sum that
+// the forward divides by is that of the unrounded p, which lse needs.  One of the rounded p beside it takes a tenth off what rounding p costs, and 4 to 6 %
+// of the time: spilled registers.)
 //
 // The backward pass takes ds = p (dp - delta) twice, from the queries' side and from the keys', instead of adding one side's sums in
 // memory: eight products where five would do, but the same bits from the same call, and no f32 gradients that pass through memory.
@@ -21,16 +23,17 @@
 // on the diagonal row by row, f32 rows, whose parts make NaN of an infinity, leave the parts alone (product_f32).  6 x 2048 rows of 8 heads of 64 with
 // a NaN in the first value of each: 1.5 ms where clean ones take 0.12; 8192 bf16 rows of 16 heads of 128, backward: 4.9 for 1.5.
 //
-// What bounds them (a large bf16 product by the library reaches 1370 TFLOP/s, an f32 one 153):
-//   forward, 16384 rows, 16 heads of 128, bf16, causal: 1.14 ms, 965 TFLOP/s.  A wave reads every tile from LDS whole, which takes as many cycles
-//     of the LDS as the products take of the matrix cores; both are busy seven cycles of ten.
+// What bounds them (a large bf16 product by the library reaches 1370 TFLOP/s, an f32 one 153; times of long calls differ by a tenth from card to card):
+//   forward, 16384 rows, 16 heads of 128, bf16, causal: 1.14 to 1.28 ms, 860 to 965 TFLOP/s.  A wave reads every tile from LDS whole, which takes as many
+//     cycles of the LDS as the products take of the matrix cores; both are busy seven cycles of ten.
 //   heads of 64 (8 x 2048 rows, 8 heads): 52 us, 660 TFLOP/s: a block has half the products and as many exponentials, which take
 //     as long as they do; three workgroups a unit instead of two give 8 %.
-//   backward, 8192 rows, 16 heads of 128, bf16: 0.65 ms (dq, with its fourth product) and 0.77 (dk, dv), 840 and 710 TFLOP/s of the products taken:
+//   backward, 8192 rows, 16 heads of 128, bf16: 0.59 ms (dq, with its fourth product) and 0.75 (dk, dv), 940 and 730 TFLOP/s of the products taken:
 //     registers leave one wave a SIMD, which waits for its exponentials.
 //   short or ragged calls: the longest rows' workgroups; f32 rows: 6 products for one, and cutting p and ds in parts.  (Parts rounded to nearest, small
 //     products and blocks summed apart: errors of 1.1 to 1.5e-7 of the result forward, 3.3 to 5e-7 of the gradients, where f32 products by the library have
-//     2 to 6e-7 and 5e-7 to 1.5e-6; 2 % of the time forward and 10 backward, 6 x 2048 and 3 x 700 rows of 8 heads of 64.)
+//     2 to 6e-7 and 5e-7 to 1.5e-6.  6 x 2048 rows of 8 heads of 64 117 us, as before with parts cut off; backward of 3 x 700 72 for 67.  Heads of 128: 4096
+//     rows of 16 heads 457 us, 150 TFLOP/s.)
 #include "attention_kernels.h"
 
 #include <algorithm>
@@ -483,7 +486,8 @@ constexpr int tile_rows() {
     return sizeof(T) == 2 && TEAM == 4 && !(GRAD_Q && D == 64) ? 64 : 32;
 }
 // Stages of tiles.  TEAM 4: two, one is filled while the other is used.  TEAM 1: one, where workgroups beside this one on its compute unit are busy
-// meanwhile, or the next tile waits in registers; two for kernels whose registers leave room for one workgroup (ALONE).
+// meanwhile, or the next tile waits in registers; two for kernels whose registers leave room for one workgroup (ALONE).  (us with one / two, bf16: heads of 64,
+// backward of 8 sequences up to 2048 rows 158 / 161, of 512 rows 22.8 / 22.9, forward of 2048 rows 17.1 / 16.2; heads of 128, backward of 8192 rows 1356 / 1338.)
 template <typename T, int D, int TEAM, bool ALONE>
 constexpr int tile_stages() {
     return TEAM == 4 || (ALONE && sizeof(T) == 2 && D == 128) ? 2 : 1;
@@ -985,9 +989,10 @@ hipError_t with_kernel(bool bf16, int head_dim, bool few, bool aligned, F f) {
 // Workgroups of 128 rows below which 32 rows make one.  Two of them fill a compute unit, so 512 fill the device.  us with teams of 1 / 4: 5 bf16 prompts
 // behind 4000 keys, 32 heads of 128 (800 workgroups) 188 / 147; keys' gradients of 8 sequences up to 2048 rows, 2 kv heads of 64 (256) 92 / 190.
 constexpr int kFew = 512;
-// Workgroups of 32 keys below which a group's heads get their own.  us with / without: 2 x 2048 rows, 8 heads of 64, bf16 (256 workgroups) 74 / 100, 4 x 1024
-// f32 175 / 200, 8 x 512 bf16 (256, short ones) 44 / 41; 512 rows, 32 heads of 128 (128) 56 / 55, 1024 (256) 124 / 112: heads of 128 leave room
-// for one workgroup a unit.
+// Workgroups of 32 keys below which a group's heads get their own (half as many for heads of 128, which leave room for one workgroup a unit).  us of the
+// backward pass with / without: 8 heads of 64 in groups of 4, bf16: 2 x 2048 rows (256 workgroups) 76 / 97, 1 x 512 23 / 31, 8 x 512 (256, short ones) 46 / 43;
+// f32: 4 x 1024 193 / 224.  Heads of 128 in groups of 4: 1 x 512 (64) bf16 35 / 45, f32 193 / 451; 1 x 1024 (128) bf16 65 / 82; 1 x 64 of 32 heads (16) 24 / 22, where the
+// third launch shows.
 constexpr int kShared = 512;
 // Whether a launch over `longest` rows of `heads` heads a sequence would have few workgroups of 128 rows.
 bool few_workgroups(const AttentionCall& a, int longest, int heads) { return (long long)((longest + 127) / 128) * heads * a.sequences < kFew; }

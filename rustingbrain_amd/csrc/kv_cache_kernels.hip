@@ -4,7 +4,8 @@
 // stored * scale.  (127 x is exact for bf16 rows, so one division decides the rounding, and ties are ties.)  A row with an
 // infinity or NaN reads back as NaN whole.
 //
-// All of it is bound by memory (a large copy moves 4.9 TB/s): 23165 bf16 rows of 8 x 128 to 8 bits and back 57 us, 5.0 TB/s; new rows over 4 x 131072 cached
+// All of it is bound by memory (a large copy moves 4.9 TB/s): 23165 bf16 rows of 8 x 128 to 8 bits and back 65 us, 4.4 TB/s (57 where
+// the same rows come again, out of the Infinity Cache), f32 rows as they are 180, 4.2 TB/s, to 8 bits 119; new rows over 4 x 131072 cached
 // ones, bf16, 8 kv heads of 128, 192 us, 5.6 TB/s; over 64 sequences up to 8192 rows in 8 bits 114 us, 4.3 TB/s (5.0 without the new rows' write and the
 // join).  Small calls: launches of 2 to 8 us.
 #include "kv_cache_kernels.h"
