@@ -420,7 +420,7 @@ int rbmoe_get_weight(rbmoe_layer* layer, int32_t which, int32_t expert, float* h
  * (forward only), not queries.
  *   out  [query_rows, heads, head_dim] without gaps      lse [heads, query_rows] f32 or NULL
  * Sums and statistics are f32.  f32 rows are multiplied in parts that keep their 24 bits, and results are as exact as with f32 products; bf16 rows
- * round exp(s_ij - m) to bf16 for the product with v, and p and ds for the gradients. */
+ * round exp(s_ij - m) to bf16 for the product with v, and p and ds for the gradients (sequences of up to 32 rows or keys: to 16 bits). */
 typedef struct rbmoe_attention rbmoe_attention;
 /* backward_rows: the most query rows of a backward pass (0: forward only): 8 bytes a row and head, and for the first 16384 / kv_heads rows of
  * heads in groups 8 * head_dim bytes a row and head more, counted against the budget. */

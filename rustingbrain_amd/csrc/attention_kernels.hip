@@ -11,7 +11,7 @@
 // in the order in which the next product takes them as its B operand: scores never leave registers, and no lane hands a value to another
 // except the row statistics.  The second product needs the tile with rows and columns exchanged, which the transposing LDS read gives.  For
 // bf16 rows p and ds are rounded to bf16 (the matrix cores take bf16 operands): half a step a term at random, no more than the rounding of the result
-// itself, 0.235 % of a gradient in all for 0.166 %; their sums, the running maximum and sum of the softmax and all accumulators are f32.  (The sum that
+// itself, 0.235 % of a gradient in all for 0.166 % (short sequences: in two parts, kShort); their sums, the running maximum and sum of the softmax and all accumulators are f32.  (The sum that
 // the forward divides by is that of the unrounded p, which lse needs.  One of the rounded p beside it takes a tenth off what rounding p costs, and 4 to 6 %
 // of the time: spilled registers.)
 //
@@ -127,6 +127,17 @@ struct Mma<bf16_t> {
             r.c[i] = __builtin_bit_cast(bf16x8, make_uint4(pack2(p[8 * i], p[8 * i + 1]), pack2(p[8 * i + 2], p[8 * i + 3]),
                                                            pack2(p[8 * i + 4], p[8 * i + 5]), pack2(p[8 * i + 6], p[8 * i + 7])));
         return r;
+    }
+    static __device__ __forceinline__ Cols rest(const floatx16& p, const Cols& rounded) {  // what rounding left, rounded
+        floatx16 r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float back[8];
+            Vec16<bf16_t>::widen(__builtin_bit_cast(uint4, rounded.c[i]), back);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[8 * i + j] = p[8 * i + j] - back[j];
+        }
+        return cols(r);
     }
     static __device__ __forceinline__ float total(const Cols& p, float sum) {  // of the lane's own values
         typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
@@ -496,6 +507,12 @@ template <typename T, int D, int TEAM, int N, bool ALONE>
 constexpr int tiles_lds(int extra) {  // of two tiles of N rows and `extra` bytes a stage
     return (kWaves / TEAM) * tile_stages<T, D, TEAM, ALONE>() * (2 * Tile<T, D, N>::BYTES + extra);
 }
+// bf16 sequences of so few rows or keys take p and ds in two parts for the gradients, 16 bits: a few roundings decide there and do not even out (sequences of two
+// rows were up to 0.3 % off, 1.9 times the rounding of the result).  For all sequences it would be 0.166 % instead of 0.235, and a quarter of the time more:
+// 8192 rows of 16 heads of 128 1.68 ms for 1.34, 8 x 2048 of 8 heads of 64 195 us for 158.
+constexpr int kShort = 32;
+__device__ __forceinline__ bool few_terms(const Sequence& s) { return min(s.nq, s.nk) <= kShort; }
+
 __device__ __forceinline__ void wait_for_tile(bool common) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this wave's part of the tile has landed, its reads of the other stage are done
     if (common) __syncthreads();                                 // and the other waves'
@@ -770,7 +787,14 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                 const auto ds = Mma<T>::cols(dp);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += dp[i];
-                if constexpr (sizeof(T) == 2) rounded_sum = Mma<T>::total(ds, rounded_sum);
+                if constexpr (sizeof(T) == 2) {
+                    rounded_sum = Mma<T>::total(ds, rounded_sum);
+                    if (!decltype(careful)::value && few_terms(s)) {
+                        const auto rest = Mma<T>::rest(dp, ds);
+                        rounded_sum = Mma<T>::total(rest, rounded_sum);
+                        Tl::add(acc, kt, 32 * b, rest);
+                    }
+                }
                 auto sees = [&](int r) { return r0 + r < own_limit; };
                 if constexpr (F32) {
                     auto quad = quads_of(k + (long long)r0 * a.k_stride, a.k_stride, s.nk - r0, a.head_dim);
@@ -921,8 +945,14 @@ __global__ __launch_bounds__(kThreads, D == 128 || sizeof(T) == 4 ? 1 : 2) void 
                     add_seen<T, D>(dv, p, [&](int r, int d, float (&y)[4]) { Tl::quad(ot, 32 * b + r, d, y); }, sees);
                     add_seen<T, D>(dk, dp, [&](int r, int d, float (&y)[4]) { Tl::quad(qt, 32 * b + r, d, y); }, sees);
                 } else {
-                    Tl::add(dv, ot, 32 * b, Mma<T>::cols(p));
-                    Tl::add(dk, qt, 32 * b, Mma<T>::cols(dp));
+                    const auto ps = Mma<T>::cols(p), ds = Mma<T>::cols(dp);
+                    Tl::add(dv, ot, 32 * b, ps);
+                    Tl::add(dk, qt, 32 * b, ds);
+                    if constexpr (sizeof(T) == 2)
+                        if (!decltype(careful)::value && few_terms(s)) {
+                            Tl::add(dv, ot, 32 * b, Mma<T>::rest(p, ps));
+                            Tl::add(dk, qt, 32 * b, Mma<T>::rest(dp, ds));
+                        }
                 }
             }
         };

@@ -1,5 +1,5 @@
-"""How exact attention is: f32 rows beside the same formulas in f32, bf16 rows beside what rounding p, ds and the results costs (attention_precision has
-the tolerances)."""
+"""How exact attention is: f32 rows beside the same formulas in f32, bf16 rows beside what rounding p, ds and the results costs, short
+sequences of them beside what rounding the results alone costs (attention_precision has the tolerances)."""
 import numpy as np
 import pytest
 
@@ -50,4 +50,18 @@ def test_bf16_rows_lose_what_rounding_costs(device, counts, earlier, heads, caus
     model, want = per_head(p, (np.float64, ap.bf16_rounded), (np.float64, ap.formulas))
     got = {**p.forward(), **p.backward()}
     assert not ap.as_exact_as_bf16(got, model, want)
+    p.op.close()
+
+
+@pytest.mark.parametrize("counts,earlier,heads,causal", [
+    ([1, 2, 3, 5, 32, 17], 0, (8, 2, 64), True), ([2], 0, (32, 4, 64), True), ([2, 2], 0, (8, 8, 64), False), ([2], 0, (24, 2, 128), True), ([2, 3], [160, 300], (5, 5, 40), True),
+    ([300, 90], [-290, -70], (4, 2, 64), False), ([2, 30, 7] * 30, 0, (16, 16, 104), True), ([3] * 70, 40, (16, 8, 64), True)])
+def test_gradients_of_short_bf16_sequences_are_rounded_once(device, counts, earlier, heads, causal):
+    """p and ds have 16 bits there, 2^8 times as many as a result: what is left is the rounding of the result, but for values within a hundredth of a
+    step of a tie."""
+    p = Problem(device, counts, earlier, heads, "bf16", causal)
+    want, = per_head(p, (np.float64, ap.formulas))
+    p.forward()
+    bad = ap.as_exact_as_f32(p.backward(), {n: ap.rounded(a) for n, a in want.items()}, want, 1.05, 2.0 ** -17)
+    assert not bad
     p.op.close()
