@@ -44,6 +44,18 @@ def test_f32_rows_are_as_exact_as_f32(device, counts, earlier, heads, causal):
     p.op.close()
 
 
+@pytest.mark.parametrize("counts,earlier,heads,causal", [
+    ([1] * 30, 0, (4, 4, 64), True), ([2], 0, (8, 8, 64), True), ([2] * 10, 0, (6, 3, 80), False), ([2] * 24, 0, (24, 2, 128), True), ([4] * 24, 0, (6, 3, 80), True),
+    ([1, 2, 3, 5, 9, 17], 0, (8, 2, 64), True), ([8] * 24, 0, (32, 4, 64), True), ([1, 2, 1], [3, 0, 9], (8, 8, 40), True)])
+def test_short_f32_sequences_are_as_exact_as_f32(device, counts, earlier, heads, causal):
+    """Where a key has most of a row's weight the formula in f32 rounds its score as it rounds lse, and p is nearly exact."""
+    p = Problem(device, counts, earlier, heads, "f32", causal)
+    f32, want = per_head(p, (np.float32, ap.formulas), (np.float64, ap.formulas))
+    got = {**p.forward(), **p.backward()}
+    assert not ap.as_exact_as_f32(got, f32, want)
+    p.op.close()
+
+
 @pytest.mark.parametrize("counts,earlier,heads,causal", CASES)
 def test_bf16_rows_lose_what_rounding_costs(device, counts, earlier, heads, causal):
     p = Problem(device, counts, earlier, heads, "bf16", causal)
