@@ -32,7 +32,7 @@
 //     registers leave one wave a SIMD, which waits for its exponentials.
 //   short or ragged calls: the longest rows' workgroups; f32 rows: 6 products for one, and cutting p and ds in parts.  (Parts rounded to nearest, small
 //     products and blocks summed apart: errors of 1.1 to 1.5e-7 of the result forward, 3.3 to 5e-7 of the gradients, where f32 products by the library have
-//     2 to 6e-7 and 5e-7 to 1.5e-6.  6 x 2048 rows of 8 heads of 64 117 us, as before with parts cut off; backward of 3 x 700 72 for 67.  Heads of 128: 4096
+//     2 to 6e-7 and 5e-7 to 1.5e-6.  6 x 2048 rows of 8 heads of 64 117 us, as before with parts cut off; backward of 3 x 700 70 for 67.  Heads of 128: 4096
 //     rows of 16 heads 457 us, 150 TFLOP/s.)
 #include "attention_kernels.h"
 
